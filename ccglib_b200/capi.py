@@ -30,6 +30,9 @@ EXPORTS = [
     "ccglib_b200_pipeline_launches", "ccglib_b200_pipeline_scratch_bytes",
     "ccglib_b200_pipeline_set_gemm_events", "ccglib_b200_pipeline_set_overlap",
     "ccglib_b200_pipeline_destroy",
+    "ccglib_b200_quantize_run", "ccglib_b200_scaled_gemm_plan_create",
+    "ccglib_b200_scaled_gemm_run", "ccglib_b200_scaled_gemm_plan_destroy",
+    "ccglib_b200_scaled_gemm_plan_scratch_bytes", "ccglib_b200_scaled_gemm_plan_tile",
 ]
 
 
@@ -51,6 +54,23 @@ class PipelineDesc(ctypes.Structure):
                 ("b_mem_order", ctypes.c_int), ("c_mem_order", ctypes.c_int),
                 ("alpha_re", ctypes.c_float), ("alpha_im", ctypes.c_float),
                 ("beta_re", ctypes.c_float), ("beta_im", ctypes.c_float)]
+
+
+class QuantizeDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_size_t), ("rows", ctypes.c_size_t), ("k", ctypes.c_size_t),
+                ("type_in", ctypes.c_int), ("type_out", ctypes.c_int),
+                ("input_complex_axis", ctypes.c_int), ("input_mem_order", ctypes.c_int),
+                ("block_rows", ctypes.c_size_t)]
+
+
+class ScaledGemmDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_size_t), ("m", ctypes.c_size_t), ("n", ctypes.c_size_t),
+                ("k", ctypes.c_size_t), ("type_a", ctypes.c_int), ("type_b", ctypes.c_int),
+                ("type_out", ctypes.c_int), ("a_block_rows", ctypes.c_size_t),
+                ("b_block_rows", ctypes.c_size_t), ("c_complex_axis", ctypes.c_int),
+                ("c_mem_order", ctypes.c_int), ("alpha_re", ctypes.c_float),
+                ("alpha_im", ctypes.c_float), ("beta_re", ctypes.c_float),
+                ("beta_im", ctypes.c_float)]
 
 
 class Share(ctypes.Structure):
@@ -133,6 +153,19 @@ def lib() -> ctypes.CDLL:
         L.ccglib_b200_pipeline_scratch_bytes.restype = sz
         L.ccglib_b200_pipeline_destroy.argtypes = [vp]
         L.ccglib_b200_pipeline_destroy.restype = ci
+        L.ccglib_b200_quantize_run.argtypes = [ctypes.POINTER(QuantizeDesc), vp, vp, vp, vp]
+        L.ccglib_b200_quantize_run.restype = ci
+        L.ccglib_b200_scaled_gemm_plan_create.argtypes = [ctypes.POINTER(ScaledGemmDesc),
+                                                          ctypes.POINTER(vp)]
+        L.ccglib_b200_scaled_gemm_plan_create.restype = ci
+        L.ccglib_b200_scaled_gemm_run.argtypes = [vp, vp, vp, vp, vp, vp, vp]
+        L.ccglib_b200_scaled_gemm_run.restype = ci
+        L.ccglib_b200_scaled_gemm_plan_destroy.argtypes = [vp]
+        L.ccglib_b200_scaled_gemm_plan_destroy.restype = ci
+        L.ccglib_b200_scaled_gemm_plan_scratch_bytes.argtypes = [vp]
+        L.ccglib_b200_scaled_gemm_plan_scratch_bytes.restype = sz
+        L.ccglib_b200_scaled_gemm_plan_tile.argtypes = [vp, ctypes.POINTER(ci * 3)]
+        L.ccglib_b200_scaled_gemm_plan_tile.restype = ci
         L.ccglib_b200_status_string.argtypes = [ci]
         L.ccglib_b200_status_string.restype = ctypes.c_char_p
         L.ccglib_b200_last_error.argtypes = []
@@ -188,6 +221,46 @@ class GemmPlan:
     def close(self) -> None:
         if self._plan:
             lib().ccglib_b200_gemm_plan_destroy(self._plan)
+            self._plan = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class ScaledGemmPlan:
+    """Owns a ccglib_b200_scaled_gemm_plan: fp8 operands with one float32 scale per block of 128 k."""
+
+    def __init__(self, batch, m, n, k, type_a, type_b, type_out, a_block_rows=1, b_block_rows=128,
+                 c_complex_axis=PLANAR, c_mem_order=ROW_MAJOR, alpha=(1.0, 0.0), beta=(0.0, 0.0)):
+        self.desc = ScaledGemmDesc(batch, m, n, k, type_a, type_b, type_out, a_block_rows,
+                                   b_block_rows, c_complex_axis, c_mem_order, alpha[0], alpha[1],
+                                   beta[0], beta[1])
+        self._plan = ctypes.c_void_p()
+        _check(lib().ccglib_b200_scaled_gemm_plan_create(ctypes.byref(self.desc),
+                                                         ctypes.byref(self._plan)))
+
+    @property
+    def scratch_bytes(self) -> int:
+        return int(lib().ccglib_b200_scaled_gemm_plan_scratch_bytes(self._plan))
+
+    @property
+    def tile(self) -> dict:
+        """Columns per 128-row tile, whether B is the row side, CTAs that share blocks (0: none)."""
+        t = (ctypes.c_int * 3)()
+        _check(lib().ccglib_b200_scaled_gemm_plan_tile(self._plan, ctypes.byref(t)))
+        return {"bn": int(t[0]), "swapped": bool(t[1]), "runs": int(t[2])}
+
+    def run(self, d_a: int, d_a_scale: int, d_b: int, d_b_scale: int, d_c: int,
+            stream: int = 0) -> None:
+        _check(lib().ccglib_b200_scaled_gemm_run(self._plan, d_a, d_a_scale, d_b, d_b_scale, d_c,
+                                                 stream))
+
+    def close(self) -> None:
+        if self._plan:
+            lib().ccglib_b200_scaled_gemm_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
 
     def __del__(self):
@@ -295,6 +368,20 @@ def transpose(batch, m, n, m_chunk, n_chunk, nr_bits, input_complex_axis, d_in, 
 
 def pack(n, direction, input_complex_axis, d_in, d_out, stream: int = 0) -> None:
     _check(lib().ccglib_b200_pack_run(n, direction, input_complex_axis, d_in, d_out, stream))
+
+
+def quantize(batch, rows, k, type_in, type_out, d_in, d_out, d_scale, stream: int = 0,
+             input_complex_axis=PLANAR, input_mem_order=ROW_MAJOR, block_rows=1) -> None:
+    """Complex float matrices -> fp8 planes [batch][2][rows][pitch] and block scales
+    [batch][ceil(k / 128)][ceil(rows / block_rows)] (see include/ccglib_b200.h)."""
+    desc = QuantizeDesc(batch, rows, k, type_in, type_out, input_complex_axis, input_mem_order,
+                        block_rows)
+    _check(lib().ccglib_b200_quantize_run(ctypes.byref(desc), d_in, d_out, d_scale, stream))
+
+
+def operand_pitch(k: int) -> int:
+    """Bytes of one row of a quantised operand."""
+    return -(-k // 16) * 16
 
 
 def selftest_wait_timeout(limit_cycles: int, pair: bool = False) -> tuple[int, int]:

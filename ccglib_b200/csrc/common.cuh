@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstdio>
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "../../include/ccglib_b200.h"
@@ -41,6 +42,18 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 // Number of SMs of the current device (cached per device ordinal).
 int sm_count();
+
+// Device address of the sticky status word of the current device.
+int device_status_address(unsigned int **out);
+
+// Limit of the device-side waits in SM clock cycles (see gemm.cu).
+long long wait_limit_cycles();
+
+// Byte-typed 3-D tensor map: dims (row bytes, rows, slices), box (sw bytes, box_rows, box_slices),
+// sw = 64 or 128 with the matching swizzle.
+int make_map(CUtensorMap *tm, const void *base, uint64_t row_bytes, uint64_t rows, uint64_t slices,
+             uint64_t row_pitch, uint64_t slice_pitch, uint32_t sw, uint32_t box_rows,
+             uint32_t box_slices);
 
 // Launchers implemented in the individual .cu files (host side, no extern "C").
 int launch_expand_bits(const void *d_in, void *d_out, size_t batch, size_t rows, size_t k_bits,

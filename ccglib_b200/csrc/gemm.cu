@@ -15,6 +15,16 @@
 
 namespace ccglib_b200 {
 
+// Sticky device-side status word: kernels OR a code into it when a bounded wait gives up.
+__device__ unsigned int g_device_status = 0;
+
+int device_status_address(unsigned int **out) {
+  if (cudaGetSymbolAddress(reinterpret_cast<void **>(out), g_device_status) != cudaSuccess) {
+    return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(g_device_status)");
+  }
+  return CCGLIB_B200_OK;
+}
+
 namespace {
 
 using namespace ptx;
@@ -40,6 +50,8 @@ EncodeTiledFn get_encode_fn() {
   }
   return fn;
 }
+
+} // namespace
 
 // Byte-typed 3-D tensor map: dims (row bytes, rows, slices), box (sw bytes, box_rows, box_slices).
 int make_map(CUtensorMap *tm, const void *base, uint64_t row_bytes, uint64_t rows, uint64_t slices,
@@ -69,6 +81,16 @@ int make_map(CUtensorMap *tm, const void *base, uint64_t row_bytes, uint64_t row
   }
   return CCGLIB_B200_OK;
 }
+
+// Limit of the device-side waits in SM clock cycles: CCGLIB_B200_WAIT_CYCLES, else about two
+// seconds.  Never unbounded: values below 1 fall back to the default.
+long long wait_limit_cycles() {
+  const char *v = std::getenv("CCGLIB_B200_WAIT_CYCLES");
+  const long long n = (v != nullptr && *v != '\0') ? std::atoll(v) : 0;
+  return n > 0 ? n : kWaitLimitCycles;
+}
+
+namespace {
 
 using KernelFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
                           const GemmParams);
@@ -136,14 +158,6 @@ template <int KIND> KernelEntry pick_float_out(int type_out, int bn, int sw, boo
 int env_int(const char *name, int fallback) {
   const char *v = std::getenv(name);
   return (v != nullptr && *v != '\0') ? std::atoi(v) : fallback;
-}
-
-// Limit of the device-side waits in SM clock cycles: CCGLIB_B200_WAIT_CYCLES, else about two
-// seconds.  Never unbounded: values below 1 fall back to the default.
-long long wait_limit_cycles() {
-  const char *v = std::getenv("CCGLIB_B200_WAIT_CYCLES");
-  const long long n = (v != nullptr && *v != '\0') ? std::atoll(v) : 0;
-  return n > 0 ? n : kWaitLimitCycles;
 }
 
 size_t type_bits(int t) {
@@ -791,10 +805,9 @@ int launch_gemm(const ccglib_b200_gemm_plan &plan, const void *a, const void *b,
     plan.map_c = c;
     plan.map_nb = nb;
   }
-  if (plan.status_ptr == nullptr &&
-      cudaGetSymbolAddress(reinterpret_cast<void **>(&plan.status_ptr), g_device_status) !=
-          cudaSuccess) {
-    return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(g_device_status)");
+  if (plan.status_ptr == nullptr) {
+    rc = device_status_address(&plan.status_ptr);
+    if (rc != CCGLIB_B200_OK) return rc;
   }
   p.status = plan.status_ptr;
   p.wait_cycles = plan.wait_cycles;
@@ -1050,7 +1063,8 @@ extern "C" int ccglib_b200_selftest_wait_timeout(long long limit_cycles, int pai
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
   unsigned int *status = nullptr;
-  CCGLIB_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void **>(&status), g_device_status));
+  const int rc = device_status_address(&status);
+  if (rc != CCGLIB_B200_OK) return rc;
   const long long other_limit = 200 * limit_cycles;  // bounded as well: at most 2e9 cycles
   if (pair != 0) {
     cudaLaunchConfig_t cfg{};

@@ -1,6 +1,7 @@
 // Device side of the batched complex GEMM for sm_100a: kernel parameters, shared-memory
 // geometry, the epilogue, and the two kernels (one CTA per tile; a cluster of two CTAs per tile).
-// Included by gemm.cu only, which instantiates the kernels and owns the host-side plan.
+// gemm.cu instantiates the kernels and owns the host-side plan; scaled_gemm.cu uses the wait, the
+// tile walk and the output helpers.
 //
 // One persistent CTA per SM, warp-specialised:
 //   warp 0      TMA producer   -- stages [planes][rows][SW bytes] tiles of A and B in swizzled
@@ -31,15 +32,12 @@
 
 namespace ccglib_b200 {
 
-// Sticky device-side status word: kernels OR a code into it when a bounded wait gives up.
-__device__ unsigned int g_device_status = 0;
-
 #ifdef CCGLIB_B200_TRACE
 // Instrumented builds only (-DCCGLIB_B200_TRACE; never in the shipped library): SM clock stamps of
 // the first tiles of every CTA of cgemm_tcgen05_kernel: [0] tile start at the MMA issuer,
 // [1] last MMA issued, [2] accumulator complete at the epilogue, [3] epilogue done.
 constexpr int kTraceTiles = 48;
-__device__ long long g_trace[160][kTraceTiles][4];
+static __device__ long long g_trace[160][kTraceTiles][4];
 #define CCGLIB_TRACE(iter, slot)                                                         \
   do {                                                                                   \
     if ((iter) < kTraceTiles && blockIdx.x < 160) g_trace[blockIdx.x][(iter)][(slot)] = clock64(); \
@@ -79,6 +77,7 @@ struct GemmParams {
   void *c;
   uint32_t c_layout;
   uint32_t have_alpha, have_beta, vec_ok;
+  uint32_t pair_ok;  // scaled GEMM: (re, im) of an interleaved C may be stored as one word
   uint32_t epi_tma;  // stage C through shared memory and store it with TMA (row-major, 4-byte)
   uint32_t prefetch;  // k-blocks the producer asks L2 to fetch ahead of its own loads (0 = off)
   float alpha_re, alpha_im, beta_re, beta_im;

@@ -156,6 +156,88 @@ CCGLIB_B200_API int ccglib_b200_pack_run(size_t n, int direction, int input_comp
                          void *d_out, void *stream);
 
 /*
+ * Block quantiser: float16 / bfloat16 / float32 complex matrices -> fp8 planes with one float32 scale
+ * per block, the operands of the scaled GEMM below.  No counterpart in the reference.
+ *
+ * Input, `rows` x `k` complex samples per batch item, dense, 16-byte aligned:
+ *   row-major: planar [batch][2][rows][k], interleaved [batch][rows][k][2]
+ *   col-major: planar [batch][2][k][rows], interleaved [batch][k][rows][2]; the quantised matrix is
+ *              the transposed one, so the same data can be contracted over either axis
+ * Output: fp8 planes [batch][2][rows][pitch], pitch = k rounded up to a multiple of 16, the bytes
+ *   behind k written as zeros; scales [batch][ceil(k / 128)][ceil(rows / block_rows)] float32.
+ * A block is block_rows (1 or 128) rows x 128 k, both planes together:
+ *   amax = max(|re|, |im|) over its finite entries,  scale = max(amax / FMAX, 2^-126),
+ *   q = x * (1 / scale) rounded to nearest even, FMAX = 448 (e4m3) or 57344 (e5m2),
+ * in float32.  NaN stays NaN; an infinity becomes an infinity in e5m2 and NaN in e4m3.
+ * Asynchronous on `stream`, one launch, no scratch.
+ */
+typedef struct ccglib_b200_quantize_desc {
+  size_t batch;
+  size_t rows;
+  size_t k;
+  int type_in;            /* FLOAT16, BFLOAT16 or FLOAT32 */
+  int type_out;           /* FLOAT8E4M3 or FLOAT8E5M2 */
+  int input_complex_axis; /* CCGLIB_B200_PLANAR / CCGLIB_B200_INTERLEAVED */
+  int input_mem_order;    /* CCGLIB_B200_ROW_MAJOR (k contiguous) / CCGLIB_B200_COL_MAJOR */
+  size_t block_rows;      /* 1 or 128 */
+} ccglib_b200_quantize_desc;
+
+CCGLIB_B200_API int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *desc, const void *d_in,
+                                             void *d_out, float *d_scale, void *stream);
+
+/*
+ * Block-scaled fp8 complex GEMM:
+ *   C[b][m][n] = alpha * sum_g sA[b][g][m / a_block_rows] * sB[b][g][n / b_block_rows]
+ *                             * sum_{k in block g} A[b][m][k] * B[b][n][k]   + beta * C[b][m][n]
+ * with blocks of 128 k.  A is [batch][2][M][pitch], B [batch][2][N][pitch] fp8 bytes (16-byte
+ * aligned, pitch = K rounded up to a multiple of 16, bytes behind K never read), scales float32
+ * [batch][ceil(K / 128)][ceil(rows / block_rows)]: what ccglib_b200_quantize_run writes; for K a
+ * multiple of 16 the planes are plain dense arrays.  A and B may have different fp8 types.
+ * C in any of the four layouts of the GEMM above, float32, float16 or bfloat16; sums are float32 and
+ * rounded once.  With beta = 0 C is not read.  Results do not depend on timing: the same call gives
+ * the same bits.  No counterpart in the reference, whose fp8 GEMM takes unscaled values.
+ */
+typedef struct ccglib_b200_scaled_gemm_desc {
+  size_t batch;
+  size_t m;
+  size_t n;
+  size_t k;
+  int type_a; /* FLOAT8E4M3 or FLOAT8E5M2 */
+  int type_b;
+  int type_out; /* FLOAT32, FLOAT16 or BFLOAT16 */
+  size_t a_block_rows; /* rows of A per scale: 1 or 128 */
+  size_t b_block_rows;
+  int c_complex_axis;
+  int c_mem_order;
+  float alpha_re, alpha_im;
+  float beta_re, beta_im;
+} ccglib_b200_scaled_gemm_desc;
+
+typedef struct ccglib_b200_scaled_gemm_plan ccglib_b200_scaled_gemm_plan;
+
+/* Validates, chooses the tile and, where the blocks of a tile are shared between CTAs, allocates
+ * the workspace that holds their partial sums (and waits for it to be cleared).  The plan belongs to
+ * the device that is current here; running it with another one current is an error. */
+CCGLIB_B200_API int ccglib_b200_scaled_gemm_plan_create(const ccglib_b200_scaled_gemm_desc *desc,
+                                                        ccglib_b200_scaled_gemm_plan **plan);
+
+/* Enqueues one launch on `stream`; no allocation, no synchronisation; may be captured into a graph.
+ * Runs of one plan (replays of graphs that hold one included) must not overlap: they share its
+ * workspace.  Plans are independent of each other. */
+CCGLIB_B200_API int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, const void *d_a,
+                                                const float *d_a_scale, const void *d_b,
+                                                const float *d_b_scale, void *d_c, void *stream);
+
+CCGLIB_B200_API int ccglib_b200_scaled_gemm_plan_destroy(ccglib_b200_scaled_gemm_plan *plan);
+
+/* Introspection: device bytes the plan owns; tile = {columns per 128-row tile, 1 if the 128 rows are
+ * rows of B, CTAs that share all blocks in equal runs (0: whole tiles)}. */
+CCGLIB_B200_API size_t
+ccglib_b200_scaled_gemm_plan_scratch_bytes(const ccglib_b200_scaled_gemm_plan *plan);
+CCGLIB_B200_API int ccglib_b200_scaled_gemm_plan_tile(const ccglib_b200_scaled_gemm_plan *plan,
+                                                      int tile[3]);
+
+/*
  * The Pipeline: the caller's matrices in their natural layout -> C, as one object that owns the
  * intermediate buffers.  Replaces ccglib::pipeline::Pipeline (reference
  * include/ccglib/pipeline/pipeline.h:28-73, src/pipeline/Pipeline.cpp:44-188), whose chain is
