@@ -28,7 +28,12 @@ namespace ccglib_b200 {
 namespace {
 
 constexpr int kEpiWarps = 8;
-constexpr int kScaledThreads = 64 + 32 * kEpiWarps;
+constexpr int kFirstEpiWarp = 4;  // warps 2 and 3 only complete the first warpgroup
+constexpr int kScaledThreads = 32 * (kFirstEpiWarp + kEpiWarps);
+// Registers: 384 threads start with 168 each (64512 in all); the first warpgroup hands back all but 40,
+// the two epilogue warpgroups take 232: 128 * 40 + 256 * 232 = 64512.
+constexpr int kRegsFirst = 40, kRegsEpi = 232;
+static_assert(128 * kRegsFirst + 32 * kEpiWarps * kRegsEpi <= kScaledThreads * 168, "register split");
 constexpr int kBlockK = 128;
 constexpr int kAccBuffers = 2;
 
@@ -124,6 +129,13 @@ __device__ __forceinline__ void fma2(float &acc0, float &acc1, uint32_t d0, uint
       : "r"(d0), "r"(d1), "f"(s), "f"(t0), "f"(t1));
 }
 
+template <int N> __device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 template <int N> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t *r);
 template <> __device__ __forceinline__ void tmem_ld_cols<8>(uint32_t taddr, uint32_t *r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -141,6 +153,25 @@ template <> __device__ __forceinline__ void tmem_ld_cols<16>(uint32_t taddr, uin
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+
+// Wait for this warp's tensor-memory loads; the values are operands, so nothing that uses them can be
+// scheduled ahead of the wait.
+template <int N> __device__ __forceinline__ void tmem_wait_cols(uint32_t *r);
+template <> __device__ __forceinline__ void tmem_wait_cols<8>(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+template <> __device__ __forceinline__ void tmem_wait_cols<16>(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
@@ -339,6 +370,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  if (warp < kFirstEpiWarp) {
+  regs_dec<kRegsFirst>();
   Walk walk(p);
   Segment seg;
   if (warp == 0) {
@@ -426,12 +459,16 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         }
       }
     }
+  }
   } else {
     // ------------------------------------------------------------------ epilogue warps
-    const uint32_t quad = warp & 3;         // tensor-memory lanes of this warp
-    const uint32_t half = (warp - 2) >> 2;  // which half of the columns
+    regs_inc<kRegsEpi>();
+    Walk walk(p);
+    Segment seg;
+    const uint32_t quad = warp & 3;                     // tensor-memory lanes of this warp
+    const uint32_t half = (warp - kFirstEpiWarp) >> 2;  // which half of the columns
     const uint32_t staging =
-        smem_base + kStages * C::kStageBytes + (warp - 2) * kStagingTile;
+        smem_base + kStages * C::kStageBytes + (warp - kFirstEpiWarp) * kStagingTile;
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
     float re[HALF], im[HALF];
@@ -476,14 +513,20 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         __syncwarp();  // the column scales are in place
         tc_fence_after();
         const uint32_t t_re = tmem_base + ((quad * 32) << 16) + acc * (2 * BN) + half * HALF;
+        // 16 columns of both planes at a time, the next ones on their way while these are added
         constexpr int kCols = HALF < 16 ? HALF : 16;
+        uint32_t dr[2][kCols], di[2][kCols];
+        tmem_ld_cols<kCols>(t_re, dr[0]);
+        tmem_ld_cols<kCols>(t_re + BN, di[0]);
 #pragma unroll
         for (int c = 0; c < HALF; c += kCols) {
-          uint32_t dr[kCols], di[kCols];
-          tmem_ld_cols<kCols>(t_re + c, dr);
-          tmem_ld_cols<kCols>(t_re + BN + c, di);
-          tmem_wait_ld();
-          if (c + kCols == HALF) {
+          const int now = (c / kCols) & 1;
+          tmem_wait_cols<kCols>(dr[now]);
+          tmem_wait_cols<kCols>(di[now]);
+          if (c + kCols < HALF) {
+            tmem_ld_cols<kCols>(t_re + c + kCols, dr[now ^ 1]);
+            tmem_ld_cols<kCols>(t_re + BN + c + kCols, di[now ^ 1]);
+          } else {
             // the buffer is read: the next block's MMAs may fill it
             tc_fence_before();
             __syncwarp();
@@ -492,10 +535,10 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
 #pragma unroll
           for (int j = 0; j < kCols; j += 4) {
             const float4 f = ld_shared_f4(cols + (c + j) * 4);
-            fma2(re[c + j], re[c + j + 1], dr[j], dr[j + 1], s, f.x, f.y);
-            fma2(im[c + j], im[c + j + 1], di[j], di[j + 1], s, f.x, f.y);
-            fma2(re[c + j + 2], re[c + j + 3], dr[j + 2], dr[j + 3], s, f.z, f.w);
-            fma2(im[c + j + 2], im[c + j + 3], di[j + 2], di[j + 3], s, f.z, f.w);
+            fma2(re[c + j], re[c + j + 1], dr[now][j], dr[now][j + 1], s, f.x, f.y);
+            fma2(im[c + j], im[c + j + 1], di[now][j], di[now][j + 1], s, f.x, f.y);
+            fma2(re[c + j + 2], re[c + j + 3], dr[now][j + 2], dr[now][j + 3], s, f.z, f.w);
+            fma2(im[c + j + 2], im[c + j + 3], di[now][j + 2], di[now][j + 3], s, f.z, f.w);
           }
         }
         if (++acc == kAccBuffers) {
@@ -520,7 +563,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         }
         __threadfence();
         epi_sync();
-        if (threadIdx.x == 64) {
+        if (threadIdx.x == 32 * kFirstEpiWarp) {
           const unsigned add = seg.k1 - seg.k0;
           const unsigned before = atomicAdd(p.counters + seg.tile, add);
           const bool last = before + add == p.g.k_blocks;
