@@ -59,7 +59,13 @@ template <int BN> struct ScaledCfg {
   static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarrierBytes + 1024;
   static constexpr int kHalf = BN / 2;  // columns of one epilogue warp
   static_assert(kStages >= 2, "need at least two stages");
-  static_assert(2 * BN * kAccBuffers <= kTmemCols, "accumulators exceed tensor memory");
+  // Up to 64 columns one MMA multiplies an A plane by both B planes, which lie one behind the other in
+  // the stage: columns [Ar.Br | Ar.Bi] and [Ai.Br | Ai.Bi], added up on the way out of tensor
+  // memory.  An MMA of 128 rows costs the same for 64 columns as for 128, so this halves the tensor
+  // time of narrow tiles; at 128 columns there is no tensor memory for it.
+  static constexpr bool kStacked = BN <= 64;
+  static constexpr int kAccCols = kStacked ? 4 * BN : 2 * BN;
+  static_assert(kAccCols * kAccBuffers <= kTmemCols, "accumulators exceed tensor memory");
   static_assert(BN % 16 == 0 && BN >= 16 && BN <= 128, "tile width");
 };
 
@@ -117,16 +123,38 @@ __device__ __forceinline__ void epi_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
 }
 
-// acc += (d * s) * t on two neighbouring columns.
-__device__ __forceinline__ void fma2(float &acc0, float &acc1, uint32_t d0, uint32_t d1, float s,
-                                     float t0, float t1) {
-  asm("{\n\t.reg .b64 d, s, t, a;\n\t"
-      "mov.b64 d, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 t, {%5, %6};\n\t"
-      "mov.b64 a, {%0, %1};\n\t"
-      "mul.rn.f32x2 d, d, s;\n\tfma.rn.f32x2 a, d, t, a;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(acc0), "+f"(acc1)
-      : "r"(d0), "r"(d1), "f"(s), "f"(t0), "f"(t1));
+// Two neighbouring columns as one register pair.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ f32x2 pair_of(uint32_t lo, uint32_t hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void split_pair(f32x2 v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+// acc += (d * s) * t.  In this order nothing overflows or vanishes that the scaled sum itself does not:
+// s * t alone may leave float32 where d is zero or large.
+__device__ __forceinline__ void scale_add(f32x2 &acc, f32x2 d, f32x2 s, f32x2 t) {
+  asm("{\n\t.reg .b64 v;\n\tmul.rn.f32x2 v, %1, %2;\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}"
+      : "+l"(acc)
+      : "l"(d), "l"(s), "l"(t));
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 template <int N> __device__ __forceinline__ void regs_inc() {
@@ -172,12 +200,6 @@ template <> __device__ __forceinline__ void tmem_wait_cols<16>(uint32_t *r) {
                  "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
-}
-
-__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
-  uint32_t a, b, c, d;
-  ld_shared_v4(addr, a, b, c, d);
-  return make_float4(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c), __uint_as_float(d));
 }
 
 // alpha and beta on the sums of row m, columns n0 .. n0 + HALF.
@@ -433,17 +455,22 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         if (lane == 0) {
           const uint32_t a_base = smem_base + stage * C::kStageBytes;
           const uint32_t b_base = a_base + C::kABytes;
-          const uint32_t d_re = tmem_base + acc * (2 * BN), d_im = d_re + BN;
+          const uint32_t d = tmem_base + acc * C::kAccCols;
 #pragma unroll
           for (int k = 0; k < kBlockK / 32; ++k) {
             const uint64_t a_re = smem_desc<128>(a_base + k * 32);
             const uint64_t a_im = smem_desc<128>(a_base + C::kAPlane + k * 32);
             const uint64_t b_re = smem_desc<128>(b_base + k * 32);
-            const uint64_t b_im = smem_desc<128>(b_base + C::kBPlane + k * 32);
-            tc_mma<kKindF8F6F4>(d_re, a_re, b_re, p.g.idesc, k != 0);
-            tc_mma<kKindF8F6F4>(d_im, a_re, b_im, p.g.idesc, k != 0);
-            tc_mma<kKindF8F6F4>(d_im, a_im, b_re, p.g.idesc, 1u);
-            tc_mma<kKindF8F6F4>(d_re, a_im, b_im, p.g.idesc_neg_a, 1u);
+            if constexpr (C::kStacked) {
+              tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
+              tc_mma<kKindF8F6F4>(d + 2 * BN, a_im, b_re, p.g.idesc, k != 0);
+            } else {
+              const uint64_t b_im = smem_desc<128>(b_base + C::kBPlane + k * 32);
+              tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
+              tc_mma<kKindF8F6F4>(d + BN, a_re, b_im, p.g.idesc, k != 0);
+              tc_mma<kKindF8F6F4>(d + BN, a_im, b_re, p.g.idesc, 1u);
+              tc_mma<kKindF8F6F4>(d, a_im, b_im, p.g.idesc_neg_a, 1u);
+            }
           }
           tc_commit(bar_empty + 8 * stage);
           tc_commit(bar_acc_full + 8 * acc);
@@ -469,10 +496,13 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     const uint32_t half = (warp - kFirstEpiWarp) >> 2;  // which half of the columns
     const uint32_t staging =
         smem_base + kStages * C::kStageBytes + (warp - kFirstEpiWarp) * kStagingTile;
+    // the column scales of the block (two buffers) at the head of the staging tile
+    f32x2 *col_buf = reinterpret_cast<f32x2 *>(
+        smem + kStages * C::kStageBytes + (warp - kFirstEpiWarp) * kStagingTile);
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
-    float re[HALF], im[HALF];
     while (walk.next(p, seg)) {
+      f32x2 sum[2][HALF / 2];  // Re, Im
       const TileCoord t = decode_tile(p.g, seg.tile);
       const uint32_t m = t.mt * kBlockM + quad * 32 + lane;
       const uint32_t n0 = t.nt * BN + half * HALF;
@@ -487,18 +517,14 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       float t0_next = in0 ? __ldg(cs + i0) : 0.0f;
       float t1_next = in1 ? __ldg(cs + i1) : 0.0f;
 #pragma unroll
-      for (int j = 0; j < HALF; ++j) re[j] = im[j] = 0.0f;
+      for (int j = 0; j < HALF / 2; ++j) sum[0][j] = sum[1][j] = 0;
       // the column scales go through the staging tile: its last store must have read it
       if (lane == 0) bulk_wait_group_read<0>();
       __syncwarp();
       for (uint32_t kb = seg.k0; ok && kb < seg.k1; ++kb) {
-        const float s = s_next;
-        const uint32_t cols = staging + (kb & 1) * (HALF * 4);
-        if (2 * lane < HALF) {
-          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(cols + lane * 8), "f"(t0_next),
-                       "f"(t1_next)
-                       : "memory");
-        }
+        const f32x2 s = pair_of(s_next, s_next);
+        f32x2 *cols = col_buf + (kb & 1) * (HALF / 2);
+        if (2 * lane < HALF) cols[lane] = pair_of(t0_next, t1_next);
         if (kb + 1 < seg.k1) {
           rs += p.row_blocks;
           cs += p.col_blocks;
@@ -506,45 +532,63 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           t0_next = in0 ? __ldg(cs + i0) : 0.0f;
           t1_next = in1 ? __ldg(cs + i1) : 0.0f;
         }
+        __syncwarp();  // the column scales are in place
         ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.g.status,
                        kDevTimeoutEpilogue, p.g.wait_cycles);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
-        __syncwarp();  // the column scales are in place
         tc_fence_after();
-        const uint32_t t_re = tmem_base + ((quad * 32) << 16) + acc * (2 * BN) + half * HALF;
-        // 16 columns of both planes at a time, the next ones on their way while these are added
-        constexpr int kCols = HALF < 16 ? HALF : 16;
-        uint32_t dr[2][kCols], di[2][kCols];
-        tmem_ld_cols<kCols>(t_re, dr[0]);
-        tmem_ld_cols<kCols>(t_re + BN, di[0]);
+        const uint32_t taddr =
+            tmem_base + ((quad * 32) << 16) + acc * C::kAccCols + half * HALF;
+        // kCols columns of every accumulator at a time, the next ones on their way while these are added
+        constexpr int kCols = HALF < 16 || C::kStacked ? 8 : 16;
+        constexpr int kAccs = C::kStacked ? 4 : 2;
+        uint32_t d[2][kAccs][kCols];
+#pragma unroll
+        for (int i = 0; i < kAccs; ++i) tmem_ld_cols<kCols>(taddr + i * BN, d[0][i]);
 #pragma unroll
         for (int c = 0; c < HALF; c += kCols) {
           const int now = (c / kCols) & 1;
-          tmem_wait_cols<kCols>(dr[now]);
-          tmem_wait_cols<kCols>(di[now]);
+#pragma unroll
+          for (int i = 0; i < kAccs; ++i) tmem_wait_cols<kCols>(d[now][i]);
           if (c + kCols < HALF) {
-            tmem_ld_cols<kCols>(t_re + c + kCols, dr[now ^ 1]);
-            tmem_ld_cols<kCols>(t_re + BN + c + kCols, di[now ^ 1]);
+#pragma unroll
+            for (int i = 0; i < kAccs; ++i) {
+              tmem_ld_cols<kCols>(taddr + i * BN + c + kCols, d[now ^ 1][i]);
+            }
           } else {
-            // the buffer is read: the next block's MMAs may fill it
+            // the buffer is read: the MMAs of the block after next may fill it
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
           }
 #pragma unroll
           for (int j = 0; j < kCols; j += 4) {
-            const float4 f = ld_shared_f4(cols + (c + j) * 4);
-            fma2(re[c + j], re[c + j + 1], dr[now][j], dr[now][j + 1], s, f.x, f.y);
-            fma2(im[c + j], im[c + j + 1], di[now][j], di[now][j + 1], s, f.x, f.y);
-            fma2(re[c + j + 2], re[c + j + 3], dr[now][j + 2], dr[now][j + 3], s, f.z, f.w);
-            fma2(im[c + j + 2], im[c + j + 3], di[now][j + 2], di[now][j + 3], s, f.z, f.w);
+            const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(cols + (c + j) / 2);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int e = j + 2 * h;
+              f32x2 v_re = pair_of(d[now][0][e], d[now][0][e + 1]);
+              f32x2 v_im = pair_of(d[now][1][e], d[now][1][e + 1]);
+              if constexpr (C::kStacked) {
+                v_re = sub2(v_re, pair_of(d[now][3][e], d[now][3][e + 1]));
+                v_im = add2(v_im, pair_of(d[now][2][e], d[now][2][e + 1]));
+              }
+              scale_add(sum[0][(c + e) / 2], v_re, s, h == 0 ? t.x : t.y);
+              scale_add(sum[1][(c + e) / 2], v_im, s, h == 0 ? t.x : t.y);
+            }
           }
         }
         if (++acc == kAccBuffers) {
           acc = 0;
           acc_phase ^= 1;
         }
+      }
+      float re[HALF], im[HALF];
+#pragma unroll
+      for (int j = 0; j < HALF / 2; ++j) {
+        split_pair(sum[0][j], re[2 * j], re[2 * j + 1]);
+        split_pair(sum[1][j], im[2 * j], im[2 * j + 1]);
       }
       bool finish = ok;
       if (seg.k1 - seg.k0 < p.g.k_blocks) {
@@ -814,10 +858,11 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
   g.num_tiles = static_cast<uint32_t>(plan->tiles);
   const int row_type = plan->swapped ? d.type_b : d.type_a;
   const int col_type = plan->swapped ? d.type_a : d.type_b;
+  const int mma_n = plan->bn <= 64 ? 2 * plan->bn : plan->bn;
   // instruction descriptor: fp32 accumulator, operand formats (0 e4m3, 1 e5m2), N >> 3, M >> 4
   g.idesc = (1u << 4) | ((row_type == CCGLIB_B200_FLOAT8E5M2 ? 1u : 0u) << 7) |
             ((col_type == CCGLIB_B200_FLOAT8E5M2 ? 1u : 0u) << 10) |
-            (static_cast<uint32_t>(plan->bn >> 3) << 17) | (static_cast<uint32_t>(kBlockM >> 4) << 24);
+            (static_cast<uint32_t>(mma_n >> 3) << 17) | (static_cast<uint32_t>(kBlockM >> 4) << 24);
   g.idesc_neg_a = g.idesc | (1u << 13);
   g.c = d_c;
   // C^T of the swapped product in one order is C in the other
