@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libccglib_b200.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 SOURCES = ["gemm.cu", "pipeline.cu", "staging.cu", "transpose.cu", "packing.cu", "capi.cu",
-           "quantize.cu", "scaled_gemm.cu"]
+           "quantize.cu", "scaled_gemm.cu", "orthogonalize.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 

@@ -33,6 +33,8 @@ EXPORTS = [
     "ccglib_b200_quantize_run", "ccglib_b200_scaled_gemm_plan_create",
     "ccglib_b200_scaled_gemm_run", "ccglib_b200_scaled_gemm_plan_destroy",
     "ccglib_b200_scaled_gemm_plan_scratch_bytes", "ccglib_b200_scaled_gemm_plan_tile",
+    "ccglib_b200_orthogonalize_plan_create", "ccglib_b200_orthogonalize_run",
+    "ccglib_b200_orthogonalize_plan_destroy", "ccglib_b200_orthogonalize_plan_scratch_bytes",
 ]
 
 
@@ -71,6 +73,13 @@ class ScaledGemmDesc(ctypes.Structure):
                 ("c_mem_order", ctypes.c_int), ("alpha_re", ctypes.c_float),
                 ("alpha_im", ctypes.c_float), ("beta_re", ctypes.c_float),
                 ("beta_im", ctypes.c_float)]
+
+
+class OrthogonalizeDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_size_t), ("m", ctypes.c_size_t), ("n", ctypes.c_size_t),
+                ("type_in", ctypes.c_int), ("type_out", ctypes.c_int),
+                ("input_complex_axis", ctypes.c_int), ("steps", ctypes.c_int),
+                ("a", ctypes.c_float), ("b", ctypes.c_float), ("c", ctypes.c_float)]
 
 
 class Share(ctypes.Structure):
@@ -166,6 +175,15 @@ def lib() -> ctypes.CDLL:
         L.ccglib_b200_scaled_gemm_plan_scratch_bytes.restype = sz
         L.ccglib_b200_scaled_gemm_plan_tile.argtypes = [vp, ctypes.POINTER(ci * 3)]
         L.ccglib_b200_scaled_gemm_plan_tile.restype = ci
+        L.ccglib_b200_orthogonalize_plan_create.argtypes = [ctypes.POINTER(OrthogonalizeDesc),
+                                                            ctypes.POINTER(vp)]
+        L.ccglib_b200_orthogonalize_plan_create.restype = ci
+        L.ccglib_b200_orthogonalize_run.argtypes = [vp, vp, vp, vp]
+        L.ccglib_b200_orthogonalize_run.restype = ci
+        L.ccglib_b200_orthogonalize_plan_destroy.argtypes = [vp]
+        L.ccglib_b200_orthogonalize_plan_destroy.restype = ci
+        L.ccglib_b200_orthogonalize_plan_scratch_bytes.argtypes = [vp]
+        L.ccglib_b200_orthogonalize_plan_scratch_bytes.restype = sz
         L.ccglib_b200_status_string.argtypes = [ci]
         L.ccglib_b200_status_string.restype = ctypes.c_char_p
         L.ccglib_b200_last_error.argtypes = []
@@ -261,6 +279,36 @@ class ScaledGemmPlan:
     def close(self) -> None:
         if self._plan:
             lib().ccglib_b200_scaled_gemm_plan_destroy(self._plan)
+            self._plan = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class OrthogonalizePlan:
+    """Owns a ccglib_b200_orthogonalize_plan: Newton-Schulz orthogonalisation of M x N matrices."""
+
+    def __init__(self, batch, m, n, type_in, type_out, steps=5,
+                 coefficients=(3.4445, -4.7750, 2.0315), input_complex_axis=PLANAR):
+        self.desc = OrthogonalizeDesc(batch, m, n, type_in, type_out, input_complex_axis, steps,
+                                      *coefficients)
+        self._plan = ctypes.c_void_p()
+        _check(lib().ccglib_b200_orthogonalize_plan_create(ctypes.byref(self.desc),
+                                                           ctypes.byref(self._plan)))
+
+    @property
+    def scratch_bytes(self) -> int:
+        return int(lib().ccglib_b200_orthogonalize_plan_scratch_bytes(self._plan))
+
+    def run(self, d_in: int, d_out: int, stream: int = 0) -> None:
+        _check(lib().ccglib_b200_orthogonalize_run(self._plan, d_in, d_out, stream))
+
+    def close(self) -> None:
+        if self._plan:
+            lib().ccglib_b200_orthogonalize_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
 
     def __del__(self):

@@ -27,15 +27,10 @@
 namespace ccglib_b200 {
 namespace {
 
-constexpr int kEpiWarps = 8;
-constexpr int kFirstEpiWarp = 4;  // warps 2 and 3 only complete the first warpgroup
-constexpr int kScaledThreads = 32 * (kFirstEpiWarp + kEpiWarps);
-// Registers: 384 threads start with 168 each (64512 in all); the first warpgroup hands back all but 40,
-// the two epilogue warpgroups take 232: 128 * 40 + 256 * 232 = 64512.
-constexpr int kRegsFirst = 40, kRegsEpi = 232;
-static_assert(128 * kRegsFirst + 32 * kEpiWarps * kRegsEpi <= kScaledThreads * 168, "register split");
 constexpr int kBlockK = 128;
 constexpr int kAccBuffers = 2;
+constexpr int kStoreBytes = 64;                // bytes of a row in one TMA store
+constexpr int kStoreTile = 32 * kStoreBytes;  // 32 rows of them: an epilogue warp's staging
 
 struct ScaledParams {
   GemmParams g;  // M, N, tiles, layout of C, alpha, beta, waits; row side = tile rows
@@ -52,12 +47,20 @@ template <int BN> struct ScaledCfg {
   static constexpr int kBPlane = BN * kBlockK;
   static constexpr int kABytes = 2 * kAPlane;
   static constexpr int kStageBytes = 2 * kAPlane + 2 * kBPlane;
-  static constexpr int kStagingBytes = kEpiWarps * kStagingTile;
+  // Epilogue warps: four (one per quarter of the lanes) for each half of the columns.
+  static constexpr int kCols = BN / 2;
+  static constexpr int kEpiWarps = 4 * BN / kCols;
+  // 128 sums per thread need a register split: 384 threads start with 168 each (64512 in all); the
+  // first warpgroup (two warps of it idle) hands back all but 40, the others take 232: 128 * 40 +
+  // 256 * 232 = 64512.
+  static constexpr bool kSplitRegs = BN == 128;
+  static constexpr int kFirstEpiWarp = kSplitRegs ? 4 : 2;
+  static constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
+  static constexpr int kStagingBytes = kEpiWarps * kStoreTile;
   static constexpr int kBarrierBytes = 256;
   static constexpr int kRaw = (kMaxSmem - 1024 - kBarrierBytes - kStagingBytes) / kStageBytes;
   static constexpr int kStages = kRaw > 6 ? 6 : kRaw;
   static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarrierBytes + 1024;
-  static constexpr int kHalf = BN / 2;  // columns of one epilogue warp
   static_assert(kStages >= 2, "need at least two stages");
   // Up to 64 columns one MMA multiplies an A plane by both B planes, which lie one behind the other in
   // the stage: columns [Ar.Br | Ar.Bi] and [Ai.Br | Ai.Bi], added up on the way out of tensor
@@ -99,6 +102,12 @@ struct Walk {
     }
     tile = blockIdx.x;
   }
+  // Blocks of the whole list.
+  __device__ __forceinline__ uint64_t blocks(const ScaledParams &p) const {
+    if (runs) return end - at;
+    if (tile >= p.g.num_tiles) return 0;
+    return static_cast<uint64_t>((p.g.num_tiles - 1 - tile) / gridDim.x + 1) * p.g.k_blocks;
+  }
   __device__ __forceinline__ bool next(const ScaledParams &p, Segment &s) {
     if (!runs) {
       if (tile >= p.g.num_tiles) return false;
@@ -119,42 +128,16 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ void epi_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+// Barrier of the epilogue warps.
+template <int THREADS> __device__ __forceinline__ void epi_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
-// Two neighbouring columns as one register pair.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ f32x2 pair_of(uint32_t lo, uint32_t hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ void split_pair(f32x2 v, float &lo, float &hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-// acc += (d * s) * t.  In this order nothing overflows or vanishes that the scaled sum itself does not:
-// s * t alone may leave float32 where d is zero or large.
-__device__ __forceinline__ void scale_add(f32x2 &acc, f32x2 d, f32x2 s, f32x2 t) {
-  asm("{\n\t.reg .b64 v;\n\tmul.rn.f32x2 v, %1, %2;\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}"
-      : "+l"(acc)
-      : "l"(d), "l"(s), "l"(t));
-}
-
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
+// Volatile, so that it stays behind the wait for the tensor-memory load that `a` comes from.  (The packed
+// two-value form of it was slower here: moving values in and out of aligned register pairs took more
+// instructions than it saved.)
+__device__ __forceinline__ void fma_to(float &acc, float a, float b) {
+  asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(a), "f"(b));
 }
 
 template <int N> __device__ __forceinline__ void regs_inc() {
@@ -183,32 +166,72 @@ template <> __device__ __forceinline__ void tmem_ld_cols<16>(uint32_t taddr, uin
       : "memory");
 }
 
-// Wait for this warp's tensor-memory loads; the values are operands, so nothing that uses them can be
-// scheduled ahead of the wait.
-template <int N> __device__ __forceinline__ void tmem_wait_cols(uint32_t *r);
-template <> __device__ __forceinline__ void tmem_wait_cols<8>(uint32_t *r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                 "+r"(r[6]), "+r"(r[7])
-               :
-               : "memory");
-}
-template <> __device__ __forceinline__ void tmem_wait_cols<16>(uint32_t *r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+template <> __device__ __forceinline__ void tmem_ld_cols<32>(uint32_t taddr, uint32_t *r) {
+  tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
 }
 
-// alpha and beta on the sums of row m, columns n0 .. n0 + HALF.
-template <typename OutT, int HALF>
+// How a block's sums are scaled.  s * t is formed first, once per row and column, unless a scale is
+// so large that the product could overflow where d * s * t does not (d may be zero): then d * s
+// comes first.
+enum ScaleMode { kOneFactor, kColumnFactors, kTwoSteps };
+constexpr float kTame = 1.8446744e19f;  // 2^64
+
+// The accumulators of one block at `taddr` (this warp's lanes and columns) -> sum += scaled block;
+// arrives on `done` when tensor memory is read.
+template <int BN, ScaleMode MODE>
+__device__ __forceinline__ void add_block(uint32_t taddr, uint32_t done, uint32_t lane,
+                                          const float *cols, float row_scale, float col_scale,
+                                          float (&sum)[2][ScaledCfg<BN>::kCols]) {
+  using C = ScaledCfg<BN>;
+  const float s = MODE == kOneFactor ? row_scale * col_scale : row_scale;
+  // Steps of kStep columns of both planes; the next step's loads are on their way while this one's
+  // values are added.  Stacked accumulators are [Ar.Br | Ar.Bi | Ai.Br | Ai.Bi].
+  constexpr int kAccs = C::kStacked ? 4 : 2;
+  constexpr int kStep = C::kStacked || C::kCols < 16 ? 8 : 16;
+  uint32_t d[2][kAccs][kStep];
+#pragma unroll
+  for (int i = 0; i < kAccs; ++i) tmem_ld_cols<kStep>(taddr + i * BN, d[0][i]);
+#pragma unroll
+  for (int c = 0; c < C::kCols; c += kStep) {
+    uint32_t(&v)[kAccs][kStep] = d[(c / kStep) & 1];
+    tmem_wait_ld();
+    if (c + kStep < C::kCols) {
+#pragma unroll
+      for (int i = 0; i < kAccs; ++i) {
+        tmem_ld_cols<kStep>(taddr + i * BN + c + kStep, d[((c / kStep) & 1) ^ 1][i]);
+      }
+    } else {
+      // the buffer is read: the MMAs of the block after next may fill it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(done);
+    }
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {
+      float f = s;
+      if constexpr (MODE == kColumnFactors) f = s * cols[c + j];
+      if constexpr (MODE == kTwoSteps) f = cols[c + j];
+#pragma unroll
+      for (int plane = 0; plane < 2; ++plane) {
+        float x = __uint_as_float(v[plane][j]);
+        // Re = Ar.Br - Ai.Bi, Im = Ar.Bi + Ai.Br
+        if constexpr (C::kStacked) {
+          fma_to(x, __uint_as_float(v[kAccs - 1 - plane][j]), plane == 0 ? -1.0f : 1.0f);
+        }
+        if constexpr (MODE == kTwoSteps) x *= s;
+        fma_to(sum[plane][c + j], x, f);
+      }
+    }
+  }
+}
+
+// alpha and beta on the sums of row m, columns n0 .. n0 + COLS.
+template <typename OutT, int COLS>
 __device__ __forceinline__ void scale_sums(const GemmParams &p, uint32_t b, uint32_t m, uint32_t n0,
-                                           float (&re)[HALF], float (&im)[HALF]) {
+                                           float (&re)[COLS], float (&im)[COLS]) {
   if (p.have_alpha) {
 #pragma unroll
-    for (int j = 0; j < HALF; ++j) {
+    for (int j = 0; j < COLS; ++j) {
       const float r = re[j];
       re[j] = p.alpha_re * r - p.alpha_im * im[j];
       im[j] = p.alpha_im * r + p.alpha_re * im[j];
@@ -218,7 +241,7 @@ __device__ __forceinline__ void scale_sums(const GemmParams &p, uint32_t b, uint
     const COffsets o = c_offsets(p, b, m, n0);
     const OutT *C = static_cast<const OutT *>(p.c);
 #pragma unroll
-    for (int j = 0; j < HALF; ++j) {
+    for (int j = 0; j < COLS; ++j) {
       if (n0 + j < p.N) {
         const float cr = OutTraits<OutT>::to_acc(C[o.base_re + j * o.stride_j]);
         const float ci = OutTraits<OutT>::to_acc(C[o.base_re + j * o.stride_j + o.off_im]);
@@ -229,94 +252,98 @@ __device__ __forceinline__ void scale_sums(const GemmParams &p, uint32_t b, uint
   }
 }
 
-// Word j (0..31) of tile t of a row as it stands in C: 128 bytes of the row.  Planar tiles are the
-// real part's 128-byte pieces, then the imaginary part's; interleaved ones follow one another.
-template <typename OutT, int HALF, int T, int J>
-__device__ __forceinline__ uint32_t row_word(bool inter, const float (&re)[HALF],
-                                             const float (&im)[HALF]) {
-  constexpr int kPer = 4 / sizeof(OutT);
-  constexpr int kTiles = HALF * 2 / (32 * kPer);
-  constexpr int kPlaneTiles = kTiles / 2;
+// The rows of a warp's part of C leave in boxes of 32 rows x 64 bytes: the pieces of the real plane,
+// then those of the imaginary one; or, interleaved, the pieces of the (re, im) sequence in order.
+template <typename OutT, int COLS> struct Boxes {
+  static constexpr int kPer = 4 / static_cast<int>(sizeof(OutT));  // values per word
+  static constexpr int kPlane = COLS * static_cast<int>(sizeof(OutT)) / kStoreBytes;
+  static constexpr int kCount = 2 * kPlane;
+};
+
+// Word J of box T of a row.
+template <typename OutT, int COLS, int T, int J>
+__device__ __forceinline__ uint32_t row_word(bool inter, const float (&re)[COLS],
+                                             const float (&im)[COLS]) {
+  using B = Boxes<OutT, COLS>;
   float v[2];
   if (inter) {
-    constexpr int e = (T * 32 + J) * kPer;  // element of the (re, im) sequence
+    constexpr int e = (T * 16 + J) * B::kPer;  // place in the (re, im) sequence
     v[0] = (e & 1) ? im[e / 2] : re[e / 2];
-    v[1] = im[e / 2];  // 16-bit: the pair (re, im); unused otherwise
+    v[1] = im[e / 2];  // 16-bit words hold a whole (re, im); unused otherwise
   } else {
-    constexpr int c = ((T % kPlaneTiles) * 32 + J) * kPer;
-    v[0] = T < kPlaneTiles ? re[c] : im[c];
-    v[1] = T < kPlaneTiles ? re[c + kPer - 1] : im[c + kPer - 1];
+    constexpr int c = ((T % B::kPlane) * 16 + J) * B::kPer;
+    v[0] = T < B::kPlane ? re[c] : im[c];
+    v[1] = T < B::kPlane ? re[c + B::kPer - 1] : im[c + B::kPer - 1];
   }
   return Packer<OutT>::word(v);
 }
 
-template <typename OutT, int HALF, int T, int... J>
-__device__ __forceinline__ void row_words(bool inter, const float (&re)[HALF],
-                                          const float (&im)[HALF], uint32_t (&w)[32]) {
-  if constexpr (sizeof...(J) < 32) {
-    row_words<OutT, HALF, T, J..., static_cast<int>(sizeof...(J))>(inter, re, im, w);
+template <typename OutT, int COLS, int T, int... J>
+__device__ __forceinline__ void row_words(bool inter, const float (&re)[COLS],
+                                          const float (&im)[COLS], uint32_t (&w)[16]) {
+  if constexpr (sizeof...(J) < 16) {
+    row_words<OutT, COLS, T, J..., static_cast<int>(sizeof...(J))>(inter, re, im, w);
   } else {
-    ((w[J] = row_word<OutT, HALF, T, J>(inter, re, im)), ...);
+    ((w[J] = row_word<OutT, COLS, T, J>(inter, re, im)), ...);
   }
 }
 
-// One tile of 32 rows x 128 bytes through the warp's staging tile and out by a TMA store.
-template <typename OutT, int HALF, int T>
-__device__ __forceinline__ void store_tile(const GemmParams &p, const CUtensorMap *tm_c,
-                                           uint32_t staging, uint32_t lane, uint32_t b, uint32_t m0,
-                                           uint32_t n0, const float (&re)[HALF],
-                                           const float (&im)[HALF]) {
-  constexpr int kPer = 4 / sizeof(OutT);
-  constexpr int kTiles = HALF * 2 / (32 * kPer);
-  constexpr int kPlaneTiles = kTiles / 2;
+// One box through the warp's staging tile (written the way a 64-byte-swizzled TMA store reads it: 16-byte
+// piece j of row r at j ^ ((r >> 1) & 3)) and out.
+template <typename OutT, int COLS, int T>
+__device__ __forceinline__ void store_box(const GemmParams &p, const CUtensorMap *tm_c,
+                                          uint32_t staging, uint32_t lane, uint32_t b, uint32_t m0,
+                                          uint32_t n0, const float (&re)[COLS],
+                                          const float (&im)[COLS]) {
+  using B = Boxes<OutT, COLS>;
   const bool inter = p.c_layout == kInterRow;
-  const uint32_t first = inter ? n0 + T * 16 * kPer : n0 + (T % kPlaneTiles) * 32 * kPer;
+  const uint32_t first = n0 + (inter ? T * 8 * B::kPer : (T % B::kPlane) * 16 * B::kPer);
   if (first >= p.N || m0 >= p.M) return;  // uniform over the warp
-  uint32_t w[32];
-  row_words<OutT, HALF, T>(inter, re, im, w);
+  uint32_t w[16];
+  row_words<OutT, COLS, T>(inter, re, im, w);
   if (lane == 0) bulk_wait_group_read<0>();
   __syncwarp();
-  const uint32_t row = staging + lane * 128;
+  const uint32_t row = staging + lane * kStoreBytes;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    st_shared_v4(row + ((j ^ (lane & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  for (int j = 0; j < 4; ++j) {
+    st_shared_v4(row + ((j ^ ((lane >> 1) & 3)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2],
+                 w[4 * j + 3]);
   }
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) {
     const int32_t x = static_cast<int32_t>(first * sizeof(OutT) * (inter ? 2 : 1));
-    const int32_t z = static_cast<int32_t>(inter ? b : 2 * b + (T < kPlaneTiles ? 0 : 1));
+    const int32_t z = static_cast<int32_t>(inter ? b : 2 * b + (T < B::kPlane ? 0 : 1));
     tma_store_3d(tm_c, staging, x, static_cast<int32_t>(m0), z);
     bulk_commit_group();
   }
 }
 
-template <typename OutT, int HALF, int... T>
-__device__ __forceinline__ void store_tiles(const GemmParams &p, const CUtensorMap *tm_c,
+template <typename OutT, int COLS, int... T>
+__device__ __forceinline__ void store_boxes(const GemmParams &p, const CUtensorMap *tm_c,
                                             uint32_t staging, uint32_t lane, uint32_t b, uint32_t m0,
-                                            uint32_t n0, const float (&re)[HALF],
-                                            const float (&im)[HALF]) {
-  constexpr int kTiles = HALF * 2 * static_cast<int>(sizeof(OutT)) / 128;
-  if constexpr (sizeof...(T) < kTiles) {
-    store_tiles<OutT, HALF, T..., static_cast<int>(sizeof...(T))>(p, tm_c, staging, lane, b, m0, n0,
+                                            uint32_t n0, const float (&re)[COLS],
+                                            const float (&im)[COLS]) {
+  if constexpr (sizeof...(T) < Boxes<OutT, COLS>::kCount) {
+    store_boxes<OutT, COLS, T..., static_cast<int>(sizeof...(T))>(p, tm_c, staging, lane, b, m0, n0,
                                                                   re, im);
   } else {
-    (store_tile<OutT, HALF, T>(p, tm_c, staging, lane, b, m0, n0, re, im), ...);
+    (store_box<OutT, COLS, T>(p, tm_c, staging, lane, b, m0, n0, re, im), ...);
   }
 }
 
-// Row m, HALF columns from n0, straight from registers.
-template <typename OutT, int HALF>
+// Row m, COLS columns from n0, straight from registers.
+template <typename OutT, int COLS>
 __device__ __forceinline__ void store_direct(const GemmParams &p, uint32_t b, uint32_t m, uint32_t n0,
-                                             const float (&re)[HALF], const float (&im)[HALF]) {
+                                             const float (&re)[COLS], const float (&im)[COLS]) {
   if (m >= p.M || n0 >= p.N) return;
   using Tr = OutTraits<OutT>;
   OutT *C = static_cast<OutT *>(p.c);
   const COffsets o = c_offsets(p, b, m, n0);
-  const int valid = static_cast<int>(min(static_cast<uint32_t>(HALF), p.N - n0));
-  if (p.vec_ok && valid == HALF && p.c_layout == kPlanarRow) {
-    store_run<OutT, HALF>(C + o.base_re, re, valid, true);
-    store_run<OutT, HALF>(C + o.base_re + o.off_im, im, valid, true);
+  const int valid = static_cast<int>(min(static_cast<uint32_t>(COLS), p.N - n0));
+  if (p.vec_ok && valid == COLS && p.c_layout == kPlanarRow) {
+    store_run<OutT, COLS>(C + o.base_re, re, valid, true);
+    store_run<OutT, COLS>(C + o.base_re + o.off_im, im, valid, true);
     return;
   }
   if (p.c_layout == kInterRow || p.c_layout == kInterCol) {
@@ -326,7 +353,7 @@ __device__ __forceinline__ void store_direct(const GemmParams &p, uint32_t b, ui
     };
     if (p.pair_ok) {
 #pragma unroll
-      for (int j = 0; j < HALF; ++j) {
+      for (int j = 0; j < COLS; ++j) {
         if (j < valid) {
           *reinterpret_cast<Pair *>(C + o.base_re + j * o.stride_j) =
               Pair{Tr::to_out(re[j]), Tr::to_out(im[j])};
@@ -336,7 +363,7 @@ __device__ __forceinline__ void store_direct(const GemmParams &p, uint32_t b, ui
     }
   }
 #pragma unroll
-  for (int j = 0; j < HALF; ++j) {
+  for (int j = 0; j < COLS; ++j) {
     if (j < valid) {
       C[o.base_re + j * o.stride_j] = Tr::to_out(re[j]);
       C[o.base_re + j * o.stride_j + o.off_im] = Tr::to_out(im[j]);
@@ -345,12 +372,12 @@ __device__ __forceinline__ void store_direct(const GemmParams &p, uint32_t b, ui
 }
 
 template <int BN, typename OutT>
-__global__ void __launch_bounds__(kScaledThreads, 1)
+__global__ void __launch_bounds__(ScaledCfg<BN>::kThreads, 1)
 scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const __grid_constant__ CUtensorMap tm_c, const ScaledParams p) {
   using C = ScaledCfg<BN>;
   constexpr int kStages = C::kStages;
-  constexpr int HALF = C::kHalf;
+  constexpr int COLS = C::kCols;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
@@ -375,7 +402,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     }
     for (int s = 0; s < kAccBuffers; ++s) {
       mbar_init(bar_acc_full + 8 * s, 1);
-      mbar_init(bar_acc_empty + 8 * s, kEpiWarps);
+      mbar_init(bar_acc_empty + 8 * s, C::kEpiWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -392,8 +419,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp < kFirstEpiWarp) {
-  regs_dec<kRegsFirst>();
+  if (warp < C::kFirstEpiWarp) {
+  if constexpr (C::kSplitRegs) regs_dec<40>();
   Walk walk(p);
   Segment seg;
   if (warp == 0) {
@@ -441,90 +468,93 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-    bool ok = true;
-    while (ok && walk.next(p, seg)) {
-      for (uint32_t kb = seg.k0; kb < seg.k1; ++kb) {
-        if (!mbar_wait(bar_acc_empty + 8 * acc, acc_phase ^ 1, abort_flag, p.g.status,
-                       kDevTimeoutMma, p.g.wait_cycles) ||
-            !mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.g.status, kDevTimeoutMma,
-                       p.g.wait_cycles)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t a_base = smem_base + stage * C::kStageBytes;
-          const uint32_t b_base = a_base + C::kABytes;
-          const uint32_t d = tmem_base + acc * C::kAccCols;
+    const uint64_t blocks = walk.blocks(p);
+    for (uint64_t i = 0; i < blocks; ++i) {
+      if (!mbar_wait(bar_acc_empty + 8 * acc, acc_phase ^ 1, abort_flag, p.g.status, kDevTimeoutMma,
+                     p.g.wait_cycles) ||
+          !mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.g.status, kDevTimeoutMma,
+                     p.g.wait_cycles)) {
+        break;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t a_base = smem_base + stage * C::kStageBytes;
+        const uint32_t b_base = a_base + C::kABytes;
+        const uint32_t d = tmem_base + acc * C::kAccCols;
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k) {
-            const uint64_t a_re = smem_desc<128>(a_base + k * 32);
-            const uint64_t a_im = smem_desc<128>(a_base + C::kAPlane + k * 32);
-            const uint64_t b_re = smem_desc<128>(b_base + k * 32);
-            if constexpr (C::kStacked) {
-              tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
-              tc_mma<kKindF8F6F4>(d + 2 * BN, a_im, b_re, p.g.idesc, k != 0);
-            } else {
-              const uint64_t b_im = smem_desc<128>(b_base + C::kBPlane + k * 32);
-              tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
-              tc_mma<kKindF8F6F4>(d + BN, a_re, b_im, p.g.idesc, k != 0);
-              tc_mma<kKindF8F6F4>(d + BN, a_im, b_re, p.g.idesc, 1u);
-              tc_mma<kKindF8F6F4>(d, a_im, b_im, p.g.idesc_neg_a, 1u);
-            }
+        for (int k = 0; k < kBlockK / 32; ++k) {
+          const uint64_t a_re = smem_desc<128>(a_base + k * 32);
+          const uint64_t a_im = smem_desc<128>(a_base + C::kAPlane + k * 32);
+          const uint64_t b_re = smem_desc<128>(b_base + k * 32);
+          if constexpr (C::kStacked) {
+            tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
+            tc_mma<kKindF8F6F4>(d + 2 * BN, a_im, b_re, p.g.idesc, k != 0);
+          } else {
+            const uint64_t b_im = smem_desc<128>(b_base + C::kBPlane + k * 32);
+            tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
+            tc_mma<kKindF8F6F4>(d + BN, a_re, b_im, p.g.idesc, k != 0);
+            tc_mma<kKindF8F6F4>(d + BN, a_im, b_re, p.g.idesc, 1u);
+            tc_mma<kKindF8F6F4>(d, a_im, b_im, p.g.idesc_neg_a, 1u);
           }
-          tc_commit(bar_empty + 8 * stage);
-          tc_commit(bar_acc_full + 8 * acc);
         }
-        __syncwarp();
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-        if (++acc == kAccBuffers) {
-          acc = 0;
-          acc_phase ^= 1;
-        }
+        tc_commit(bar_empty + 8 * stage);
+        tc_commit(bar_acc_full + 8 * acc);
+      }
+      __syncwarp();
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      if (++acc == kAccBuffers) {
+        acc = 0;
+        acc_phase ^= 1;
       }
     }
   }
   } else {
     // ------------------------------------------------------------------ epilogue warps
-    regs_inc<kRegsEpi>();
+    if constexpr (C::kSplitRegs) regs_inc<232>();
     Walk walk(p);
     Segment seg;
-    const uint32_t quad = warp & 3;                     // tensor-memory lanes of this warp
-    const uint32_t half = (warp - kFirstEpiWarp) >> 2;  // which half of the columns
+    const uint32_t quad = warp & 3;                       // tensor-memory lanes of this warp
+    const uint32_t first_col = ((warp - C::kFirstEpiWarp) >> 2) * COLS;  // columns of this warp
     const uint32_t staging =
-        smem_base + kStages * C::kStageBytes + (warp - kFirstEpiWarp) * kStagingTile;
+        smem_base + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * kStoreTile;
     // the column scales of the block (two buffers) at the head of the staging tile
-    f32x2 *col_buf = reinterpret_cast<f32x2 *>(
-        smem + kStages * C::kStageBytes + (warp - kFirstEpiWarp) * kStagingTile);
+    float *col_buf = reinterpret_cast<float *>(
+        smem + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * kStoreTile);
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
     while (walk.next(p, seg)) {
-      f32x2 sum[2][HALF / 2];  // Re, Im
+      float sum[2][COLS];  // Re, Im
       const TileCoord t = decode_tile(p.g, seg.tile);
       const uint32_t m = t.mt * kBlockM + quad * 32 + lane;
-      const uint32_t n0 = t.nt * BN + half * HALF;
+      const uint32_t n0 = t.nt * BN + first_col;
       // this lane's row scale, and the scales of two of the warp's columns
       const float *rs = p.row_scale + (static_cast<size_t>(t.b) * p.g.k_blocks + seg.k0) * p.row_blocks;
       const float *cs = p.col_scale + (static_cast<size_t>(t.b) * p.g.k_blocks + seg.k0) * p.col_blocks;
       const uint32_t c0 = n0 + 2 * lane, c1 = c0 + 1;
       const bool row_in = m < p.g.M;
-      const bool in0 = 2 * lane < HALF && c0 < p.g.N, in1 = 2 * lane < HALF && c1 < p.g.N;
+      const bool in0 = 2 * lane < COLS && c0 < p.g.N, in1 = 2 * lane < COLS && c1 < p.g.N;
       const uint32_t ri = m >> p.row_shift, i0 = c0 >> p.col_shift, i1 = c1 >> p.col_shift;
       float s_next = row_in ? __ldg(rs + ri) : 0.0f;
       float t0_next = in0 ? __ldg(cs + i0) : 0.0f;
       float t1_next = in1 ? __ldg(cs + i1) : 0.0f;
 #pragma unroll
-      for (int j = 0; j < HALF / 2; ++j) sum[0][j] = sum[1][j] = 0;
+      for (int j = 0; j < COLS; ++j) sum[0][j] = sum[1][j] = 0.0f;
       // the column scales go through the staging tile: its last store must have read it
       if (lane == 0) bulk_wait_group_read<0>();
       __syncwarp();
       for (uint32_t kb = seg.k0; ok && kb < seg.k1; ++kb) {
-        const f32x2 s = pair_of(s_next, s_next);
-        f32x2 *cols = col_buf + (kb & 1) * (HALF / 2);
-        if (2 * lane < HALF) cols[lane] = pair_of(t0_next, t1_next);
+        const float s = s_next;
+        // any column's scale stands for the block's where one covers 128 columns
+        const float t = __shfl_sync(0xFFFFFFFFu, t0_next, 0);
+        const bool tame = __all_sync(0xFFFFFFFFu, fabsf(s) <= kTame && fabsf(t0_next) <= kTame &&
+                                                      fabsf(t1_next) <= kTame);
+        float *cols = col_buf + (kb & 1) * COLS;
+        if (2 * lane < COLS) {
+          *reinterpret_cast<float2 *>(cols + 2 * lane) = make_float2(t0_next, t1_next);
+        }
         if (kb + 1 < seg.k1) {
           rs += p.row_blocks;
           cs += p.col_blocks;
@@ -539,57 +569,21 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         if (!ok) break;
         tc_fence_after();
         const uint32_t taddr =
-            tmem_base + ((quad * 32) << 16) + acc * C::kAccCols + half * HALF;
-        // kCols columns of every accumulator at a time, the next ones on their way while these are added
-        constexpr int kCols = HALF < 16 || C::kStacked ? 8 : 16;
-        constexpr int kAccs = C::kStacked ? 4 : 2;
-        uint32_t d[2][kAccs][kCols];
-#pragma unroll
-        for (int i = 0; i < kAccs; ++i) tmem_ld_cols<kCols>(taddr + i * BN, d[0][i]);
-#pragma unroll
-        for (int c = 0; c < HALF; c += kCols) {
-          const int now = (c / kCols) & 1;
-#pragma unroll
-          for (int i = 0; i < kAccs; ++i) tmem_wait_cols<kCols>(d[now][i]);
-          if (c + kCols < HALF) {
-#pragma unroll
-            for (int i = 0; i < kAccs; ++i) {
-              tmem_ld_cols<kCols>(taddr + i * BN + c + kCols, d[now ^ 1][i]);
-            }
-          } else {
-            // the buffer is read: the MMAs of the block after next may fill it
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
-          }
-#pragma unroll
-          for (int j = 0; j < kCols; j += 4) {
-            const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(cols + (c + j) / 2);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int e = j + 2 * h;
-              f32x2 v_re = pair_of(d[now][0][e], d[now][0][e + 1]);
-              f32x2 v_im = pair_of(d[now][1][e], d[now][1][e + 1]);
-              if constexpr (C::kStacked) {
-                v_re = sub2(v_re, pair_of(d[now][3][e], d[now][3][e + 1]));
-                v_im = add2(v_im, pair_of(d[now][2][e], d[now][2][e + 1]));
-              }
-              scale_add(sum[0][(c + e) / 2], v_re, s, h == 0 ? t.x : t.y);
-              scale_add(sum[1][(c + e) / 2], v_im, s, h == 0 ? t.x : t.y);
-            }
-          }
+            tmem_base + ((quad * 32) << 16) + acc * C::kAccCols + first_col;
+        const uint32_t done = bar_acc_empty + 8 * acc;
+        if (!tame) {
+          add_block<BN, kTwoSteps>(taddr, done, lane, cols, s, 0.0f, sum);
+        } else if (p.col_shift != 0) {
+          add_block<BN, kOneFactor>(taddr, done, lane, cols, s, t, sum);
+        } else {
+          add_block<BN, kColumnFactors>(taddr, done, lane, cols, s, 0.0f, sum);
         }
         if (++acc == kAccBuffers) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
-      float re[HALF], im[HALF];
-#pragma unroll
-      for (int j = 0; j < HALF / 2; ++j) {
-        split_pair(sum[0][j], re[2 * j], re[2 * j + 1]);
-        split_pair(sum[1][j], im[2 * j], im[2 * j + 1]);
-      }
+      float(&re)[COLS] = sum[0], (&im)[COLS] = sum[1];
       bool finish = ok;
       if (seg.k1 - seg.k0 < p.g.k_blocks) {
         // Part of a tile: add it through the workspace.  A CTA's run holds at most one part that
@@ -598,16 +592,16 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         constexpr size_t kPart = 2 * BN * kBlockM;
         const uint64_t units = static_cast<uint64_t>(p.g.num_tiles) * p.g.k_blocks;
         const uint64_t base = static_cast<uint64_t>(seg.tile) * p.g.k_blocks;
-        const uint32_t at = half * HALF * kBlockM + quad * 32 + lane;
+        const uint32_t at = first_col * kBlockM + quad * 32 + lane;
         float *mine = p.parts + (2 * static_cast<size_t>(blockIdx.x) + (seg.k0 == 0 ? 1 : 0)) * kPart + at;
 #pragma unroll
-        for (int j = 0; j < HALF; ++j) {
+        for (int j = 0; j < COLS; ++j) {
           __stcg(mine + j * kBlockM, re[j]);
           __stcg(mine + (BN + j) * kBlockM, im[j]);
         }
         __threadfence();
-        epi_sync();
-        if (threadIdx.x == 32 * kFirstEpiWarp) {
+        epi_sync<32 * C::kEpiWarps>();
+        if (threadIdx.x == 32 * C::kFirstEpiWarp) {
           const unsigned add = seg.k1 - seg.k0;
           const unsigned before = atomicAdd(p.counters + seg.tile, add);
           const bool last = before + add == p.g.k_blocks;
@@ -615,19 +609,19 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           __threadfence();
           *last_flag = last ? 1u : 0u;
         }
-        epi_sync();
+        epi_sync<32 * C::kEpiWarps>();
         finish = *last_flag != 0 && ok;
-        epi_sync();  // the flag may be written again
+        epi_sync<32 * C::kEpiWarps>();  // the flag may be written again
         if (finish) {
 #pragma unroll
-          for (int j = 0; j < HALF; ++j) re[j] = im[j] = 0.0f;
+          for (int j = 0; j < COLS; ++j) re[j] = im[j] = 0.0f;
           const uint32_t from = run_owner(units, gridDim.x, base);
           const uint32_t to = run_owner(units, gridDim.x, base + p.g.k_blocks - 1);
           for (uint32_t c = from; c <= to; ++c) {
             const uint32_t slot = run_start(units, gridDim.x, c) > base ? 0 : 1;
             const float *part = p.parts + (2 * static_cast<size_t>(c) + slot) * kPart + at;
 #pragma unroll
-            for (int j = 0; j < HALF; ++j) {
+            for (int j = 0; j < COLS; ++j) {
               re[j] += __ldcg(part + j * kBlockM);
               im[j] += __ldcg(part + (BN + j) * kBlockM);
             }
@@ -635,16 +629,16 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         }
       }
       if (finish) {
-        scale_sums<OutT, HALF>(p.g, t.b, m, n0, re, im);
+        scale_sums<OutT, COLS>(p.g, t.b, m, n0, re, im);
         bool stored = false;
-        if constexpr (HALF * 2 * sizeof(OutT) >= 256) {
+        if constexpr (Boxes<OutT, COLS>::kPlane > 0) {
           if (p.g.epi_tma) {
-            store_tiles<OutT, HALF>(p.g, &tm_c, staging, lane, t.b, t.mt * kBlockM + quad * 32, n0,
+            store_boxes<OutT, COLS>(p.g, &tm_c, staging, lane, t.b, t.mt * kBlockM + quad * 32, n0,
                                     re, im);
             stored = true;
           }
         }
-        if (!stored) store_direct<OutT, HALF>(p.g, t.b, m, n0, re, im);
+        if (!stored) store_direct<OutT, COLS>(p.g, t.b, m, n0, re, im);
       }
     }
     if (p.g.epi_tma && lane == 0) bulk_wait_group<0>();
@@ -665,20 +659,20 @@ using ScaledFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMa
 
 struct ScaledEntry {
   ScaledFn fn;
-  int smem;
+  int smem, threads;
+  bool boxes;  // a warp's columns fill the boxes of the TMA store
 };
 
+template <int BN, typename OutT> ScaledEntry entry() {
+  using C = ScaledCfg<BN>;
+  return {scaled_gemm_kernel<BN, OutT>, C::kSmemBytes, C::kThreads, Boxes<OutT, C::kCols>::kPlane > 0};
+}
+
 template <typename OutT> ScaledEntry pick_width(int bn) {
-  switch (bn) {
-  case 128:
-    return {scaled_gemm_kernel<128, OutT>, ScaledCfg<128>::kSmemBytes};
-  case 64:
-    return {scaled_gemm_kernel<64, OutT>, ScaledCfg<64>::kSmemBytes};
-  case 32:
-    return {scaled_gemm_kernel<32, OutT>, ScaledCfg<32>::kSmemBytes};
-  default:
-    return {scaled_gemm_kernel<16, OutT>, ScaledCfg<16>::kSmemBytes};
-  }
+  return bn == 128  ? entry<128, OutT>()
+         : bn == 64 ? entry<64, OutT>()
+         : bn == 32 ? entry<32, OutT>()
+                    : entry<16, OutT>();
 }
 
 bool is_fp8(int t) { return t == CCGLIB_B200_FLOAT8E4M3 || t == CCGLIB_B200_FLOAT8E5M2; }
@@ -878,7 +872,7 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
   const size_t run_bytes = (planar ? plan->cols : 2 * plan->cols) * plan->out_bytes;
   g.vec_ok = (row && aligned16(d_c) && run_bytes % 16 == 0) ? 1u : 0u;
   g.pair_ok = reinterpret_cast<uintptr_t>(d_c) % (2 * plan->out_bytes) == 0 ? 1u : 0u;
-  g.epi_tma = g.vec_ok && plan->bn / 2 * 2 * plan->out_bytes >= 256 ? 1u : 0u;
+  g.epi_tma = g.vec_ok && plan->kernel.boxes ? 1u : 0u;
   g.status = plan->status;
   g.wait_cycles = plan->wait_cycles;
   p.row_scale = plan->swapped ? d_b_scale : d_a_scale;
@@ -903,13 +897,13 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
   tm_c = tm_a;  // placeholder when the epilogue stores from registers
   if (g.epi_tma) {
     rc = make_map(&tm_c, d_c, run_bytes, plan->rows, planar ? 2 * d.batch : d.batch, run_bytes,
-                  plan->rows * run_bytes, 128, 32, 1);
+                  plan->rows * run_bytes, kStoreBytes, 32, 1);
     if (rc != CCGLIB_B200_OK) return rc;
   }
   const size_t ctas = plan->runs > 0 ? plan->runs
                       : plan->tiles < static_cast<size_t>(plan->sms) ? plan->tiles
                                                                      : plan->sms;
-  plan->kernel.fn<<<static_cast<unsigned>(ctas), kScaledThreads, plan->kernel.smem,
+  plan->kernel.fn<<<static_cast<unsigned>(ctas), plan->kernel.threads, plan->kernel.smem,
                     static_cast<cudaStream_t>(stream_v)>>>(tm_a, tm_b, tm_c, p);
   CCGLIB_CUDA_TRY(cudaGetLastError());
   return CCGLIB_B200_OK;

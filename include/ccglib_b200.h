@@ -238,6 +238,52 @@ CCGLIB_B200_API int ccglib_b200_scaled_gemm_plan_tile(const ccglib_b200_scaled_g
                                                       int tile[3]);
 
 /*
+ * Orthogonalisation by Newton-Schulz products: for every complex M x N matrix of the batch
+ *   X <- X / ||X||_F,  then `steps` times on the shorter side (M <= N: S = X X^H, else S = X^H X)
+ *   X <- a X + (b S + c S^2) X     (M > N: X <- a X + X (b S + c S^2)),
+ * which keeps the singular vectors and maps every singular value s to s (a + b s^2 + c s^4).  The
+ * coefficients (3.4445, -4.7750, 2.0315) take any full-rank matrix to singular values of about
+ * 0.7 .. 1.2 in five steps; (15/8, -5/4, 3/8) converge to 1: orthonormal rows (columns), e.g. a
+ * set of beam weights or the basis of a subspace iteration.  A zero matrix stays zero; a NaN or an
+ * infinity makes its own matrix NaN.
+ *
+ * Input planar [batch][2][M][N] or interleaved [batch][M][N][2], float16, bfloat16 or float32; output
+ * planar [batch][2][M][N], float16 or bfloat16: an operand of the GEMM or input of the quantiser.
+ * Norms are float64, sums float32; between the products X, S and P are float16 (rms error of the
+ * result 1 to 2.5e-3 after 5 to 8 steps).  Results do not depend on timing.  In place (d_out ==
+ * d_in) is allowed where input and output have the same type and the input is planar.
+ * No counterpart in the reference.
+ */
+typedef struct ccglib_b200_orthogonalize_desc {
+  size_t batch;
+  size_t m;
+  size_t n;
+  int type_in;            /* FLOAT16, BFLOAT16 or FLOAT32 */
+  int type_out;           /* FLOAT16 or BFLOAT16 */
+  int input_complex_axis; /* CCGLIB_B200_PLANAR / CCGLIB_B200_INTERLEAVED */
+  int steps;              /* 1 .. 1000 */
+  float a, b, c;
+} ccglib_b200_orthogonalize_desc;
+
+typedef struct ccglib_b200_orthogonalize_plan ccglib_b200_orthogonalize_plan;
+
+/* Validates, chooses the kernels and allocates the workspace (the iterates); it belongs to the
+ * device that is current here. */
+CCGLIB_B200_API int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogonalize_desc *desc,
+                                                          ccglib_b200_orthogonalize_plan **plan);
+
+/* Enqueues all steps on `stream`; no allocation, no synchronisation; may be captured into a graph.
+ * Runs of one plan (replays of graphs that hold one included) must not overlap. */
+CCGLIB_B200_API int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *plan,
+                                                  const void *d_in, void *d_out, void *stream);
+
+CCGLIB_B200_API int ccglib_b200_orthogonalize_plan_destroy(ccglib_b200_orthogonalize_plan *plan);
+
+/* Device bytes the plan owns. */
+CCGLIB_B200_API size_t
+ccglib_b200_orthogonalize_plan_scratch_bytes(const ccglib_b200_orthogonalize_plan *plan);
+
+/*
  * The Pipeline: the caller's matrices in their natural layout -> C, as one object that owns the
  * intermediate buffers.  Replaces ccglib::pipeline::Pipeline (reference
  * include/ccglib/pipeline/pipeline.h:28-73, src/pipeline/Pipeline.cpp:44-188), whose chain is

@@ -57,3 +57,21 @@ def test_scaled_gemm_plan_refuses(args, kw, status, text):
 
 def test_operand_pitch():
     assert [capi.operand_pitch(k) for k in (1, 16, 17, 128, 1990)] == [16, 16, 32, 128, 2000]
+
+
+@pytest.mark.parametrize("args, kw, status, text", [
+    ((0, 4, 4, F16, F16), {}, capi.INVALID_ARGUMENT, "positive"),
+    ((1, 0, 4, F16, F16), {}, capi.INVALID_ARGUMENT, "positive"),
+    ((1, 4, 0, F16, F16), {}, capi.INVALID_ARGUMENT, "positive"),
+    ((1, 1 << 30, 4, F16, F16), {}, capi.INVALID_ARGUMENT, "too large"),
+    ((1 << 29, 1 << 20, 1 << 20, F16, F16), {}, capi.INVALID_ARGUMENT, "too large"),
+    ((1, 4, 4, E4M3, F16), {}, capi.UNSUPPORTED, "input must be"),
+    ((1, 4, 4, F16, F32), {}, capi.UNSUPPORTED, "output must be"),
+    ((1, 4, 4, F16, F16), {"steps": 0}, capi.INVALID_ARGUMENT, "steps"),
+    ((1, 4, 4, F16, F16), {"steps": 1001}, capi.INVALID_ARGUMENT, "steps"),
+    ((1, 4, 4, F16, F16), {"coefficients": (1.0, float("nan"), 0.0)}, capi.INVALID_ARGUMENT, "finite"),
+    ((1, 4, 4, F16, F16), {"input_complex_axis": 5}, capi.INVALID_ARGUMENT, "axis"),
+])
+def test_orthogonalize_plan_refuses(args, kw, status, text):
+    got, message = _status(capi.OrthogonalizePlan, *args, **kw)
+    assert got == status and text in message
