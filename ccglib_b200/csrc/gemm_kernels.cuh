@@ -27,8 +27,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -83,14 +81,6 @@ struct GemmParams {
   uint32_t epi_tma;  // stage C through shared memory and store it with TMA (row-major, 4-byte)
   uint32_t prefetch;  // k-blocks the producer asks L2 to fetch ahead of its own loads (0 = off)
   float alpha_re, alpha_im, beta_re, beta_im;
-  // OrthHalf instances only (orthogonalize.cu)
-  const void *c_in;      // C0 of alpha A B^H + beta C0, laid out as c
-  void *c_t;             // the result transposed (null: not written)
-  uint32_t conj_b;       // multiply by the conjugate of B
-  uint32_t hermitian;    // the result is Hermitian: tiles below the diagonal are mirrored, not computed
-  uint32_t final_type;   // 0: c is float16 planes of M x N; else the last product: value type of c,
-  uint32_t final_trans;  // which holds final_m x final_n of the result, transposed if final_trans
-  uint32_t final_m, final_n;
   unsigned int *status;
   long long wait_cycles;  // SM clock cycles after which a wait on an mbarrier gives up
 };
@@ -157,40 +147,6 @@ __device__ __forceinline__ TileCoord decode_tile(const GemmParams &p, uint32_t t
   t.mt = rr / width;
   t.nt = first_n + (rr - t.mt * width);
   return t;
-}
-
-// Tiles of a Hermitian result that touch its diagonal or lie above it, row by row.
-template <int BN>
-__device__ __forceinline__ TileCoord decode_upper_tile(const GemmParams &p, uint32_t tile,
-                                                       uint32_t per_batch) {
-  TileCoord t;
-  t.b = tile / per_batch;
-  uint32_t r = tile - t.b * per_batch;
-  t.mt = 0;
-  for (;;) {
-    const uint32_t first = t.mt * kBlockM / BN;
-    const uint32_t width = p.tiles_n - first;
-    if (r < width) {
-      t.nt = first + r;
-      return t;
-    }
-    r -= width;
-    ++t.mt;
-  }
-}
-
-// float16 output of the products of the orthogonalisation (see GemmParams).
-struct OrthHalf {
-  __half v;
-};
-
-// The tile of a work item of an instance with output type OutT.
-template <int BN, typename OutT>
-__device__ __forceinline__ TileCoord tile_of(const GemmParams &p, uint32_t tile) {
-  if constexpr (std::is_same_v<OutT, OrthHalf>) {
-    if (p.hermitian) return decode_upper_tile<BN>(p, tile, p.hermitian);
-  }
-  return decode_tile(p, tile);
 }
 
 template <typename T> struct OutTraits;
@@ -397,118 +353,6 @@ __device__ __forceinline__ void epilogue_chunk(const GemmParams &p, uint32_t b, 
   }
 }
 
-// Epilogue of the orthogonalisation's products (real alpha and beta, planes of M x N float16, M and N
-// multiples of eight): row m, 32 columns from n0.
-__device__ __forceinline__ void epilogue_chunk_orth(const GemmParams &p, uint32_t b, uint32_t m,
-                                                    uint32_t n0, const uint32_t (&bits_re)[32],
-                                                    const uint32_t (&bits_im)[32]) {
-  if (m >= p.M) return;
-  const size_t M = p.M, N = p.N, plane = M * N;
-  const uint32_t valid = min(32u, p.N - n0);
-  float re[32], im[32];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    re[j] = p.alpha_re * __uint_as_float(bits_re[j]);
-    im[j] = p.alpha_re * __uint_as_float(bits_im[j]);
-  }
-  const size_t at = static_cast<size_t>(b) * 2 * plane + m * N + n0;
-  if (p.have_beta) {
-    const __half *c0 = static_cast<const __half *>(p.c_in) + at;
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (j < valid) {
-        const uint4 r = *reinterpret_cast<const uint4 *>(c0 + j);
-        const uint4 i = *reinterpret_cast<const uint4 *>(c0 + plane + j);
-        const uint32_t rw[4] = {r.x, r.y, r.z, r.w}, iw[4] = {i.x, i.y, i.z, i.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 rv = __half22float2(*reinterpret_cast<const __half2 *>(&rw[e]));
-          const float2 iv = __half22float2(*reinterpret_cast<const __half2 *>(&iw[e]));
-          re[j + 2 * e] += p.beta_re * rv.x;
-          re[j + 2 * e + 1] += p.beta_re * rv.y;
-          im[j + 2 * e] += p.beta_re * iv.x;
-          im[j + 2 * e + 1] += p.beta_re * iv.y;
-        }
-      }
-    }
-  }
-  if (p.final_type != 0) {
-    // the last product: beta_im carries the factor that undoes the scaling of the iterates
-    if (m >= p.final_m) return;
-    const size_t fm = p.final_m, fn = p.final_n;
-    const size_t base = static_cast<size_t>(b) * 2 * fm * fn + (p.final_trans ? n0 * fm + m : m * fn + n0);
-    const size_t stride = p.final_trans ? fm : 1;
-    const bool bf16 = p.final_type == CCGLIB_B200_BFLOAT16;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      re[j] *= p.beta_im;
-      im[j] *= p.beta_im;
-    }
-    if (p.vec_ok && n0 + 32 <= fn) {
-      if (bf16) {
-        __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + base;
-        store_run<__nv_bfloat16, 32>(c, re, 32, true);
-        store_run<__nv_bfloat16, 32>(c + fm * fn, im, 32, true);
-      } else {
-        __half *c = static_cast<__half *>(p.c) + base;
-        store_run<__half, 32>(c, re, 32, true);
-        store_run<__half, 32>(c + fm * fn, im, 32, true);
-      }
-      return;
-    }
-    uint16_t *c = static_cast<uint16_t *>(p.c) + base;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (n0 + j < fn) {
-        c[j * stride] = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(re[j]))
-                             : __half_as_ushort(__float2half_rn(re[j]));
-        c[j * stride + fm * fn] = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(im[j]))
-                                       : __half_as_ushort(__float2half_rn(im[j]));
-      }
-    }
-    return;
-  }
-  __half *c = static_cast<__half *>(p.c) + at;
-  if (!p.hermitian || n0 > m) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (j < valid) {
-        uint4 r, i;
-        r.x = Packer<__half>::word(re + j);
-        r.y = Packer<__half>::word(re + j + 2);
-        r.z = Packer<__half>::word(re + j + 4);
-        r.w = Packer<__half>::word(re + j + 6);
-        i.x = Packer<__half>::word(im + j);
-        i.y = Packer<__half>::word(im + j + 2);
-        i.z = Packer<__half>::word(im + j + 4);
-        i.w = Packer<__half>::word(im + j + 6);
-        *reinterpret_cast<uint4 *>(c + j) = r;
-        *reinterpret_cast<uint4 *>(c + plane + j) = i;
-      }
-    }
-  } else {
-    // the diagonal runs through this row's columns: what is left of it comes from the mirror image
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (j < valid && n0 + j >= m) {
-        c[j] = __float2half_rn(re[j]);
-        c[plane + j] = __float2half_rn(n0 + j == m ? 0.0f : im[j]);
-      }
-    }
-  }
-  if (p.c_t != nullptr) {
-    // consecutive lanes hold consecutive m: 64-byte runs
-    __half *t = static_cast<__half *>(p.c_t) + static_cast<size_t>(b) * 2 * plane + n0 * M + m;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (j < valid && (!p.hermitian || n0 + j > m)) {
-        t[j * M] = __float2half_rn(re[j]);
-        t[j * M + plane] = __float2half_rn(p.hermitian ? -im[j] : im[j]);
-      }
-    }
-  }
-}
-
 // One lane writes its row of 32 four-byte values into a 4 KiB staging tile laid out the way a
 // 128-byte-swizzled TMA store reads it (16-byte chunk j of row r sits at chunk j ^ (r & 7)).
 template <typename Acc>
@@ -694,7 +538,7 @@ cgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
     auto prefetch_next = [&]() {
       if (pf_tile >= p.num_tiles) return;
       int32_t ax, ay, az, bx, by, bz;
-      coords(tile_of<BN, OutT>(p, pf_tile), pf_kb, ax, ay, az, bx, by, bz);
+      coords(decode_tile(p, pf_tile), pf_kb, ax, ay, az, bx, by, bz);
       tma_prefetch_3d(&tm_a, ax, ay, az);
       tma_prefetch_3d(&tm_b, bx, by, bz);
       if (++pf_kb == p.k_blocks) {
@@ -707,7 +551,7 @@ cgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
     }
     uint32_t tile_iter = 0;
     for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x, ++tile_iter) {
-      const TileCoord t = tile_of<BN, OutT>(p, tile);
+      const TileCoord t = decode_tile(p, tile);
       for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
         if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status,
                        kDevTimeoutProducer, p.wait_cycles)) {
@@ -799,23 +643,15 @@ cgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                 tc_mma_mxf4(d_re, a_im, b_im, p.idesc_neg_a, sf, sf + 16, 1u);
               }
             } else {
-              uint32_t idesc_ar_bi = p.idesc, idesc_ai_bi = p.idesc_neg_a;
-              if constexpr (std::is_same_v<OutT, OrthHalf>) {
-                // conj(B): Re = Ar.Br + Ai.Bi, Im = Ai.Br - Ar.Bi
-                if (p.conj_b) {
-                  idesc_ar_bi = p.idesc_neg_a;
-                  idesc_ai_bi = p.idesc;
-                }
-              }
               tc_mma<KIND>(d_re, a_re, b_re, p.idesc, accum);
-              tc_mma<KIND>(d_im, a_re, b_im, idesc_ar_bi, accum);
+              tc_mma<KIND>(d_im, a_re, b_im, p.idesc, accum);
               tc_mma<KIND>(d_im, a_im, b_re, p.idesc, 1u);
               if constexpr (A_PLANES == 3) {
                 // third plane already holds -Ai (integer kinds have no negate bit)
                 const uint64_t a_neg = smem_desc<SW>(a_base + 2 * C::kAPlane + k * 32);
                 tc_mma<KIND>(d_re, a_neg, b_im, p.idesc, 1u);
               } else {
-                tc_mma<KIND>(d_re, a_im, b_im, idesc_ai_bi, 1u);
+                tc_mma<KIND>(d_re, a_im, b_im, p.idesc_neg_a, 1u);
               }
             }
           }
@@ -843,7 +679,7 @@ cgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
     uint32_t slot = 0;  // staging tile rotation
     [[maybe_unused]] uint32_t iter = 0;
     for (uint32_t tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++iter) {
-      const TileCoord t = tile_of<BN, OutT>(p, tile);
+      const TileCoord t = decode_tile(p, tile);
       if (!mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.status,
                      kDevTimeoutEpilogue, p.wait_cycles)) {
         break;
@@ -883,11 +719,7 @@ cgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
             continue;
           }
         }
-        if constexpr (std::is_same_v<OutT, OrthHalf>) {
-          epilogue_chunk_orth(p, t.b, m, n0, bits_re, bits_im);
-        } else {
-          epilogue_chunk<OutT>(p, t.b, m, n0, bits_re, bits_im);
-        }
+        epilogue_chunk<OutT>(p, t.b, m, n0, bits_re, bits_im);
       }
       tc_fence_before();
       __syncwarp();

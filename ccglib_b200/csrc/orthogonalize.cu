@@ -2,21 +2,22 @@
 //
 //   X <- X / ||X||_F;   `steps` times:  S = X X^H,  P = b S + c S S,  X <- a X + P X
 //
-// (on the shorter side: a matrix with more rows than columns is iterated as its transpose).  Every step
-// keeps the singular vectors and maps each singular value s to s (a + b s^2 + c s^4).
+// (M <= N; for M > N the same on X^T, i.e. S = X^T conj(X) and X <- a X + X P^T).  Every step keeps the
+// singular vectors and maps each singular value s to s (a + b s^2 + c s^4).
 //
-// The three products of a step run on the tensor cores, kind::f16 with float32 sums, through
-// cgemm_tcgen05_kernel with an epilogue of its own: the conjugate of B comes from the negate bit of
-// the other cross product, S and P are computed on and above the diagonal and mirrored on the way
-// out, b S and a X are added from the operand that is there already, and the update stores X and its
-// transpose (the next step contracts over the one, then the other), so a step is three launches and
-// nothing else.  The last update writes the caller's type and layout.
+// Three launches per step and nothing else, float32 sums on the tensor cores (kind::f16).  S and P are
+// Hermitian: only tiles on and above the diagonal are computed, each stored a second time as its
+// mirror image.  X is never transposed: where a product contracts over rows, its operand is read with
+// the rows as K (the MN-major form of the shared-memory descriptor).  b S and a X are added in the
+// epilogue; the last update writes the caller's type and layout.
 //
-// Between products X, S and P are float16.  All three are bounded (a singular value is at most about
+// Between products X, S and P are float16.  All three are bounded (singular values stay near or below
 // one), X is kept times a power of two near sqrt(long side) so that its entries are near one, and float16
-// keeps eleven bits where bfloat16, the other 16-bit choice, keeps eight: rms error 1 to 2.5e-3 of the
-// result after 5 to 8 steps, about that of rounding it to bfloat16.  Sums and the norm
-// are float32 and float64.
+// keeps eleven bits where bfloat16, the usual 16-bit choice, keeps eight.  A step is computed from the
+// rounded X throughout, a X included: an error of X then goes through the map like X itself, which
+// contracts it.  (A float32 copy of X for the a X term alone adds a times the rounding of X instead; it
+// took the error of eight steps of the steep quintic from 2.1e-3 to 3.7e-3.)  Error of the result, rms:
+// 0.7e-3 after eight steps that converge, 1.2 to 2.5e-3 after 5 to 8 of the quintic.
 #include <cmath>
 #include <new>
 
@@ -25,42 +26,455 @@
 namespace ccglib_b200 {
 namespace {
 
-using OrthFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const GemmParams);
+constexpr int kOrthK = 64;          // float16 values of K per stage: one 128-byte swizzle span
+constexpr int kOrthBox = 32 * 64;   // staging box: 32 rows x 32 float16
+constexpr int kOrthStaging = 4 * 4 * kOrthBox;  // per epilogue warp: Re, Im and their mirror images
 
-OrthFn orth_kernel(int bn) {
-  return bn == 256   ? cgemm_tcgen05_kernel<kKindF16, 256, 128, 2, OrthHalf, 0>
-         : bn == 128 ? cgemm_tcgen05_kernel<kKindF16, 128, 128, 2, OrthHalf, 0>
-                     : cgemm_tcgen05_kernel<kKindF16, 64, 128, 2, OrthHalf, 0>;
+struct OrthParams {
+  uint32_t m, n;        // result: m x n per batch item
+  uint32_t k_blocks;
+  uint32_t tiles_m, tiles_n, group_n;
+  uint32_t per_batch, num_tiles;
+  uint32_t hermitian;   // compute tiles that touch or lie above the diagonal, store their mirror image
+  uint32_t conj_b;      // A x B^H instead of A x B^T
+  float alpha, beta, gain;  // result = gain * (alpha * sum + beta * c0)
+  const __half *c0;     // [batch][2][m][c0_pitch] (null: none)
+  uint32_t c0_pitch;
+  uint32_t bf16;        // the result is bfloat16
+  uint32_t boxes;       // the result leaves by TMA; else value by value to `out` [batch][2][m][n_out]
+  uint16_t *out;
+  uint32_t n_out;
+  unsigned int *status;
+  long long wait_cycles;
+};
+
+template <int BN> struct OrthCfg {
+  // 64 columns: one MMA multiplies an A plane by both B planes (see scaled_gemm.cu)
+  static constexpr bool kStacked = BN == 64;
+  static constexpr int kAccCols = kStacked ? 4 * BN : 2 * BN;
+  static constexpr int kAccStages = 2;
+  static constexpr int kABytes = 2 * kBlockM * 128;
+  static constexpr int kBBytes = 2 * BN * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = (kMaxSmem - 1024 - 256 - kOrthStaging) / kStageBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kOrthStaging + 1024 + 256;
+  static_assert(kStages >= 3 && kAccCols * kAccStages <= kTmemCols, "tile does not fit");
+};
+
+// Shared-memory descriptor of an operand whose rows are K: 128-byte rows of 64 values along M or N,
+// groups of eight rows 1024 bytes apart, the next 64 values `atom` bytes on.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t atom) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(atom >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-int orth_smem(int bn) {
-  return bn == 256   ? Cfg<256, 128, 2, 0>::kSmemBytes
-         : bn == 128 ? Cfg<128, 128, 2, 0>::kSmemBytes
-                     : Cfg<64, 128, 2, 0>::kSmemBytes;
+template <int BN>
+__device__ __forceinline__ TileCoord orth_tile(const OrthParams &p, uint32_t tile) {
+  TileCoord t;
+  t.b = tile / p.per_batch;
+  uint32_t r = tile - t.b * p.per_batch;
+  if (p.hermitian) {
+    for (t.mt = 0;; ++t.mt) {
+      const uint32_t first = t.mt * kBlockM / BN, width = p.tiles_n - first;
+      if (r < width) {
+        t.nt = first + r;
+        return t;
+      }
+      r -= width;
+    }
+  }
+  // column panels, as in decode_tile
+  const uint32_t panel = p.group_n * p.tiles_m;
+  const uint32_t g = r / panel, first_n = g * p.group_n;
+  const uint32_t width = min(p.group_n, p.tiles_n - first_n);
+  r -= g * panel;
+  t.mt = r / width;
+  t.nt = first_n + (r - t.mt * width);
+  return t;
 }
 
-// Tiles of one product and the width that finishes soonest: waves x time per tile relative to a 128-wide
-// tile (a 64-wide one takes as long on the tensor pipe, a 256-wide one 5 % less per column).
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+__device__ __forceinline__ uint16_t round_half(float v, bool bf16) {
+  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+
+__device__ __forceinline__ void st_shared_u16(uint32_t addr, uint16_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
+}
+
+// 32 rows x 32 columns (one row per lane, from m0; columns from n0) of one batch item.
+__device__ __forceinline__ void orth_store(const OrthParams &p, const CUtensorMap *tm_c,
+                                           uint32_t staging, uint32_t lane, uint32_t b, uint32_t m0,
+                                           uint32_t n0, float (&re)[32], float (&im)[32]) {
+  const uint32_t m = m0 + lane;
+  if (p.c0 != nullptr && m < p.m) {
+    const size_t plane = static_cast<size_t>(p.m) * p.c0_pitch;
+    const __half *src = p.c0 + static_cast<size_t>(b) * 2 * plane +
+                        static_cast<size_t>(m) * p.c0_pitch + n0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      if (n0 + j < p.c0_pitch) {  // the pitch is a multiple of eight
+        const uint4 r = *reinterpret_cast<const uint4 *>(src + j);
+        const uint4 i = *reinterpret_cast<const uint4 *>(src + plane + j);
+        const uint32_t rw[4] = {r.x, r.y, r.z, r.w}, iw[4] = {i.x, i.y, i.z, i.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 rv = __half22float2(*reinterpret_cast<const __half2 *>(&rw[e]));
+          const float2 iv = __half22float2(*reinterpret_cast<const __half2 *>(&iw[e]));
+          re[j + 2 * e] = fmaf(p.beta, rv.x, p.alpha * re[j + 2 * e]);
+          re[j + 2 * e + 1] = fmaf(p.beta, rv.y, p.alpha * re[j + 2 * e + 1]);
+          im[j + 2 * e] = fmaf(p.beta, iv.x, p.alpha * im[j + 2 * e]);
+          im[j + 2 * e + 1] = fmaf(p.beta, iv.y, p.alpha * im[j + 2 * e + 1]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      re[j] *= p.alpha;
+      im[j] *= p.alpha;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    re[j] *= p.gain;
+    im[j] *= p.gain;
+  }
+  if (!p.boxes) {
+    if (m < p.m) {
+      const size_t plane = static_cast<size_t>(p.m) * p.n_out;
+      uint16_t *dst = p.out + static_cast<size_t>(b) * 2 * plane + static_cast<size_t>(m) * p.n_out + n0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        if (n0 + j < p.n_out) {
+          dst[j] = round_half(re[j], p.bf16);
+          dst[plane + j] = round_half(im[j], p.bf16);
+        }
+      }
+    }
+    return;
+  }
+  const bool diagonal = p.hermitian && n0 == m0;
+  // 16-byte piece j of row r of a box stands at j ^ ((r >> 1) & 3): the 64-byte swizzle
+  if (lane == 0) bulk_wait_group_read<0>();
+  __syncwarp();
+  const uint32_t row = staging + lane * 64;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t at = row + ((j ^ ((lane >> 1) & 3)) << 4);
+    const int e = 8 * j;
+    st_shared_v4(at, pack_half(re[e], re[e + 1], p.bf16), pack_half(re[e + 2], re[e + 3], p.bf16),
+                 pack_half(re[e + 4], re[e + 5], p.bf16), pack_half(re[e + 6], re[e + 7], p.bf16));
+    st_shared_v4(at + kOrthBox, pack_half(im[e], im[e + 1], p.bf16),
+                 pack_half(im[e + 2], im[e + 3], p.bf16), pack_half(im[e + 4], im[e + 5], p.bf16),
+                 pack_half(im[e + 6], im[e + 7], p.bf16));
+  }
+  if (p.hermitian) {
+    // the mirror image: row n0 + j, this lane's column.  On the diagonal block it goes over the
+    // rows just written: below the diagonal, and zero imaginary parts on it.
+    const uint32_t mirror = diagonal ? staging : staging + 2 * kOrthBox;
+    if (diagonal) __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (!diagonal || j > static_cast<int>(lane)) {
+        const uint32_t at = mirror + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
+        st_shared_u16(at, __half_as_ushort(__float2half_rn(re[j])));
+        st_shared_u16(at + kOrthBox, __half_as_ushort(__float2half_rn(-im[j])));
+      }
+    }
+    if (diagonal) {
+      st_shared_u16(staging + kOrthBox + lane * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4) +
+                        (lane & 7) * 2, 0);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    const int32_t z = static_cast<int32_t>(2 * b);
+    const int32_t x = static_cast<int32_t>(n0 * 2), y = static_cast<int32_t>(m0);
+    if (m0 < p.m) {
+      tma_store_3d(tm_c, staging, x, y, z);
+      tma_store_3d(tm_c, staging + kOrthBox, x, y, z + 1);
+      if (p.hermitian && !diagonal && n0 < p.m) {
+        const int32_t tx = static_cast<int32_t>(m0 * 2), ty = static_cast<int32_t>(n0);
+        tma_store_3d(tm_c, staging + 2 * kOrthBox, tx, ty, z);
+        tma_store_3d(tm_c, staging + 3 * kOrthBox, tx, ty, z + 1);
+      }
+    }
+    bulk_commit_group();
+  }
+}
+
+// result = gain * (alpha * A x op(B)^T + beta * c0), tiles of 128 x BN.  An operand that is MN-major is
+// stored [K][M or N]; the others are stored [M or N][K].  Roles as in cgemm_tcgen05_kernel.
+template <int BN, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kThreads, 1)
+orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
+                    const __grid_constant__ CUtensorMap tm_b,
+                    const __grid_constant__ CUtensorMap tm_c, const OrthParams p) {
+  using C = OrthCfg<BN>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kAtom = 2 * kOrthK * 128;  // 64 values along M or N of both planes
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~static_cast<uintptr_t>(1023u));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * C::kStageBytes + kOrthStaging);
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_acc_full = bar_empty + 8 * kStages;
+  const uint32_t bar_acc_empty = bar_acc_full + 8 * C::kAccStages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 2 * C::kAccStages);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < C::kAccStages; ++s) {
+      mbar_init(bar_acc_full + 8 * s, 1);
+      mbar_init(bar_acc_empty + 8 * s, 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+    prefetch_tensormap(&tm_c);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    uint32_t stage = 0, phase = 0, issued = 0;
+    bool ok = true;
+    for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+      const TileCoord t = orth_tile<BN>(p, tile);
+      for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
+        if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, kDevTimeoutProducer,
+                       p.wait_cycles)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t full = bar_full + 8 * stage;
+          const uint32_t dst = smem_base + stage * C::kStageBytes;
+          const int32_t k = static_cast<int32_t>(kb * kOrthK), z = static_cast<int32_t>(2 * t.b);
+          const int32_t m0 = static_cast<int32_t>(t.mt * kBlockM), n0 = static_cast<int32_t>(t.nt * BN);
+          mbar_arrive_expect_tx(full, C::kStageBytes);
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int i = 0; i < kBlockM / 64; ++i) {
+              tma_load_3d(dst + i * kAtom, &tm_a, (m0 + 64 * i) * 2, k, z, full);
+            }
+          } else {
+            tma_load_3d(dst, &tm_a, k * 2, m0, z, full);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int i = 0; i < BN / 64; ++i) {
+              tma_load_3d(dst + C::kABytes + i * kAtom, &tm_b, (n0 + 64 * i) * 2, k, z, full);
+            }
+          } else {
+            tma_load_3d(dst + C::kABytes, &tm_b, k * 2, n0, z, full);
+          }
+        }
+        __syncwarp();
+        issued |= 1u << stage;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (*abort_flag) {
+      // our own copies must land before the CTA leaves
+      for (int s = 0; s < kStages; ++s) {
+        if (!(issued & (1u << s))) continue;
+        const uint32_t parity = (static_cast<uint32_t>(s) < stage) ? phase : (phase ^ 1);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar_full + 8 * s, parity)) {
+          if (clock64() - t0 > p.wait_cycles) {
+            atomicOr(p.status, kDevTimeoutDrain);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    // descriptor: fp32 sums, f16 operands, bit 13 negates A, bits 15 / 16 say that A / B is MN-major
+    constexpr uint32_t kIdesc = (1u << 4) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) |
+                                (static_cast<uint32_t>((C::kStacked ? 2 * BN : BN) >> 3) << 17) |
+                                (static_cast<uint32_t>(kBlockM >> 4) << 24);
+    constexpr uint32_t kNegA = kIdesc | (1u << 13);
+    // A x B^T: Re = Ar.Br - Ai.Bi, Im = Ar.Bi + Ai.Br; with conj(B): Re = Ar.Br + Ai.Bi, Im = Ai.Br - Ar.Bi
+    const uint32_t ar_bi = p.conj_b ? kNegA : kIdesc, ai_bi = p.conj_b ? kIdesc : kNegA;
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+    bool ok = true;
+    for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+      if (!mbar_wait(bar_acc_empty + 8 * acc, acc_phase ^ 1, abort_flag, p.status, kDevTimeoutMma,
+                     p.wait_cycles)) {
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem_base + acc * C::kAccCols;
+      for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
+        if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, kDevTimeoutMma,
+                       p.wait_cycles)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t a_base = smem_base + stage * C::kStageBytes;
+          const uint32_t b_base = a_base + C::kABytes;
+#pragma unroll
+          for (int k = 0; k < kOrthK / 16; ++k) {
+            // plane of 64 x 64 values of an MN-major atom: 8 KiB; 16 rows of K: 2 KiB
+            const uint64_t a_re = A_MN ? smem_desc_mn(a_base + k * 2048, kAtom)
+                                       : smem_desc<128>(a_base + k * 32);
+            const uint64_t a_im = A_MN ? smem_desc_mn(a_base + kAtom / 2 + k * 2048, kAtom)
+                                       : smem_desc<128>(a_base + kBlockM * 128 + k * 32);
+            const uint32_t more = (kb | static_cast<uint32_t>(k)) != 0 ? 1u : 0u;
+            if constexpr (C::kStacked) {
+              // both B planes lie one behind the other: [Ar.Br | Ar.Bi], [Ai.Br | Ai.Bi]
+              const uint64_t b_both = B_MN ? smem_desc_mn(b_base + k * 2048, kAtom / 2)
+                                           : smem_desc<128>(b_base + k * 32);
+              tc_mma<kKindF16>(d, a_re, b_both, kIdesc, more);
+              tc_mma<kKindF16>(d + 2 * BN, a_im, b_both, kIdesc, more);
+            } else {
+              const uint64_t b_re = B_MN ? smem_desc_mn(b_base + k * 2048, kAtom)
+                                         : smem_desc<128>(b_base + k * 32);
+              const uint64_t b_im = B_MN ? smem_desc_mn(b_base + kAtom / 2 + k * 2048, kAtom)
+                                         : smem_desc<128>(b_base + BN * 128 + k * 32);
+              tc_mma<kKindF16>(d, a_re, b_re, kIdesc, more);
+              tc_mma<kKindF16>(d + BN, a_re, b_im, ar_bi, more);
+              tc_mma<kKindF16>(d + BN, a_im, b_re, kIdesc, 1u);
+              tc_mma<kKindF16>(d, a_im, b_im, ai_bi, 1u);
+            }
+          }
+          tc_commit(bar_empty + 8 * stage);
+          if (kb + 1 == p.k_blocks) tc_commit(bar_acc_full + 8 * acc);
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (++acc == C::kAccStages) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue warps
+    const uint32_t quad = warp & 3;
+    const uint32_t staging = smem_base + kStages * C::kStageBytes + quad * (4 * kOrthBox);
+    uint32_t acc = 0, acc_phase = 0;
+    for (uint32_t tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x) {
+      const TileCoord t = orth_tile<BN>(p, tile);
+      bool ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.status,
+                          kDevTimeoutEpilogue, p.wait_cycles);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      tc_fence_after();
+      const uint32_t m0 = t.mt * kBlockM + quad * 32;
+      const uint32_t taddr = tmem_base + ((quad * 32) << 16) + acc * C::kAccCols;
+#pragma unroll 1
+      for (uint32_t c0 = 0; c0 < BN; c0 += 32) {
+        const uint32_t n0 = t.nt * BN + c0;
+        if (n0 >= p.n) break;
+        if (m0 >= p.m || (p.hermitian && n0 < m0)) continue;  // comes from the mirror image
+        uint32_t r[32], i[32];
+        float re[32], im[32];
+        tmem_ld_32x32b_x32(taddr + c0, r);
+        tmem_ld_32x32b_x32(taddr + BN + c0, i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          re[j] = __uint_as_float(r[j]);
+          im[j] = __uint_as_float(i[j]);
+        }
+        if constexpr (C::kStacked) {
+          tmem_ld_32x32b_x32(taddr + 2 * BN + c0, i);  // Ai.Br
+          tmem_ld_32x32b_x32(taddr + 3 * BN + c0, r);  // Ai.Bi
+          tmem_wait_ld();
+          const float sign = p.conj_b ? -1.0f : 1.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            re[j] -= sign * __uint_as_float(r[j]);
+            im[j] = sign * im[j] + __uint_as_float(i[j]);
+          }
+        }
+        orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
+      if (++acc == C::kAccStages) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
+  }
+
+  // ------------------------------------------------------------------ tear-down
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+using OrthFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const OrthParams);
+
+template <int BN> OrthFn orth_kernel(bool a_mn, bool b_mn) {
+  return a_mn ? orth_product_kernel<BN, true, true>
+         : b_mn ? orth_product_kernel<BN, false, true>
+                : orth_product_kernel<BN, false, false>;
+}
+OrthFn orth_kernel(int bn, bool a_mn, bool b_mn) {
+  return bn == 128 ? orth_kernel<128>(a_mn, b_mn) : orth_kernel<64>(a_mn, b_mn);
+}
+int orth_smem(int bn) { return bn == 128 ? OrthCfg<128>::kSmemBytes : OrthCfg<64>::kSmemBytes; }
+
+// Tiles of one product, of the width that finishes sooner: waves x tensor time of a tile.  (A 64-wide
+// tile takes half the MMAs of a 128-wide one.)
 struct ProductShape {
   int bn;
   size_t per_batch;
 };
 
-size_t upper_tiles(size_t n, size_t bn) {
-  const size_t rows = ceil_div<size_t>(n, kBlockM), cols = ceil_div<size_t>(n, bn);
-  size_t tiles = 0;
-  for (size_t i = 0; i < rows; ++i) tiles += cols - i * kBlockM / bn;
-  return tiles;
-}
-
 ProductShape pick_shape(size_t batch, size_t m, size_t n, bool hermitian, size_t sms) {
   ProductShape best{0, 0};
   double least = 0.0;
-  for (int bn : {128, 256, 64}) {
-    const size_t tiles = hermitian ? upper_tiles(m, bn)
-                                   : ceil_div<size_t>(m, kBlockM) * ceil_div<size_t>(n, bn);
-    const double cost = static_cast<double>(ceil_div(batch * tiles, sms)) *
-                        (bn == 256 ? 1.9 : bn == 128 ? 1.0 : 0.95);
+  for (int bn : {128, 64}) {
+    const size_t rows = ceil_div<size_t>(m, kBlockM), cols = ceil_div<size_t>(n, bn);
+    size_t tiles = 0;
+    for (size_t i = 0; i < rows; ++i) tiles += cols - (hermitian ? i * kBlockM / bn : 0);
+    const double cost =
+        static_cast<double>(ceil_div(batch * tiles, sms)) * (bn == 128 ? 1.0 : 0.6);
     if (best.bn == 0 || cost < least) {
       best = {bn, tiles};
       least = cost;
@@ -109,28 +523,21 @@ struct FirstParams {
   const void *in;      // the caller's matrices, rows x cols
   const double *sums;  // [batch][chunks]
   size_t chunks, batch, rows, cols;
-  __half *x, *x_t;       // x: [batch][2][short_p][long_p], x_t: [batch][2][long_p][short_p]
-  size_t rows_p, cols_p;  // rows and cols rounded up to eight
-  bool tall;              // rows is the long side: x is the transpose of the input
+  __half *x;           // [batch][2][rows][pitch], zeros behind cols
+  size_t pitch;
   float scale;
 };
 
-constexpr int kFirstTile = 64;
+constexpr size_t kFirstChunk = 4096;  // complex values (padded rows) one CTA converts
 
-// X0 = scale * input / norm and its transpose, zero padded.  A CTA turns one 64 x 64 tile of a plane
-// pair in shared memory, so that both copies are written along their rows.
+// X0 = scale * input / norm.
 template <typename T, bool IL>
 __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
-  __shared__ __half tile[2][kFirstTile][kFirstTile + 2];
   __shared__ double part[256 / 32];
-  const size_t tr = ceil_div<size_t>(p.rows_p, kFirstTile), tc = ceil_div<size_t>(p.cols_p, kFirstTile);
-  const size_t items = p.batch * tr * tc;
-  // input rows x cols planes: `straight` has its layout, `turned` the transposed one
-  __half *straight = p.tall ? p.x_t : p.x, *turned = p.tall ? p.x : p.x_t;
-  const size_t plane_p = p.rows_p * p.cols_p;
+  const size_t plane = p.rows * p.pitch, per_batch = ceil_div<size_t>(plane, kFirstChunk);
+  const size_t items = p.batch * per_batch;
   for (size_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const size_t b = item / (tr * tc), rest = item - b * (tr * tc);
-    const size_t r0 = rest / tc * kFirstTile, c0 = rest % tc * kFirstTile;
+    const size_t b = item / per_batch;
     double sum = 0.0;
     for (size_t i = threadIdx.x; i < p.chunks; i += 256) sum += p.sums[b * p.chunks + i];
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -141,33 +548,19 @@ __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
     // a zero matrix stays zero (and one with a NaN becomes NaN)
     const double factor = sum == 0.0 ? 0.0 : static_cast<double>(p.scale) / sqrt(sum);
     const T *in = static_cast<const T *>(p.in) + b * 2 * p.rows * p.cols;
-    for (int i = threadIdx.x; i < kFirstTile * kFirstTile; i += 256) {
-      const size_t r = r0 + i / kFirstTile, c = c0 + i % kFirstTile;
+    __half *x = p.x + b * 2 * plane;
+    const size_t first = (item - b * per_batch) * kFirstChunk;
+#pragma unroll 4
+    for (size_t i = first + threadIdx.x; i < min(plane, first + kFirstChunk); i += 256) {
+      const size_t r = i / p.pitch, c = i - r * p.pitch;
       float re = 0.0f, im = 0.0f;
-      if (r < p.rows && c < p.cols) {
+      if (c < p.cols) {
         const size_t s = r * p.cols + c;
         re = as_float(IL ? in[2 * s] : in[s]);
         im = as_float(IL ? in[2 * s + 1] : in[s + p.rows * p.cols]);
       }
-      const __half hr = __float2half_rn(static_cast<float>(re * factor));
-      const __half hi = __float2half_rn(static_cast<float>(im * factor));
-      if (r < p.rows_p && c < p.cols_p) {
-        __half *dst = straight + b * 2 * plane_p + r * p.cols_p + c;
-        dst[0] = hr;
-        dst[plane_p] = hi;
-      }
-      tile[0][i / kFirstTile][i % kFirstTile] = hr;
-      tile[1][i / kFirstTile][i % kFirstTile] = hi;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kFirstTile * kFirstTile; i += 256) {
-      const int y = i / kFirstTile, x = i % kFirstTile;
-      const size_t c = c0 + y, r = r0 + x;
-      if (r < p.rows_p && c < p.cols_p) {
-        __half *dst = turned + b * 2 * plane_p + c * p.rows_p + r;
-        dst[0] = tile[0][x][y];
-        dst[plane_p] = tile[1][x][y];
-      }
+      x[i] = __float2half_rn(static_cast<float>(re * factor));
+      x[i + plane] = __float2half_rn(static_cast<float>(im * factor));
     }
     __syncthreads();
   }
@@ -180,73 +573,87 @@ using namespace ccglib_b200;
 
 struct ccglib_b200_orthogonalize_plan {
   ccglib_b200_orthogonalize_desc desc;
-  size_t n, l, n_p, l_p;  // short and long side, and both rounded up to eight
-  bool tall;              // m > n: iterate on the transpose
-  float scale;            // power of two near sqrt(long side)
-  ProductShape gram, update;
+  size_t n, l;          // short and long side
+  size_t n_p, cols_p;   // row pitches of S and P, and of X: multiples of eight
+  bool tall;            // m > n
+  float scale;          // power of two near sqrt(long side)
+  ProductShape square, update;
   size_t chunks;
   int device, sms;
   long long wait_cycles;
   unsigned *status;
   void *scratch;
   size_t scratch_bytes;
-  __half *x, *x_t[2], *s, *p;
+  __half *x[2], *s, *p;  // [batch][2][m][cols_p], [batch][2][n][n_p]
   double *sums;
 };
 
 namespace {
 
+// One operand: planes of `rows` x `cols` (row pitch `pitch` values), contracted over its columns, or over
+// its rows (by_rows).
+struct Operand {
+  const __half *data;
+  size_t rows, cols, pitch;
+  bool by_rows;
+};
+
 struct Product {
-  const __half *a, *b;  // planes of m x k and n x k
-  size_t m, n, k;
+  Operand a, b;
+  size_t m, n;  // n: columns written
   ProductShape shape;
   bool hermitian, conj;
-  float alpha, beta;
+  float alpha, beta, gain;
   const __half *c0;
-  void *c;
-  __half *c_t;
-  bool last;
+  size_t c0_pitch;
+  void *out;
+  size_t out_pitch;
+  bool boxes, bf16;
 };
+
+int operand_map(CUtensorMap *tm, const Operand &o, size_t batch, int tile) {
+  const uint32_t box = o.by_rows ? kOrthK : static_cast<uint32_t>(tile);
+  return make_map(tm, o.data, o.cols * 2, o.rows, 2 * batch, o.pitch * 2, o.rows * o.pitch * 2, 128, box, 2);
+}
 
 int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q, cudaStream_t stream) {
   const size_t batch = plan.desc.batch;
-  GemmParams g{};
-  g.M = static_cast<uint32_t>(q.m);
-  g.N = static_cast<uint32_t>(q.n);
-  g.k_blocks = static_cast<uint32_t>(ceil_div<size_t>(q.k * 2, 128));
+  OrthParams g{};
+  g.m = static_cast<uint32_t>(q.m);
+  g.n = static_cast<uint32_t>(q.n);
+  g.k_blocks = static_cast<uint32_t>(ceil_div<size_t>(q.a.by_rows ? q.a.rows : q.a.cols, kOrthK));
   g.tiles_m = static_cast<uint32_t>(ceil_div<size_t>(q.m, kBlockM));
   g.tiles_n = static_cast<uint32_t>(ceil_div<size_t>(q.n, q.shape.bn));
-  g.group_n = (q.shape.bn == 256 || g.tiles_m <= 2) ? 4 : 8;
+  g.group_n = g.tiles_m <= 2 ? 4 : 8;
+  g.per_batch = static_cast<uint32_t>(q.shape.per_batch);
   g.num_tiles = static_cast<uint32_t>(batch * q.shape.per_batch);
-  g.idesc = (1u << 4) | (static_cast<uint32_t>(q.shape.bn >> 3) << 17) |
-            (static_cast<uint32_t>(kBlockM >> 4) << 24);  // fp32 sums, f16 operands
-  g.idesc_neg_a = g.idesc | (1u << 13);
-  g.c = q.c;
-  g.c_layout = kPlanarRow;
-  g.alpha_re = q.alpha;
-  g.beta_re = q.beta;
-  g.have_beta = q.c0 != nullptr ? 1u : 0u;
-  g.c_in = q.c0;
-  g.c_t = q.c_t;
+  g.hermitian = q.hermitian ? 1u : 0u;
   g.conj_b = q.conj ? 1u : 0u;
-  g.hermitian = q.hermitian ? static_cast<uint32_t>(q.shape.per_batch) : 0u;
-  if (q.last) {
-    g.final_type = static_cast<uint32_t>(plan.desc.type_out);
-    g.final_trans = plan.tall ? 1u : 0u;
-    g.final_m = static_cast<uint32_t>(plan.n);
-    g.final_n = static_cast<uint32_t>(plan.l);
-    g.beta_im = 1.0f / plan.scale;
-    g.vec_ok = (!plan.tall && plan.l % 8 == 0 && aligned16(q.c)) ? 1u : 0u;
-  }
+  g.alpha = q.alpha;
+  g.beta = q.beta;
+  g.gain = q.gain;
+  g.c0 = q.c0;
+  g.c0_pitch = static_cast<uint32_t>(q.c0_pitch);
+  g.bf16 = q.bf16 ? 1u : 0u;
+  g.boxes = q.boxes ? 1u : 0u;
+  g.out = static_cast<uint16_t *>(q.out);
+  g.n_out = static_cast<uint32_t>(q.out_pitch);
   g.status = plan.status;
   g.wait_cycles = plan.wait_cycles;
-  CUtensorMap tm_a, tm_b;
-  int rc = make_map(&tm_a, q.a, q.k * 2, q.m, 2 * batch, q.k * 2, q.m * q.k * 2, 128, kBlockM, 2);
+  CUtensorMap tm_a, tm_b, tm_c;
+  int rc = operand_map(&tm_a, q.a, batch, kBlockM);
   if (rc != CCGLIB_B200_OK) return rc;
-  rc = make_map(&tm_b, q.b, q.k * 2, q.n, 2 * batch, q.k * 2, q.n * q.k * 2, 128, q.shape.bn, 2);
+  rc = operand_map(&tm_b, q.b, batch, q.shape.bn);
   if (rc != CCGLIB_B200_OK) return rc;
+  tm_c = tm_a;  // placeholder
+  if (q.boxes) {
+    rc = make_map(&tm_c, q.out, q.out_pitch * 2, q.m, 2 * batch, q.out_pitch * 2, q.m * q.out_pitch * 2,
+                  64, 32, 1);
+    if (rc != CCGLIB_B200_OK) return rc;
+  }
   const unsigned grid = g.num_tiles < static_cast<uint32_t>(plan.sms) ? g.num_tiles : plan.sms;
-  orth_kernel(q.shape.bn)<<<grid, kThreads, orth_smem(q.shape.bn), stream>>>(tm_a, tm_b, tm_a, g);
+  orth_kernel(q.shape.bn, q.a.by_rows, q.b.by_rows)<<<grid, kThreads, orth_smem(q.shape.bn), stream>>>(
+      tm_a, tm_b, tm_c, g);
   CCGLIB_CUDA_TRY(cudaGetLastError());
   return CCGLIB_B200_OK;
 }
@@ -254,8 +661,8 @@ int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q,
 template <typename T>
 int launch_first(const ccglib_b200_orthogonalize_plan &plan, const void *d_in, cudaStream_t stream) {
   const ccglib_b200_orthogonalize_desc &d = plan.desc;
-  const size_t items = d.batch * plan.chunks;
   const size_t cap = static_cast<size_t>(plan.sms) * 8;
+  size_t items = d.batch * plan.chunks;
   norm_kernel<T><<<static_cast<unsigned>(items < cap ? items : cap), kNormThreads, 0, stream>>>(
       static_cast<const T *>(d_in), plan.sums, 2 * d.m * d.n, plan.chunks, items);
   CCGLIB_CUDA_TRY(cudaGetLastError());
@@ -266,14 +673,11 @@ int launch_first(const ccglib_b200_orthogonalize_plan &plan, const void *d_in, c
   p.batch = d.batch;
   p.rows = d.m;
   p.cols = d.n;
-  p.x = plan.x;
-  p.x_t = plan.x_t[0];
-  p.rows_p = plan.tall ? plan.l_p : plan.n_p;
-  p.cols_p = plan.tall ? plan.n_p : plan.l_p;
-  p.tall = plan.tall;
+  p.x = plan.x[0];
+  p.pitch = plan.cols_p;
   p.scale = plan.scale;
-  const size_t tiles = d.batch * ceil_div<size_t>(p.rows_p, kFirstTile) * ceil_div<size_t>(p.cols_p, kFirstTile);
-  const unsigned grid = static_cast<unsigned>(tiles < cap ? tiles : cap);
+  items = d.batch * ceil_div<size_t>(d.m * plan.cols_p, kFirstChunk);
+  const unsigned grid = static_cast<unsigned>(items < cap ? items : cap);
   if (d.input_complex_axis == CCGLIB_B200_INTERLEAVED) {
     first_kernel<T, true><<<grid, 256, 0, stream>>>(p);
   } else {
@@ -331,7 +735,7 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.n = plan.tall ? d.n : d.m;
   plan.l = plan.tall ? d.m : d.n;
   plan.n_p = ceil_div<size_t>(plan.n, 8) * 8;
-  plan.l_p = ceil_div<size_t>(plan.l, 8) * 8;
+  plan.cols_p = ceil_div<size_t>(d.n, 8) * 8;
   plan.scale = std::exp2(std::rint(0.5f * std::log2(static_cast<float>(plan.l))));
   CCGLIB_CUDA_TRY(cudaGetDevice(&plan.device));
   plan.sms = sm_count();
@@ -345,21 +749,24 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.wait_cycles = wait_limit_cycles();
   int rc = device_status_address(&plan.status);
   if (rc != CCGLIB_B200_OK) return rc;
-  plan.gram = pick_shape(d.batch, plan.n_p, plan.n_p, true, plan.sms);
-  plan.update = pick_shape(d.batch, plan.n_p, plan.l_p, false, plan.sms);
-  if (d.batch * plan.gram.per_batch > 0x7FFFFFFFull ||
+  plan.square = pick_shape(d.batch, plan.n, plan.n_p, true, plan.sms);
+  plan.update = pick_shape(d.batch, d.m, plan.cols_p, false, plan.sms);
+  if (d.batch * plan.square.per_batch > 0x7FFFFFFFull ||
       d.batch * plan.update.per_batch > 0x7FFFFFFFull) {
     set_last_error("orthogonalize_plan_create: too many tiles");
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
-  for (int bn : {64, 128, 256}) {
-    CCGLIB_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void *>(orth_kernel(bn)),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, orth_smem(bn)));
+  for (int bn : {64, 128}) {
+    for (int form = 0; form < 3; ++form) {
+      CCGLIB_CUDA_TRY(cudaFuncSetAttribute(
+          reinterpret_cast<const void *>(orth_kernel(bn, form == 2, form >= 1)),
+          cudaFuncAttributeMaxDynamicSharedMemorySize, orth_smem(bn)));
+    }
   }
   plan.chunks = ceil_div<size_t>(2 * d.m * d.n, kNormChunk);
-  const size_t x_bytes = ceil_div<size_t>(d.batch * 2 * plan.n_p * plan.l_p * 2, 256) * 256;
-  const size_t s_bytes = ceil_div<size_t>(d.batch * 2 * plan.n_p * plan.n_p * 2, 256) * 256;
-  plan.scratch_bytes = 3 * x_bytes + 2 * s_bytes + d.batch * plan.chunks * sizeof(double);
+  const size_t x_bytes = ceil_div<size_t>(d.batch * 2 * d.m * plan.cols_p * 2, 256) * 256;
+  const size_t s_bytes = ceil_div<size_t>(d.batch * 2 * plan.n * plan.n_p * 2, 256) * 256;
+  plan.scratch_bytes = 2 * x_bytes + 2 * s_bytes + d.batch * plan.chunks * sizeof(double);
   if (cudaMalloc(&plan.scratch, plan.scratch_bytes) != cudaSuccess) {
     cudaGetLastError();
     set_last_error("orthogonalize_plan_create: could not allocate %zu bytes of workspace",
@@ -372,9 +779,8 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     at += bytes;
     return here;
   };
-  plan.x = reinterpret_cast<__half *>(take(x_bytes));
-  plan.x_t[0] = reinterpret_cast<__half *>(take(x_bytes));
-  plan.x_t[1] = reinterpret_cast<__half *>(take(x_bytes));
+  plan.x[0] = reinterpret_cast<__half *>(take(x_bytes));
+  plan.x[1] = reinterpret_cast<__half *>(take(x_bytes));
   plan.s = reinterpret_cast<__half *>(take(s_bytes));
   plan.p = reinterpret_cast<__half *>(take(s_bytes));
   plan.sums = reinterpret_cast<double *>(at);
@@ -410,22 +816,31 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
   int rc = d.type_in == CCGLIB_B200_FLOAT32   ? launch_first<float>(*plan, d_in, stream)
            : d.type_in == CCGLIB_B200_FLOAT16 ? launch_first<__half>(*plan, d_in, stream)
                                               : launch_first<__nv_bfloat16>(*plan, d_in, stream);
-  const size_t n = plan->n_p, l = plan->l_p;
+  const size_t n = plan->n, n_p = plan->n_p, cols_p = plan->cols_p;
+  const bool tall = plan->tall;
   const float unscale = 1.0f / (plan->scale * plan->scale);
+  const Operand s{plan->s, n, n_p, n_p, false}, p{plan->p, n, n_p, n_p, false};
   for (int step = 0; rc == CCGLIB_B200_OK && step < d.steps; ++step) {
     const bool last = step + 1 == d.steps;
-    __half *now = plan->x_t[step & 1], *next = plan->x_t[(step & 1) ^ 1];
-    const Product gram{plan->x, plan->x, n, n, l, plan->gram, true, true, unscale, 0.0f,
-                       nullptr, plan->s, plan->s, false};
-    rc = launch_product(*plan, gram, stream);
+    // X as an operand: contracted over the long side in S, over the short side in the update
+    const Operand x_long{plan->x[step & 1], d.m, cols_p, cols_p, tall};
+    Operand x_short = x_long;
+    x_short.by_rows = !tall;
+    rc = launch_product(*plan, {x_long, x_long, n, n_p, plan->square, true, true, unscale, 0.0f, 1.0f,
+                                nullptr, 0, plan->s, n_p, true, false}, stream);
     if (rc != CCGLIB_B200_OK) break;
-    const Product poly{plan->s, plan->s, n, n, n, plan->gram, true, true, d.c, d.b,
-                       plan->s, plan->p, plan->p, false};
-    rc = launch_product(*plan, poly, stream);
+    rc = launch_product(*plan, {s, s, n, n_p, plan->square, true, true, d.c, d.b, 1.0f, plan->s, n_p,
+                                plan->p, n_p, true, false}, stream);
     if (rc != CCGLIB_B200_OK) break;
-    // (X is read as C0 and written by the same thread; the operand is its transpose)
-    const Product update{plan->p, now, n, l, n, plan->update, false, false, 1.0f, d.a,
-                         plan->x, last ? d_out : plan->x, last ? nullptr : next, last};
+    Product update{tall ? x_short : p, tall ? p : x_short, d.m, cols_p, plan->update, false, false, 1.0f,
+                   d.a, 1.0f, plan->x[step & 1], cols_p, plan->x[(step & 1) ^ 1], cols_p, true, false};
+    if (last) {
+      update.gain = 1.0f / plan->scale;
+      update.out = d_out;
+      update.out_pitch = d.n;
+      update.boxes = d.n % 8 == 0 && aligned16(d_out);
+      update.bf16 = d.type_out == CCGLIB_B200_BFLOAT16;
+    }
     rc = launch_product(*plan, update, stream);
   }
   return rc;
