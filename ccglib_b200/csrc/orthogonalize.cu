@@ -490,11 +490,31 @@ template <> __device__ __forceinline__ float as_float(float v) { return v; }
 template <> __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// Eight consecutive values from a 16-byte aligned address.
+__device__ __forceinline__ void load8(const float *src, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4 *>(src)[0];
+  const float4 b = reinterpret_cast<const float4 *>(src)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <typename T> __device__ __forceinline__ void load8(const T *src, float (&v)[8]) {
+  const uint4 q = *reinterpret_cast<const uint4 *>(src);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T *h = reinterpret_cast<const T *>(&w[i]);
+    v[2 * i] = as_float(h[0]);
+    v[2 * i + 1] = as_float(h[1]);
+  }
+}
+
 constexpr int kNormThreads = 256;
 constexpr size_t kNormChunk = 16384;  // values one CTA adds up
 
-// Sums of squares of kNormChunk values each, in float64 (no input overflows or vanishes in it).
-template <typename T>
+// Sums of squares of kNormChunk values each.  Eight values at a time in float32, where that neither
+// overflows nor vanishes (else in float64); these in float64.  Memory-bound: converting every value to
+// float64 took four times as long.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kNormThreads)
 norm_kernel(const T *in, double *sums, size_t values, size_t chunks, size_t items) {
   __shared__ double part[kNormThreads / 32];
@@ -503,9 +523,24 @@ norm_kernel(const T *in, double *sums, size_t values, size_t chunks, size_t item
     const T *src = in + b * values;
     const size_t end = min(values, (c + 1) * kNormChunk);
     double sum = 0.0;
-    for (size_t i = c * kNormChunk + threadIdx.x; i < end; i += kNormThreads) {
-      const double v = static_cast<double>(as_float(src[i]));
-      sum += v * v;
+#pragma unroll 4
+    for (size_t i = c * kNormChunk + threadIdx.x * 8; i < end; i += kNormThreads * 8) {
+      float v[8];
+      if constexpr (VEC) {  // `values` is a multiple of eight
+        load8(src + i, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = i + j < end ? as_float(src[i + j]) : 0.0f;
+      }
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fmaf(v[j], v[j], s);
+      if (s > 1e-24f && s < 1e38f) {
+        sum += s;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += static_cast<double>(v[j]) * v[j];
+      }
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
@@ -528,10 +563,10 @@ struct FirstParams {
   float scale;
 };
 
-constexpr size_t kFirstChunk = 4096;  // complex values (padded rows) one CTA converts
+constexpr size_t kFirstChunk = 8192;  // complex values (padded rows) one CTA converts
 
-// X0 = scale * input / norm.
-template <typename T, bool IL>
+// X0 = scale * input / norm.  VEC: rows need no padding, the planes are converted as they lie.
+template <typename T, bool IL, bool VEC>
 __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
   __shared__ double part[256 / 32];
   const size_t plane = p.rows * p.pitch, per_batch = ceil_div<size_t>(plane, kFirstChunk);
@@ -545,24 +580,65 @@ __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < 256 / 32; ++w) sum += part[w];
-    // a zero matrix stays zero (and one with a NaN becomes NaN)
+    // A zero matrix stays zero (and one with a NaN becomes NaN).  A factor outside float32's comfortable
+    // range is applied in two steps that are inside it: |x| * factor is at most scale.
     const double factor = sum == 0.0 ? 0.0 : static_cast<double>(p.scale) / sqrt(sum);
+    const double half = factor < 1e-30 ? 1e-25 : factor > 1e30 ? 1e25 : 1.0;
+    const float f0 = static_cast<float>(half), f1 = static_cast<float>(factor / half);
     const T *in = static_cast<const T *>(p.in) + b * 2 * p.rows * p.cols;
     __half *x = p.x + b * 2 * plane;
     const size_t first = (item - b * per_batch) * kFirstChunk;
+    const size_t end = min(plane, first + kFirstChunk);
+    if constexpr (VEC) {
 #pragma unroll 4
-    for (size_t i = first + threadIdx.x; i < min(plane, first + kFirstChunk); i += 256) {
-      const size_t r = i / p.pitch, c = i - r * p.pitch;
-      float re = 0.0f, im = 0.0f;
-      if (c < p.cols) {
-        const size_t s = r * p.cols + c;
-        re = as_float(IL ? in[2 * s] : in[s]);
-        im = as_float(IL ? in[2 * s + 1] : in[s + p.rows * p.cols]);
+      for (size_t i = first + threadIdx.x * 8; i < end; i += 256 * 8) {
+        float v[2][8];
+        load8(IL ? in + 2 * i : in + i, v[0]);
+        load8(IL ? in + 2 * i + 8 : in + i + plane, v[1]);
+        __half2 re[4], im[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // interleaved: pairs 2j, 2j + 1 of the 16 values
+          const float r0 = IL ? v[j / 2][(4 * j) & 7] : v[0][2 * j];
+          const float i0 = IL ? v[j / 2][(4 * j + 1) & 7] : v[1][2 * j];
+          const float r1 = IL ? v[j / 2][(4 * j + 2) & 7] : v[0][2 * j + 1];
+          const float i1 = IL ? v[j / 2][(4 * j + 3) & 7] : v[1][2 * j + 1];
+          re[j] = __floats2half2_rn(r0 * f0 * f1, r1 * f0 * f1);
+          im[j] = __floats2half2_rn(i0 * f0 * f1, i1 * f0 * f1);
+        }
+        *reinterpret_cast<uint4 *>(x + i) = *reinterpret_cast<const uint4 *>(re);
+        *reinterpret_cast<uint4 *>(x + i + plane) = *reinterpret_cast<const uint4 *>(im);
       }
-      x[i] = __float2half_rn(static_cast<float>(re * factor));
-      x[i + plane] = __float2half_rn(static_cast<float>(im * factor));
+    } else {
+#pragma unroll 4
+      for (size_t i = first + threadIdx.x; i < end; i += 256) {
+        const size_t r = i / p.pitch, c = i - r * p.pitch;
+        float re = 0.0f, im = 0.0f;
+        if (c < p.cols) {
+          const size_t s = r * p.cols + c;
+          re = as_float(IL ? in[2 * s] : in[s]);
+          im = as_float(IL ? in[2 * s + 1] : in[s + p.rows * p.cols]);
+        }
+        x[i] = __float2half_rn(re * f0 * f1);
+        x[i + plane] = __float2half_rn(im * f0 * f1);
+      }
     }
     __syncthreads();
+  }
+}
+
+template <typename T>
+void launch_first_form(const FirstParams &p, bool il, bool vec, unsigned grid, cudaStream_t stream) {
+  if (il) {
+    if (vec) {
+      first_kernel<T, true, true><<<grid, 256, 0, stream>>>(p);
+    } else {
+      first_kernel<T, true, false><<<grid, 256, 0, stream>>>(p);
+    }
+  } else if (vec) {
+    first_kernel<T, false, true><<<grid, 256, 0, stream>>>(p);
+  } else {
+    first_kernel<T, false, false><<<grid, 256, 0, stream>>>(p);
   }
 }
 
@@ -663,8 +739,13 @@ int launch_first(const ccglib_b200_orthogonalize_plan &plan, const void *d_in, c
   const ccglib_b200_orthogonalize_desc &d = plan.desc;
   const size_t cap = static_cast<size_t>(plan.sms) * 8;
   size_t items = d.batch * plan.chunks;
-  norm_kernel<T><<<static_cast<unsigned>(items < cap ? items : cap), kNormThreads, 0, stream>>>(
-      static_cast<const T *>(d_in), plan.sums, 2 * d.m * d.n, plan.chunks, items);
+  unsigned grid = static_cast<unsigned>(items < cap ? items : cap);
+  const T *in = static_cast<const T *>(d_in);
+  if (aligned16(d_in) && 2 * d.m * d.n % 8 == 0) {
+    norm_kernel<T, true><<<grid, kNormThreads, 0, stream>>>(in, plan.sums, 2 * d.m * d.n, plan.chunks, items);
+  } else {
+    norm_kernel<T, false><<<grid, kNormThreads, 0, stream>>>(in, plan.sums, 2 * d.m * d.n, plan.chunks, items);
+  }
   CCGLIB_CUDA_TRY(cudaGetLastError());
   FirstParams p{};
   p.in = d_in;
@@ -677,12 +758,9 @@ int launch_first(const ccglib_b200_orthogonalize_plan &plan, const void *d_in, c
   p.pitch = plan.cols_p;
   p.scale = plan.scale;
   items = d.batch * ceil_div<size_t>(d.m * plan.cols_p, kFirstChunk);
-  const unsigned grid = static_cast<unsigned>(items < cap ? items : cap);
-  if (d.input_complex_axis == CCGLIB_B200_INTERLEAVED) {
-    first_kernel<T, true><<<grid, 256, 0, stream>>>(p);
-  } else {
-    first_kernel<T, false><<<grid, 256, 0, stream>>>(p);
-  }
+  grid = static_cast<unsigned>(items < cap ? items : cap);
+  launch_first_form<T>(p, d.input_complex_axis == CCGLIB_B200_INTERLEAVED,
+                       d.n % 8 == 0 && aligned16(d_in), grid, stream);
   CCGLIB_CUDA_TRY(cudaGetLastError());
   return CCGLIB_B200_OK;
 }
