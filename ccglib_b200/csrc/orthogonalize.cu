@@ -19,6 +19,7 @@
 // took the error of eight steps of the steep quintic from 2.1e-3 to 3.7e-3.)  Error of the result, rms:
 // 0.7e-3 after eight steps that converge, 1.2 to 2.5e-3 after 5 to 8 of the quintic.
 #include <cmath>
+#include <cstdlib>
 #include <new>
 
 #include "gemm_kernels.cuh"
@@ -91,6 +92,15 @@ __device__ __forceinline__ TileCoord orth_tile(const OrthParams &p, uint32_t til
   t.mt = r / width;
   t.nt = first_n + (r - t.mt * width);
   return t;
+}
+
+// Products follow one another with programmatic launch: a product's CTAs may set up (barriers, tensor
+// memory, descriptors) while the product before it drains, and wait here before they touch memory.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi, bool bf16) {
@@ -260,9 +270,11 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  let_next_start();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
+    wait_for_previous();
     uint32_t stage = 0, phase = 0, issued = 0;
     bool ok = true;
     for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
@@ -387,6 +399,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
     }
   } else {
     // ------------------------------------------------------------------ epilogue warps
+    wait_for_previous();
     const uint32_t quad = warp & 3;
     const uint32_t staging = smem_base + kStages * C::kStageBytes + quad * (4 * kOrthBox);
     uint32_t acc = 0, acc_phase = 0;
@@ -642,6 +655,249 @@ void launch_first_form(const FirstParams &p, bool il, bool vec, unsigned grid, c
   }
 }
 
+// ---- small matrices: the whole iteration in one CTA ------------------------------------------------
+//
+// X (twice), S and P in shared memory, float32 throughout, one launch: for matrices whose products are
+// too small for 128-row tiles and a launch each.  X is kept transposed, V[l][i]: with S and P
+// Hermitian, every product then reads rows of four consecutive values,
+//   S_ij = sum_l V[l][i] conj(V[l][j]),  (S S)_ij = sum_k conj(S[k][i]) S[k][j],
+//   V'[l][i] = a V[l][i] + sum_j conj(P[j][i]) V[l][j].
+// A thread computes 4 x 4 values: 64 multiply-adds on four 16-byte loads.
+
+constexpr int kSmallThreads = 256;
+constexpr size_t kSmallMaxSide = 64;
+
+struct SmallParams {
+  const void *in;
+  void *out;
+  size_t batch, m, n;  // as the caller holds them
+  uint32_t s, l, sp;   // short and long side, short side rounded up to four
+  bool tall;
+  int type_in, bf16, inter, steps;
+  float a, b, c;
+};
+
+size_t small_smem(size_t s, size_t l) {
+  const size_t sp = ceil_div<size_t>(s, 4) * 4;
+  return (2 * 2 * l * sp + 2 * 2 * sp * sp) * sizeof(float);
+}
+
+// Four rows' worth of complex values.
+struct Quad {
+  float re[4], im[4];
+};
+__device__ __forceinline__ Quad load_quad(const float *re, const float *im) {
+  const float4 r = *reinterpret_cast<const float4 *>(re), i = *reinterpret_cast<const float4 *>(im);
+  return {{r.x, r.y, r.z, r.w}, {i.x, i.y, i.z, i.w}};
+}
+__device__ __forceinline__ void store_quad(float *re, float *im, const Quad &q) {
+  *reinterpret_cast<float4 *>(re) = make_float4(q.re[0], q.re[1], q.re[2], q.re[3]);
+  *reinterpret_cast<float4 *>(im) = make_float4(q.im[0], q.im[1], q.im[2], q.im[3]);
+}
+
+// H_ij = sum_k conj(v[k][i]) v[k][j] for all i, j (Hermitian), `rows` rows of sp values; each 4 x 4 block on
+// or above the diagonal by `lanes` neighbouring threads that deal out k; store(i, j, H_ij).
+template <typename Store>
+__device__ __forceinline__ void gram_blocks(const float *re, const float *im, uint32_t rows, uint32_t sp,
+                                            uint32_t lanes, Store store) {
+  const uint32_t nb = sp / 4, pairs = nb * (nb + 1) / 2;
+  const uint32_t sub = threadIdx.x % lanes;
+  // every thread of a warp takes the same number of turns: the shuffles need all of them
+  const uint32_t turns = ceil_div<uint32_t>(pairs, kSmallThreads / lanes);
+  for (uint32_t turn = 0; turn < turns; ++turn) {
+    const uint32_t pair = turn * (kSmallThreads / lanes) + threadIdx.x / lanes;
+    uint32_t bi = 0, bj = pair;
+    if (pair < pairs) {
+      while (bj >= nb - bi) {
+        bj -= nb - bi;
+        ++bi;
+      }
+      bj += bi;
+    } else {
+      bj = 0;
+    }
+    float hr[4][4], hi[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) hr[i][j] = hi[i][j] = 0.0f;
+    }
+    if (pair < pairs) {
+      for (uint32_t k = sub; k < rows; k += lanes) {
+        const Quad u = load_quad(re + k * sp + 4 * bi, im + k * sp + 4 * bi);
+        const Quad v = load_quad(re + k * sp + 4 * bj, im + k * sp + 4 * bj);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            hr[i][j] = fmaf(u.re[i], v.re[j], fmaf(u.im[i], v.im[j], hr[i][j]));
+            hi[i][j] = fmaf(u.re[i], v.im[j], fmaf(-u.im[i], v.re[j], hi[i][j]));
+          }
+        }
+      }
+    }
+    for (uint32_t o = lanes / 2; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          hr[i][j] += __shfl_xor_sync(0xFFFFFFFFu, hr[i][j], o);
+          hi[i][j] += __shfl_xor_sync(0xFFFFFFFFu, hi[i][j], o);
+        }
+      }
+    }
+    if (pair < pairs && sub == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store(4 * bi + i, 4 * bj + j, hr[i][j], hi[i][j]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float load_value(const void *in, size_t i, int type) {
+  return type == CCGLIB_B200_FLOAT32   ? static_cast<const float *>(in)[i]
+         : type == CCGLIB_B200_FLOAT16 ? __half2float(static_cast<const __half *>(in)[i])
+                                       : __bfloat162float(static_cast<const __nv_bfloat16 *>(in)[i]);
+}
+
+// The largest power of two <= x, at most 32.
+__device__ __forceinline__ uint32_t lanes_for(uint32_t work) {
+  uint32_t lanes = 1;
+  while (lanes < 32 && lanes * 2 <= work) lanes *= 2;
+  return lanes;
+}
+
+__global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams p) {
+  extern __shared__ __align__(16) float small_smem_raw[];
+  __shared__ double part[kSmallThreads / 32];
+  const uint32_t sp = p.sp, l = p.l;
+  float *x_re[2], *x_im[2];
+  float *at = small_smem_raw;
+  for (int i = 0; i < 2; ++i) {
+    x_re[i] = at;
+    x_im[i] = at + l * sp;
+    at += 2 * l * sp;
+  }
+  float *s_re = at, *s_im = at + sp * sp, *p_re = at + 2 * sp * sp, *p_im = at + 3 * sp * sp;
+  const uint32_t nb = sp / 4, pairs = nb * (nb + 1) / 2;
+  const uint32_t lanes = lanes_for(kSmallThreads / pairs);
+  const size_t plane = p.m * p.n;
+  for (size_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    // X and its norm (float64: no input overflows or vanishes in it)
+    double sum = 0.0;
+    for (uint32_t i = threadIdx.x; i < l * sp; i += kSmallThreads) {
+      const uint32_t row = i / sp, col = i - row * sp;  // V[row][col]
+      float re = 0.0f, im = 0.0f;
+      if (col < p.s) {
+        const size_t e = p.tall ? static_cast<size_t>(row) * p.n + col : static_cast<size_t>(col) * p.n + row;
+        const size_t base = b * 2 * plane;
+        re = load_value(p.in, base + (p.inter ? 2 * e : e), p.type_in);
+        im = load_value(p.in, base + (p.inter ? 2 * e + 1 : e + plane), p.type_in);
+      }
+      x_re[0][i] = re;
+      x_im[0][i] = im;
+      sum += static_cast<double>(re) * re + static_cast<double>(im) * im;
+    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < kSmallThreads / 32; ++w) sum += part[w];
+    const double factor = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
+    for (uint32_t i = threadIdx.x; i < l * sp; i += kSmallThreads) {
+      x_re[0][i] = static_cast<float>(x_re[0][i] * factor);
+      x_im[0][i] = static_cast<float>(x_im[0][i] * factor);
+    }
+    __syncthreads();
+    for (int step = 0; step < p.steps; ++step) {
+      const int now = step & 1;
+      const float *xr = x_re[now], *xi = x_im[now];
+      float *yr = x_re[now ^ 1], *yi = x_im[now ^ 1];
+      gram_blocks(xr, xi, l, sp, lanes, [&](uint32_t i, uint32_t j, float hr, float hi) {
+        // S_ij = conj(H_ij)
+        if (i <= j) {
+          s_re[i * sp + j] = hr;
+          s_im[i * sp + j] = i == j ? 0.0f : -hi;
+          if (i < j) {
+            s_re[j * sp + i] = hr;
+            s_im[j * sp + i] = hi;
+          }
+        }
+      });
+      __syncthreads();
+      gram_blocks(s_re, s_im, sp, sp, lanes, [&](uint32_t i, uint32_t j, float hr, float hi) {
+        if (i <= j) {
+          const float re = p.b * s_re[i * sp + j] + p.c * hr;
+          const float im = i == j ? 0.0f : p.b * s_im[i * sp + j] + p.c * hi;
+          p_re[i * sp + j] = re;
+          p_im[i * sp + j] = im;
+          if (i < j) {
+            p_re[j * sp + i] = re;
+            p_im[j * sp + i] = -im;
+          }
+        }
+      });
+      __syncthreads();
+      // four rows l0 .. l0 + 3 of V' x four columns
+      const uint32_t lb = ceil_div<uint32_t>(l, 4);
+      for (uint32_t t = threadIdx.x; t < lb * nb; t += kSmallThreads) {
+        const uint32_t i0 = t % nb * 4, l0 = t / nb * 4;
+        float vr[4][4], vi[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[r][i] = vi[r][i] = 0.0f;
+        }
+        for (uint32_t j = 0; j < sp; j += 4) {
+          Quad x[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t row = min(l0 + r, l - 1);
+            x[r] = load_quad(xr + row * sp + j, xi + row * sp + j);
+          }
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            const Quad q = load_quad(p_re + (j + jj) * sp + i0, p_im + (j + jj) * sp + i0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float cr = x[r].re[jj], ci = x[r].im[jj];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                vr[r][i] = fmaf(q.re[i], cr, fmaf(q.im[i], ci, vr[r][i]));
+                vi[r][i] = fmaf(q.re[i], ci, fmaf(-q.im[i], cr, vi[r][i]));
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (l0 + r < l) {
+            Quad q = load_quad(xr + (l0 + r) * sp + i0, xi + (l0 + r) * sp + i0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              q.re[i] = fmaf(p.a, q.re[i], vr[r][i]);
+              q.im[i] = fmaf(p.a, q.im[i], vi[r][i]);
+            }
+            store_quad(yr + (l0 + r) * sp + i0, yi + (l0 + r) * sp + i0, q);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    const float *xr = x_re[p.steps & 1], *xi = x_im[p.steps & 1];
+    uint16_t *out = static_cast<uint16_t *>(p.out) + b * 2 * plane;
+    for (uint32_t e = threadIdx.x; e < plane; e += kSmallThreads) {
+      const uint32_t row = e / static_cast<uint32_t>(p.n), col = e - row * static_cast<uint32_t>(p.n);
+      const uint32_t i = p.tall ? row * sp + col : col * sp + row;
+      out[e] = round_half(xr[i], p.bf16);
+      out[e + plane] = round_half(xi[i], p.bf16);
+    }
+    __syncthreads();
+  }
+}
+
 } // namespace
 } // namespace ccglib_b200
 
@@ -654,6 +910,7 @@ struct ccglib_b200_orthogonalize_plan {
   bool tall;            // m > n
   float scale;          // power of two near sqrt(long side)
   ProductShape square, update;
+  bool small;           // the whole iteration in one launch, a CTA per matrix
   size_t chunks;
   int device, sms;
   long long wait_cycles;
@@ -728,9 +985,18 @@ int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q,
     if (rc != CCGLIB_B200_OK) return rc;
   }
   const unsigned grid = g.num_tiles < static_cast<uint32_t>(plan.sms) ? g.num_tiles : plan.sms;
-  orth_kernel(q.shape.bn, q.a.by_rows, q.b.by_rows)<<<grid, kThreads, orth_smem(q.shape.bn), stream>>>(
-      tm_a, tm_b, tm_c, g);
-  CCGLIB_CUDA_TRY(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = orth_smem(q.shape.bn);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  CCGLIB_CUDA_TRY(cudaLaunchKernelEx(&cfg, orth_kernel(q.shape.bn, q.a.by_rows, q.b.by_rows), tm_a, tm_b,
+                                     tm_c, g));
   return CCGLIB_B200_OK;
 }
 
@@ -827,6 +1093,20 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.wait_cycles = wait_limit_cycles();
   int rc = device_status_address(&plan.status);
   if (rc != CCGLIB_B200_OK) return rc;
+  const size_t smem = small_smem(plan.n, plan.l);
+  plan.small = plan.n <= kSmallMaxSide && smem <= static_cast<size_t>(kMaxSmem - 1024);
+  if (const char *v = std::getenv("CCGLIB_B200_ORTH_SMALL")) plan.small = plan.small && std::atoi(v) != 0;
+  if (plan.small) {
+    CCGLIB_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void *>(small_kernel),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kMaxSmem - 1024));
+    *out = new (std::nothrow) ccglib_b200_orthogonalize_plan(plan);
+    if (*out == nullptr) {
+      set_last_error("orthogonalize_plan_create: out of host memory");
+      return CCGLIB_B200_OUT_OF_MEMORY;
+    }
+    return CCGLIB_B200_OK;
+  }
   plan.square = pick_shape(d.batch, plan.n, plan.n_p, true, plan.sms);
   plan.update = pick_shape(d.batch, d.m, plan.cols_p, false, plan.sms);
   if (d.batch * plan.square.per_batch > 0x7FFFFFFFull ||
@@ -891,6 +1171,30 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (plan->small) {
+    SmallParams q{};
+    q.in = d_in;
+    q.out = d_out;
+    q.batch = d.batch;
+    q.m = d.m;
+    q.n = d.n;
+    q.s = static_cast<uint32_t>(plan->n);
+    q.l = static_cast<uint32_t>(plan->l);
+    q.sp = static_cast<uint32_t>(ceil_div<size_t>(plan->n, 4) * 4);
+    q.tall = plan->tall;
+    q.type_in = d.type_in;
+    q.bf16 = d.type_out == CCGLIB_B200_BFLOAT16;
+    q.inter = d.input_complex_axis == CCGLIB_B200_INTERLEAVED;
+    q.steps = d.steps;
+    q.a = d.a;
+    q.b = d.b;
+    q.c = d.c;
+    const size_t cap = static_cast<size_t>(plan->sms) * 8;
+    small_kernel<<<static_cast<unsigned>(d.batch < cap ? d.batch : cap), kSmallThreads,
+                   small_smem(plan->n, plan->l), stream>>>(q);
+    CCGLIB_CUDA_TRY(cudaGetLastError());
+    return CCGLIB_B200_OK;
+  }
   int rc = d.type_in == CCGLIB_B200_FLOAT32   ? launch_first<float>(*plan, d_in, stream)
            : d.type_in == CCGLIB_B200_FLOAT16 ? launch_first<__half>(*plan, d_in, stream)
                                               : launch_first<__nv_bfloat16>(*plan, d_in, stream);
