@@ -662,9 +662,9 @@ void launch_first_form(const FirstParams &p, bool il, bool vec, unsigned grid, c
 // Hermitian, every product then reads rows of four consecutive values,
 //   S_ij = sum_l V[l][i] conj(V[l][j]),  (S S)_ij = sum_k conj(S[k][i]) S[k][j],
 //   V'[l][i] = a V[l][i] + sum_j conj(P[j][i]) V[l][j].
-// A thread computes 4 x 4 values: 64 multiply-adds on four 16-byte loads.
 
-constexpr int kSmallThreads = 256;
+constexpr int kSmallThreads = 512;
+constexpr int kSmallRows = 2;  // rows of V' per thread in the update
 constexpr size_t kSmallMaxSide = 64;
 
 struct SmallParams {
@@ -695,62 +695,59 @@ __device__ __forceinline__ void store_quad(float *re, float *im, const Quad &q) 
   *reinterpret_cast<float4 *>(im) = make_float4(q.im[0], q.im[1], q.im[2], q.im[3]);
 }
 
-// H_ij = sum_k conj(v[k][i]) v[k][j] for all i, j (Hermitian), `rows` rows of sp values; each 4 x 4 block on
-// or above the diagonal by `lanes` neighbouring threads that deal out k; store(i, j, H_ij).
+// H_ij = sum_k conj(v[k][i]) v[k][j] for all i <= j (Hermitian), `rows` rows of sp values; each 2 x 2 block
+// on or above the diagonal by `lanes` neighbouring threads that deal out k.  store(i, j, H_ij) for
+// i <= j.  (Larger blocks load less, but the unrolled sums of k over lanes made the step as long as its
+// code: instructions arrive no faster than a few clocks each when they run once.)
 template <typename Store>
 __device__ __forceinline__ void gram_blocks(const float *re, const float *im, uint32_t rows, uint32_t sp,
                                             uint32_t lanes, Store store) {
-  const uint32_t nb = sp / 4, pairs = nb * (nb + 1) / 2;
-  const uint32_t sub = threadIdx.x % lanes;
-  // every thread of a warp takes the same number of turns: the shuffles need all of them
-  const uint32_t turns = ceil_div<uint32_t>(pairs, kSmallThreads / lanes);
-  for (uint32_t turn = 0; turn < turns; ++turn) {
-    const uint32_t pair = turn * (kSmallThreads / lanes) + threadIdx.x / lanes;
-    uint32_t bi = 0, bj = pair;
-    if (pair < pairs) {
-      while (bj >= nb - bi) {
-        bj -= nb - bi;
-        ++bi;
-      }
-      bj += bi;
-    } else {
-      bj = 0;
+  const uint32_t nb = sp / 2, pairs = nb * (nb + 1) / 2;
+  const uint32_t sub = threadIdx.x % lanes, per_turn = kSmallThreads / lanes;
+  // a warp goes on while any of its groups has a block: the shuffles need all of them
+  const uint32_t warp_first = (threadIdx.x & ~31u) / lanes;
+#pragma unroll 1
+  for (uint32_t turn = 0; turn + warp_first < pairs; turn += per_turn) {
+    const uint32_t pair = turn + threadIdx.x / lanes;
+    const bool on = pair < pairs;
+    uint32_t bi = 0, bj = on ? pair : 0;
+    while (bj >= nb - bi) {
+      bj -= nb - bi;
+      ++bi;
     }
-    float hr[4][4], hi[4][4];
+    bj += bi;
+    float h[2][2][2] = {};
+#pragma unroll 2
+    for (uint32_t k = sub; k < rows; k += lanes) {
+      const float2 ur = *reinterpret_cast<const float2 *>(re + k * sp + 2 * bi);
+      const float2 ui = *reinterpret_cast<const float2 *>(im + k * sp + 2 * bi);
+      const float2 vr = *reinterpret_cast<const float2 *>(re + k * sp + 2 * bj);
+      const float2 vi = *reinterpret_cast<const float2 *>(im + k * sp + 2 * bj);
+      const float u[2][2] = {{ur.x, ui.x}, {ur.y, ui.y}}, v[2][2] = {{vr.x, vi.x}, {vr.y, vi.y}};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) hr[i][j] = hi[i][j] = 0.0f;
-    }
-    if (pair < pairs) {
-      for (uint32_t k = sub; k < rows; k += lanes) {
-        const Quad u = load_quad(re + k * sp + 4 * bi, im + k * sp + 4 * bi);
-        const Quad v = load_quad(re + k * sp + 4 * bj, im + k * sp + 4 * bj);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            hr[i][j] = fmaf(u.re[i], v.re[j], fmaf(u.im[i], v.im[j], hr[i][j]));
-            hi[i][j] = fmaf(u.re[i], v.im[j], fmaf(-u.im[i], v.re[j], hi[i][j]));
-          }
+        for (int j = 0; j < 2; ++j) {
+          h[i][j][0] = fmaf(u[i][0], v[j][0], fmaf(u[i][1], v[j][1], h[i][j][0]));
+          h[i][j][1] = fmaf(u[i][0], v[j][1], fmaf(-u[i][1], v[j][0], h[i][j][1]));
         }
       }
     }
+#pragma unroll 1
     for (uint32_t o = lanes / 2; o > 0; o >>= 1) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          hr[i][j] += __shfl_xor_sync(0xFFFFFFFFu, hr[i][j], o);
-          hi[i][j] += __shfl_xor_sync(0xFFFFFFFFu, hi[i][j], o);
-        }
+      for (int i = 0; i < 8; ++i) {
+        float &x = (&h[0][0][0])[i];
+        x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
       }
     }
-    if (pair < pairs && sub == 0) {
+    if (on && sub == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) store(4 * bi + i, 4 * bj + j, hr[i][j], hi[i][j]);
+        for (int j = 0; j < 2; ++j) {
+          if (2 * bi + i <= 2 * bj + j) store(2 * bi + i, 2 * bj + j, h[i][j][0], h[i][j][1]);
+        }
       }
     }
   }
@@ -762,10 +759,10 @@ __device__ __forceinline__ float load_value(const void *in, size_t i, int type) 
                                        : __bfloat162float(static_cast<const __nv_bfloat16 *>(in)[i]);
 }
 
-// The largest power of two <= x, at most 32.
-__device__ __forceinline__ uint32_t lanes_for(uint32_t work) {
+// Threads per block: all there are, but at least four k for each.
+__device__ __forceinline__ uint32_t lanes_for(uint32_t pairs, uint32_t rows) {
   uint32_t lanes = 1;
-  while (lanes < 32 && lanes * 2 <= work) lanes *= 2;
+  while (lanes < 32 && lanes * 2 * pairs <= kSmallThreads && lanes * 8 <= rows) lanes *= 2;
   return lanes;
 }
 
@@ -773,16 +770,12 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
   extern __shared__ __align__(16) float small_smem_raw[];
   __shared__ double part[kSmallThreads / 32];
   const uint32_t sp = p.sp, l = p.l;
-  float *x_re[2], *x_im[2];
-  float *at = small_smem_raw;
-  for (int i = 0; i < 2; ++i) {
-    x_re[i] = at;
-    x_im[i] = at + l * sp;
-    at += 2 * l * sp;
-  }
+  const uint32_t x_size = l * sp;
+  float *x0 = small_smem_raw, *x1 = x0 + 2 * x_size;  // Re, Im of V, twice
+  float *at = x1 + 2 * x_size;
   float *s_re = at, *s_im = at + sp * sp, *p_re = at + 2 * sp * sp, *p_im = at + 3 * sp * sp;
-  const uint32_t nb = sp / 4, pairs = nb * (nb + 1) / 2;
-  const uint32_t lanes = lanes_for(kSmallThreads / pairs);
+  const uint32_t nb = sp / 4, pairs = (sp / 2) * (sp / 2 + 1) / 2;
+  const uint32_t lanes_l = lanes_for(pairs, l), lanes_s = lanes_for(pairs, sp);
   const size_t plane = p.m * p.n;
   for (size_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
     // X and its norm (float64: no input overflows or vanishes in it)
@@ -796,8 +789,8 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
         re = load_value(p.in, base + (p.inter ? 2 * e : e), p.type_in);
         im = load_value(p.in, base + (p.inter ? 2 * e + 1 : e + plane), p.type_in);
       }
-      x_re[0][i] = re;
-      x_im[0][i] = im;
+      x0[i] = re;
+      x0[i + x_size] = im;
       sum += static_cast<double>(re) * re + static_cast<double>(im) * im;
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -807,53 +800,48 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
     for (int w = 0; w < kSmallThreads / 32; ++w) sum += part[w];
     const double factor = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
     for (uint32_t i = threadIdx.x; i < l * sp; i += kSmallThreads) {
-      x_re[0][i] = static_cast<float>(x_re[0][i] * factor);
-      x_im[0][i] = static_cast<float>(x_im[0][i] * factor);
+      x0[i] = static_cast<float>(x0[i] * factor);
+      x0[i + x_size] = static_cast<float>(x0[i + x_size] * factor);
     }
     __syncthreads();
     for (int step = 0; step < p.steps; ++step) {
-      const int now = step & 1;
-      const float *xr = x_re[now], *xi = x_im[now];
-      float *yr = x_re[now ^ 1], *yi = x_im[now ^ 1];
-      gram_blocks(xr, xi, l, sp, lanes, [&](uint32_t i, uint32_t j, float hr, float hi) {
+      const float *xr = (step & 1) ? x1 : x0, *xi = xr + x_size;
+      float *yr = (step & 1) ? x0 : x1, *yi = yr + x_size;
+      gram_blocks(xr, xi, l, sp, lanes_l, [&](uint32_t i, uint32_t j, float re, float im) {
         // S_ij = conj(H_ij)
-        if (i <= j) {
-          s_re[i * sp + j] = hr;
-          s_im[i * sp + j] = i == j ? 0.0f : -hi;
-          if (i < j) {
-            s_re[j * sp + i] = hr;
-            s_im[j * sp + i] = hi;
-          }
-        }
+        const uint32_t ij = i * sp + j, ji = j * sp + i;
+        im = i == j ? 0.0f : im;
+        s_re[ij] = re;
+        s_im[ij] = -im;
+        s_re[ji] = re;
+        s_im[ji] = im;
       });
       __syncthreads();
-      gram_blocks(s_re, s_im, sp, sp, lanes, [&](uint32_t i, uint32_t j, float hr, float hi) {
-        if (i <= j) {
-          const float re = p.b * s_re[i * sp + j] + p.c * hr;
-          const float im = i == j ? 0.0f : p.b * s_im[i * sp + j] + p.c * hi;
-          p_re[i * sp + j] = re;
-          p_im[i * sp + j] = im;
-          if (i < j) {
-            p_re[j * sp + i] = re;
-            p_im[j * sp + i] = -im;
-          }
-        }
+      gram_blocks(s_re, s_im, sp, sp, lanes_s, [&](uint32_t i, uint32_t j, float re, float im) {
+        const uint32_t ij = i * sp + j, ji = j * sp + i;
+        re = p.b * s_re[ij] + p.c * re;
+        im = i == j ? 0.0f : p.b * s_im[ij] + p.c * im;
+        p_re[ij] = re;
+        p_im[ij] = im;
+        p_re[ji] = re;
+        p_im[ji] = -im;
       });
       __syncthreads();
-      // four rows l0 .. l0 + 3 of V' x four columns
-      const uint32_t lb = ceil_div<uint32_t>(l, 4);
+      // kSmallRows rows of V' x four columns
+      const uint32_t lb = ceil_div<uint32_t>(l, kSmallRows);
       for (uint32_t t = threadIdx.x; t < lb * nb; t += kSmallThreads) {
-        const uint32_t i0 = t % nb * 4, l0 = t / nb * 4;
-        float vr[4][4], vi[4][4];
+        const uint32_t i0 = t % nb * 4, l0 = t / nb * kSmallRows;
+        float vr[kSmallRows][4], vi[kSmallRows][4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < kSmallRows; ++r) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) vr[r][i] = vi[r][i] = 0.0f;
         }
+#pragma unroll 1
         for (uint32_t j = 0; j < sp; j += 4) {
-          Quad x[4];
+          Quad x[kSmallRows];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
+          for (int r = 0; r < kSmallRows; ++r) {
             const uint32_t row = min(l0 + r, l - 1);
             x[r] = load_quad(xr + row * sp + j, xi + row * sp + j);
           }
@@ -861,7 +849,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
           for (int jj = 0; jj < 4; ++jj) {
             const Quad q = load_quad(p_re + (j + jj) * sp + i0, p_im + (j + jj) * sp + i0);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < kSmallRows; ++r) {
               const float cr = x[r].re[jj], ci = x[r].im[jj];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -872,7 +860,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
           }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < kSmallRows; ++r) {
           if (l0 + r < l) {
             Quad q = load_quad(xr + (l0 + r) * sp + i0, xi + (l0 + r) * sp + i0);
 #pragma unroll
@@ -886,7 +874,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
       }
       __syncthreads();
     }
-    const float *xr = x_re[p.steps & 1], *xi = x_im[p.steps & 1];
+    const float *xr = (p.steps & 1) ? x1 : x0, *xi = xr + x_size;
     uint16_t *out = static_cast<uint16_t *>(p.out) + b * 2 * plane;
     for (uint32_t e = threadIdx.x; e < plane; e += kSmallThreads) {
       const uint32_t row = e / static_cast<uint32_t>(p.n), col = e - row * static_cast<uint32_t>(p.n);
