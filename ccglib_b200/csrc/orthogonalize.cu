@@ -666,6 +666,7 @@ void launch_first_form(const FirstParams &p, bool il, bool vec, unsigned grid, c
 constexpr int kSmallThreads = 512;
 constexpr int kSmallRows = 2;  // rows of V' per thread in the update
 constexpr size_t kSmallMaxSide = 64;
+constexpr int kSmallSmem = kMaxSmem - 2048;  // dynamic; the rest is static
 
 struct SmallParams {
   const void *in;
@@ -701,8 +702,8 @@ __device__ __forceinline__ void store_quad(float *re, float *im, const Quad &q) 
 // code: instructions arrive no faster than a few clocks each when they run once.)
 template <typename Store>
 __device__ __forceinline__ void gram_blocks(const float *re, const float *im, uint32_t rows, uint32_t sp,
-                                            uint32_t lanes, Store store) {
-  const uint32_t nb = sp / 2, pairs = nb * (nb + 1) / 2;
+                                            uint32_t lanes, const uint16_t *blocks, Store store) {
+  const uint32_t pairs = (sp / 2) * (sp / 2 + 1) / 2;
   const uint32_t sub = threadIdx.x % lanes, per_turn = kSmallThreads / lanes;
   // a warp goes on while any of its groups has a block: the shuffles need all of them
   const uint32_t warp_first = (threadIdx.x & ~31u) / lanes;
@@ -710,14 +711,9 @@ __device__ __forceinline__ void gram_blocks(const float *re, const float *im, ui
   for (uint32_t turn = 0; turn + warp_first < pairs; turn += per_turn) {
     const uint32_t pair = turn + threadIdx.x / lanes;
     const bool on = pair < pairs;
-    uint32_t bi = 0, bj = on ? pair : 0;
-    while (bj >= nb - bi) {
-      bj -= nb - bi;
-      ++bi;
-    }
-    bj += bi;
+    const uint32_t block = blocks[on ? pair : 0], bi = block >> 8, bj = block & 255;
     float h[2][2][2] = {};
-#pragma unroll 2
+#pragma unroll 4
     for (uint32_t k = sub; k < rows; k += lanes) {
       const float2 ur = *reinterpret_cast<const float2 *>(re + k * sp + 2 * bi);
       const float2 ui = *reinterpret_cast<const float2 *>(im + k * sp + 2 * bi);
@@ -769,6 +765,8 @@ __device__ __forceinline__ uint32_t lanes_for(uint32_t pairs, uint32_t rows) {
 __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams p) {
   extern __shared__ __align__(16) float small_smem_raw[];
   __shared__ double part[kSmallThreads / 32];
+  // the 2 x 2 blocks on and above the diagonal, row by row: (row << 8) + column
+  __shared__ uint16_t blocks[(kSmallMaxSide / 2) * (kSmallMaxSide / 2 + 1) / 2];
   const uint32_t sp = p.sp, l = p.l;
   const uint32_t x_size = l * sp;
   float *x0 = small_smem_raw, *x1 = x0 + 2 * x_size;  // Re, Im of V, twice
@@ -776,6 +774,13 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
   float *s_re = at, *s_im = at + sp * sp, *p_re = at + 2 * sp * sp, *p_im = at + 3 * sp * sp;
   const uint32_t nb = sp / 4, pairs = (sp / 2) * (sp / 2 + 1) / 2;
   const uint32_t lanes_l = lanes_for(pairs, l), lanes_s = lanes_for(pairs, sp);
+  for (uint32_t i = threadIdx.x; i < sp / 2; i += kSmallThreads) {
+    uint32_t at_block = i * (sp / 2) - i * (i - 1) / 2;
+    for (uint32_t j = i; j < sp / 2; ++j) blocks[at_block++] = static_cast<uint16_t>(i << 8 | j);
+  }
+  // the update deals (row group, column group) pairs to the threads: this thread's first and the stride
+  const uint32_t row_0 = threadIdx.x / nb, col_0 = threadIdx.x % nb;
+  const uint32_t row_step = kSmallThreads / nb, col_step = kSmallThreads % nb;
   const size_t plane = p.m * p.n;
   for (size_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
     // X and its norm (float64: no input overflows or vanishes in it)
@@ -807,7 +812,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
     for (int step = 0; step < p.steps; ++step) {
       const float *xr = (step & 1) ? x1 : x0, *xi = xr + x_size;
       float *yr = (step & 1) ? x0 : x1, *yi = yr + x_size;
-      gram_blocks(xr, xi, l, sp, lanes_l, [&](uint32_t i, uint32_t j, float re, float im) {
+      gram_blocks(xr, xi, l, sp, lanes_l, blocks, [&](uint32_t i, uint32_t j, float re, float im) {
         // S_ij = conj(H_ij)
         const uint32_t ij = i * sp + j, ji = j * sp + i;
         im = i == j ? 0.0f : im;
@@ -817,7 +822,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
         s_im[ji] = im;
       });
       __syncthreads();
-      gram_blocks(s_re, s_im, sp, sp, lanes_s, [&](uint32_t i, uint32_t j, float re, float im) {
+      gram_blocks(s_re, s_im, sp, sp, lanes_s, blocks, [&](uint32_t i, uint32_t j, float re, float im) {
         const uint32_t ij = i * sp + j, ji = j * sp + i;
         re = p.b * s_re[ij] + p.c * re;
         im = i == j ? 0.0f : p.b * s_im[ij] + p.c * im;
@@ -829,8 +834,14 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
       __syncthreads();
       // kSmallRows rows of V' x four columns
       const uint32_t lb = ceil_div<uint32_t>(l, kSmallRows);
-      for (uint32_t t = threadIdx.x; t < lb * nb; t += kSmallThreads) {
-        const uint32_t i0 = t % nb * 4, l0 = t / nb * kSmallRows;
+      for (uint32_t row = row_0, col = col_0; row < lb;) {
+        const uint32_t i0 = col * 4, l0 = row * kSmallRows;
+        row += row_step;
+        col += col_step;
+        if (col >= nb) {
+          col -= nb;
+          ++row;
+        }
         float vr[kSmallRows][4], vi[kSmallRows][4];
 #pragma unroll
         for (int r = 0; r < kSmallRows; ++r) {
@@ -842,8 +853,8 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
           Quad x[kSmallRows];
 #pragma unroll
           for (int r = 0; r < kSmallRows; ++r) {
-            const uint32_t row = min(l0 + r, l - 1);
-            x[r] = load_quad(xr + row * sp + j, xi + row * sp + j);
+            const uint32_t from = min(l0 + r, l - 1) * sp + j;
+            x[r] = load_quad(xr + from, xi + from);
           }
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
@@ -1081,13 +1092,30 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.wait_cycles = wait_limit_cycles();
   int rc = device_status_address(&plan.status);
   if (rc != CCGLIB_B200_OK) return rc;
-  const size_t smem = small_smem(plan.n, plan.l);
-  plan.small = plan.n <= kSmallMaxSide && smem <= static_cast<size_t>(kMaxSmem - 1024);
-  if (const char *v = std::getenv("CCGLIB_B200_ORTH_SMALL")) plan.small = plan.small && std::atoi(v) != 0;
+  plan.square = pick_shape(d.batch, plan.n, plan.n_p, true, plan.sms);
+  plan.update = pick_shape(d.batch, d.m, plan.cols_p, false, plan.sms);
+  // One launch with a CTA per matrix, or three launches per step?  Estimates in microseconds per step,
+  // within 40 % of what both forms take on short sides 1 .. 64, long sides to 1600, batches to 1024:
+  // 33 x 70 x 64 51 against 106 for five steps, 64 x 64 150 against 95, 16 x 32 x 1024 92 against 211.
+  plan.small = plan.n <= kSmallMaxSide && small_smem(plan.n, plan.l) <= static_cast<size_t>(kSmallSmem);
+  if (plan.small) {
+    const double side = static_cast<double>(ceil_div<size_t>(plan.n, 4) * 4);
+    const double macs = side * side * (2.0 * static_cast<double>(plan.l) + side);
+    const size_t sms = static_cast<size_t>(plan.sms);
+    const double turns = static_cast<double>(ceil_div(d.batch, sms));
+    const double one = turns * (1.5 + 4e-5 * macs);
+    const double waves = 2.0 * static_cast<double>(ceil_div(d.batch * plan.square.per_batch, sms)) +
+                         static_cast<double>(ceil_div(d.batch * plan.update.per_batch, sms));
+    const double three = 3 * 4.8 + 2.5 * (waves - 3.0);
+    plan.small = one < three;
+    // CCGLIB_B200_ORTH_SMALL = 0 or 1 chooses by hand (where the matrices fit)
+    const char *v = std::getenv("CCGLIB_B200_ORTH_SMALL");
+    if (v != nullptr && *v != '\0') plan.small = std::atoi(v) != 0;
+  }
   if (plan.small) {
     CCGLIB_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void *>(small_kernel),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kMaxSmem - 1024));
+                                         kSmallSmem));
     *out = new (std::nothrow) ccglib_b200_orthogonalize_plan(plan);
     if (*out == nullptr) {
       set_last_error("orthogonalize_plan_create: out of host memory");
@@ -1095,8 +1123,6 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     }
     return CCGLIB_B200_OK;
   }
-  plan.square = pick_shape(d.batch, plan.n, plan.n_p, true, plan.sms);
-  plan.update = pick_shape(d.batch, d.m, plan.cols_p, false, plan.sms);
   if (d.batch * plan.square.per_batch > 0x7FFFFFFFull ||
       d.batch * plan.update.per_batch > 0x7FFFFFFFull) {
     set_last_error("orthogonalize_plan_create: too many tiles");
