@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ccglib_b200 {
@@ -220,19 +222,79 @@ quantize_rows_kernel(const QuantizeParams p) {
   }
 }
 
+// One complex value as it lies in memory: two 16-bit halves (re low) or two floats.
+template <typename T> struct Raw {
+  uint32_t w;
+  __device__ __forceinline__ float2 value() const { return unpack2<T>(w); }
+};
+template <> struct Raw<float> {
+  float2 v;
+  __device__ __forceinline__ float2 value() const { return v; }
+};
+// N complex values `stride` complex apart, from re (and im, planar).  All loads are under way before the
+// first is used.
+template <typename T, bool IL, int N>
+__device__ __forceinline__ void load_raw(const T *re, const T *im, size_t stride, Raw<T> (&x)[N]) {
+  if constexpr (IL) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        x[i].v = __ldcs(reinterpret_cast<const float2 *>(re) + i * stride);
+      } else {
+        x[i].w = __ldcs(reinterpret_cast<const uint32_t *>(re) + i * stride);
+      }
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i].v = make_float2(__ldcs(re + i * stride), __ldcs(im + i * stride));
+  } else {
+    unsigned short lo[N], hi[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      lo[i] = __ldcs(reinterpret_cast<const unsigned short *>(re) + i * stride);
+      hi[i] = __ldcs(reinterpret_cast<const unsigned short *>(im) + i * stride);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i].w = lo[i] | (static_cast<uint32_t>(hi[i]) << 16);
+  }
+}
+
+// Largest finite |re|, |im| of N values, as the bits of a float32.
+template <typename T, int N> __device__ __forceinline__ uint32_t top_bits(const Raw<T> (&x)[N]) {
+  if constexpr (sizeof(T) == 2) {
+    // both halves at once; the patterns order like the values, infinities and NaN behind all others
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = __vmaxu2(m, x[i].w & 0x7FFF7FFFu);
+    const uint32_t top = max(m & 0xFFFFu, m >> 16);
+    if (top < (std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u)) {
+      return __float_as_uint(unpack2<T>(top).x);
+    }
+  }
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float2 v = x[i].value();
+    t = max(t, max(finite_abs_bits(v.x), finite_abs_bits(v.y)));
+  }
+  return t;
+}
+
 // Rows contiguous ([k][rows]): the operand of a product over the matrix's other axis.  A CTA takes
 // 128 rows x 128 k; a lane reads one row of every fourth of them, so a warp's loads run along the
 // rows; the bytes turn in shared memory (8 k of a row per store) and leave in runs of 128.  TILE: one
-// scale for the block, else one per row.
+// scale for the block, else one per row.  Values wait in registers as they came (16-bit types: one
+// register per complex value, so that two CTAs fit an SM and one loads while the other stores).
 constexpr int kColWarps = 16;
 constexpr int kColK = kBlockK / kColWarps;  // k per warp
 constexpr int kColPitch = kBlockK + 8;      // 8-byte accesses down the rows touch every bank once
 
 template <typename T, bool IL, bool E5M2, bool TILE>
-__global__ void __launch_bounds__(32 * kColWarps)
+__global__ void __launch_bounds__(32 * kColWarps, sizeof(T) == 2 ? 2 : 1)
 quantize_cols_kernel(const QuantizeParams p) {
   __shared__ __align__(16) uint8_t bytes[2][128 * kColPitch];
   __shared__ uint32_t row_max[128];
+  __shared__ float row_inv[128];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t groups = ceil_div<size_t>(p.rows, 128);
   const size_t items = p.batch * groups * p.blocks_k;
@@ -243,44 +305,33 @@ quantize_cols_kernel(const QuantizeParams p) {
     const size_t r0 = group * 128, k0 = kb * kBlockK + warp * kColK;
     const T *in = static_cast<const T *>(p.in) + b * 2 * p.rows * p.k;
     if (tid < 128) row_max[tid] = 0;
-    float re[4][kColK], im[4][kColK];
+    Raw<T> x[4][kColK];
+    if (r0 + 128 <= p.rows && (kb + 1) * kBlockK <= p.k) {
 #pragma unroll
-    for (int i = 0; i < kColK; ++i) {
+      for (int j = 0; j < 4; ++j) {
+        const T *re = in + (k0 * p.rows + r0 + 32 * j + lane) * (IL ? 2 : 1);
+        load_raw<T, IL, kColK>(re, re + p.rows * p.k, p.rows, x[j]);
+      }
+    } else {
+      // at the edges: the last row and k stand in for what lies outside, then zeros
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const size_t r = r0 + 32 * j + lane;
-        re[j][i] = im[j][i] = 0.0f;
-        if (r < p.rows && k0 + i < p.k) {
-          const size_t s = (k0 + i) * p.rows + r;
-          if constexpr (IL) {
-            if constexpr (sizeof(T) == 4) {
-              const float2 v = __ldcs(reinterpret_cast<const float2 *>(in) + s);
-              re[j][i] = v.x;
-              im[j][i] = v.y;
-            } else {
-              const float2 v = unpack2<T>(__ldcs(reinterpret_cast<const uint32_t *>(in) + s));
-              re[j][i] = v.x;
-              im[j][i] = v.y;
-            }
-          } else {
-            re[j][i] = to_float(in[s]);
-            im[j][i] = to_float(in[s + p.rows * p.k]);
-          }
+        const T *re = in + (min(k0, p.k - 1) * p.rows + min(r, p.rows - 1)) * (IL ? 2 : 1);
+#pragma unroll
+        for (int i = 0; i < kColK; ++i) {
+          Raw<T> one[1];
+          load_raw<T, IL, 1>(re, re + p.rows * p.k, 0, one);
+          x[j][i] = r < p.rows && k0 + i < p.k ? one[0] : Raw<T>{};
+          if (k0 + i + 1 < p.k) re += p.rows * (IL ? 2 : 1);
         }
       }
     }
     __syncthreads();  // row_max is zero; the previous item's bytes have been read
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t t = 0;
-#pragma unroll
-      for (int i = 0; i < kColK; ++i) {
-        t = max(t, max(finite_abs_bits(re[j][i]), finite_abs_bits(im[j][i])));
-      }
-      atomicMax(&row_max[32 * j + lane], t);
-    }
+    for (int j = 0; j < 4; ++j) atomicMax(&row_max[32 * j + lane], top_bits<T, kColK>(x[j]));
     __syncthreads();
-    [[maybe_unused]] float inv_tile = 0.0f;
+    float inv_tile = 0.0f;
     if constexpr (TILE) {
       uint32_t t = max(max(row_max[lane], row_max[32 + lane]), max(row_max[64 + lane], row_max[96 + lane]));
       t = __reduce_max_sync(0xFFFFFFFFu, t);
@@ -288,18 +339,16 @@ quantize_cols_kernel(const QuantizeParams p) {
       inv_tile = __fdiv_rn(1.0f, s);
       if (tid == 0) p.scale[(b * p.blocks_k + kb) * p.blocks_rows + group] = s;
     } else {
-      if (tid < 128 && r0 + tid < p.rows) {
-        p.scale[(b * p.blocks_k + kb) * p.blocks_rows + r0 + tid] = block_scale<E5M2>(row_max[tid]);
+      if (tid < 128) {
+        const float s = block_scale<E5M2>(row_max[tid]);
+        row_inv[tid] = __fdiv_rn(1.0f, s);
+        if (r0 + tid < p.rows) p.scale[(b * p.blocks_k + kb) * p.blocks_rows + r0 + tid] = s;
       }
+      __syncthreads();
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float inv;
-      if constexpr (TILE) {
-        inv = inv_tile;
-      } else {
-        inv = __fdiv_rn(1.0f, block_scale<E5M2>(row_max[32 * j + lane]));
-      }
+      const float inv = TILE ? inv_tile : row_inv[32 * j + lane];
       const uint32_t at = (32 * j + lane) * kColPitch + warp * kColK;
       uint32_t w[4];
 #pragma unroll
@@ -307,8 +356,9 @@ quantize_cols_kernel(const QuantizeParams p) {
         float a[4], c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          a[i] = re[j][4 * h + i] * inv;
-          c[i] = im[j][4 * h + i] * inv;
+          const float2 v = x[j][4 * h + i].value();
+          a[i] = v.x * inv;
+          c[i] = v.y * inv;
         }
         w[h] = pack4<E5M2>(a);
         w[2 + h] = pack4<E5M2>(c);
@@ -321,11 +371,11 @@ quantize_cols_kernel(const QuantizeParams p) {
 #pragma unroll
     for (int i = 0; i < 2 * 128 * 16 / (32 * kColWarps); ++i) {
       const uint32_t piece = i * 32 * kColWarps + tid;
-      const uint32_t plane = piece >> 11, r = (piece >> 4) & 127, x = (piece & 15) * 8;
-      const size_t k_at = kb * kBlockK + x;
+      const uint32_t plane = piece >> 11, r = (piece >> 4) & 127, y = (piece & 15) * 8;
+      const size_t k_at = kb * kBlockK + y;
       if (r0 + r < p.rows && k_at < p.pitch) {
         *reinterpret_cast<uint2 *>(p.out + ((b * 2 + plane) * p.rows + r0 + r) * p.pitch + k_at) =
-            *reinterpret_cast<const uint2 *>(&bytes[plane][r * kColPitch + x]);
+            *reinterpret_cast<const uint2 *>(&bytes[plane][r * kColPitch + y]);
       }
     }
   }
