@@ -58,17 +58,15 @@ template <bool E5M2> __device__ __forceinline__ float block_scale(uint32_t amax_
   return fmaxf(s, kMinScale);
 }
 
-// Four scaled values -> four fp8 bytes, first value in the low byte.
-template <bool E5M2> __device__ __forceinline__ uint32_t pack4(const float (&v)[4]) {
+// Four scaled values -> four fp8 bytes, first value in the low byte.  SPECIAL: the values may hold
+// infinities, which the conversion would saturate (finite ones never exceed the format here).
+template <bool E5M2, bool SPECIAL = false>
+__device__ __forceinline__ uint32_t pack4(const float (&v)[4]) {
   constexpr __nv_fp8_interpretation_t kFmt = E5M2 ? __NV_E5M2 : __NV_E4M3;
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, kFmt);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, kFmt);
   uint32_t w = lo | (hi << 16);
-  // the conversion saturates infinities (finite values never exceed the format here)
-  bool inf = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) inf |= fabsf(v[i]) == __uint_as_float(0x7F800000u);
-  if (inf) {
+  if constexpr (SPECIAL) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (fabsf(v[i]) == __uint_as_float(0x7F800000u)) {
@@ -81,16 +79,16 @@ template <bool E5M2> __device__ __forceinline__ uint32_t pack4(const float (&v)[
 }
 
 // Four consecutive complex samples k0..k0+3 of row r of one batch item (K contiguous).  VEC: K is a
-// multiple of four, so a quad is inside the row or outside it as a whole and its words are aligned.
+// multiple of four, so a quad is inside the row or outside it as a whole and its words are aligned;
+// outside, an address inside stands in and the values are dropped, so that no load waits for a branch.
 template <typename T, bool IL, bool VEC>
 __device__ __forceinline__ void load_quad(const T *in, size_t rows, size_t k, size_t r, size_t k0,
                                           float (&re)[4], float (&im)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) re[i] = im[i] = 0.0f;
-  if (k0 >= k) return;
   if constexpr (VEC) {
+    const bool inside = r < rows && k0 < k;
+    const size_t at = min(r, rows - 1) * k + (k0 < k ? k0 : 0);
     if constexpr (IL) {
-      const T *src = in + (r * k + k0) * 2;
+      const T *src = in + at * 2;
       if constexpr (sizeof(T) == 4) {
         const float4 a = __ldcs(reinterpret_cast<const float4 *>(src));
         const float4 b = __ldcs(reinterpret_cast<const float4 *>(src) + 1);
@@ -107,7 +105,7 @@ __device__ __forceinline__ void load_quad(const T *in, size_t rows, size_t k, si
         }
       }
     } else {
-      const T *s0 = in + r * k + k0;
+      const T *s0 = in + at;
       const T *s1 = s0 + rows * k;
       if constexpr (sizeof(T) == 4) {
         const float4 a = __ldcs(reinterpret_cast<const float4 *>(s0));
@@ -123,20 +121,21 @@ __device__ __forceinline__ void load_quad(const T *in, size_t rows, size_t k, si
         im[0] = b0.x; im[1] = b0.y; im[2] = b1.x; im[3] = b1.y;
       }
     }
+    if (!inside) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) re[i] = im[i] = 0.0f;
+    }
   } else {
+    const size_t row = min(r, rows - 1) * k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (k0 + i < k) {
-        if constexpr (IL) {
-          const size_t s = (r * k + k0 + i) * 2;
-          re[i] = to_float(in[s]);
-          im[i] = to_float(in[s + 1]);
-        } else {
-          const size_t s = r * k + k0 + i;
-          re[i] = to_float(in[s]);
-          im[i] = to_float(in[s + rows * k]);
-        }
-      }
+      const size_t s = row + min(k0 + i, k - 1);
+      re[i] = to_float(IL ? in[2 * s] : in[s]);
+      im[i] = to_float(IL ? in[2 * s + 1] : in[s + rows * k]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (r >= rows || k0 + i >= k) re[i] = im[i] = 0.0f;
     }
   }
 }
@@ -165,17 +164,32 @@ quantize_rows_kernel(const QuantizeParams p) {
     float re[kRows][4], im[kRows][4];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      load_quad<T, IL, VEC>(in, p.rows, p.k, r0 + i, r0 + i < p.rows ? k0 : p.k, re[i], im[i]);
+      load_quad<T, IL, VEC>(in, p.rows, p.k, r0 + i, k0, re[i], im[i]);
     }
+    // Maxima of the bits without the sign: infinities and NaN are behind all finite values and are taken
+    // out in a second go where there are any.
     uint32_t top[kRows];
+    bool special = false;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       uint32_t t = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        t = max(t, max(finite_abs_bits(re[i][j]), finite_abs_bits(im[i][j])));
+        t = max(t, max(__float_as_uint(re[i][j]) & 0x7FFFFFFFu, __float_as_uint(im[i][j]) & 0x7FFFFFFFu));
       }
       top[i] = t;
+      special |= t >= 0x7F800000u;
+    }
+    if (special) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        uint32_t t = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          t = max(t, max(finite_abs_bits(re[i][j]), finite_abs_bits(im[i][j])));
+        }
+        top[i] = t;
+      }
     }
     if constexpr (kTile) {
       uint32_t t = top[0];
@@ -212,8 +226,13 @@ quantize_rows_kernel(const QuantizeParams p) {
           c[j] = im[i][j] * inv;
         }
         uint8_t *dst = p.out + ((b * 2) * p.rows + r) * p.pitch + k0;
-        *reinterpret_cast<uint32_t *>(dst) = pack4<E5M2>(a);
-        *reinterpret_cast<uint32_t *>(dst + p.rows * p.pitch) = pack4<E5M2>(c);
+        uint32_t w_re = pack4<E5M2>(a), w_im = pack4<E5M2>(c);
+        if (special) {
+          w_re = pack4<E5M2, true>(a);
+          w_im = pack4<E5M2, true>(c);
+        }
+        *reinterpret_cast<uint32_t *>(dst) = w_re;
+        *reinterpret_cast<uint32_t *>(dst + p.rows * p.pitch) = w_im;
       }
     }
     if constexpr (!kTile) {
@@ -259,25 +278,31 @@ __device__ __forceinline__ void load_raw(const T *re, const T *im, size_t stride
   }
 }
 
-// Largest finite |re|, |im| of N values, as the bits of a float32.
-template <typename T, int N> __device__ __forceinline__ uint32_t top_bits(const Raw<T> (&x)[N]) {
+// Largest finite |re|, |im| of N values, as the bits of a float32; `special` is raised if there are others.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t top_bits(const Raw<T> (&x)[N], bool &special) {
+  // the patterns without the sign order like the values, infinities and NaN behind all others
+  uint32_t m = 0;
   if constexpr (sizeof(T) == 2) {
-    // both halves at once; the patterns order like the values, infinities and NaN behind all others
-    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) m = __vmaxu2(m, x[i].w & 0x7FFF7FFFu);
-    const uint32_t top = max(m & 0xFFFFu, m >> 16);
-    if (top < (std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u)) {
-      return __float_as_uint(unpack2<T>(top).x);
+    m = max(m & 0xFFFFu, m >> 16);
+    if (m < (std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u)) return __float_as_uint(unpack2<T>(m).x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      m = max(m, max(__float_as_uint(x[i].v.x) & 0x7FFFFFFFu, __float_as_uint(x[i].v.y) & 0x7FFFFFFFu));
     }
+    if (m < 0x7F800000u) return m;
   }
-  uint32_t t = 0;
+  special = true;
+  m = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float2 v = x[i].value();
-    t = max(t, max(finite_abs_bits(v.x), finite_abs_bits(v.y)));
+    m = max(m, max(finite_abs_bits(v.x), finite_abs_bits(v.y)));
   }
-  return t;
+  return m;
 }
 
 // Rows contiguous ([k][rows]): the operand of a product over the matrix's other axis.  A CTA takes
@@ -328,8 +353,9 @@ quantize_cols_kernel(const QuantizeParams p) {
       }
     }
     __syncthreads();  // row_max is zero; the previous item's bytes have been read
+    bool special = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) atomicMax(&row_max[32 * j + lane], top_bits<T, kColK>(x[j]));
+    for (int j = 0; j < 4; ++j) atomicMax(&row_max[32 * j + lane], top_bits<T, kColK>(x[j], special));
     __syncthreads();
     float inv_tile = 0.0f;
     if constexpr (TILE) {
@@ -362,6 +388,10 @@ quantize_cols_kernel(const QuantizeParams p) {
         }
         w[h] = pack4<E5M2>(a);
         w[2 + h] = pack4<E5M2>(c);
+        if (special) {
+          w[h] = pack4<E5M2, true>(a);
+          w[2 + h] = pack4<E5M2, true>(c);
+        }
       }
       *reinterpret_cast<uint2 *>(&bytes[0][at]) = make_uint2(w[0], w[1]);
       *reinterpret_cast<uint2 *>(&bytes[1][at]) = make_uint2(w[2], w[3]);
