@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -422,9 +423,17 @@ def quantize(batch, rows, k, type_in, type_out, d_in, d_out, d_scale, stream: in
              input_complex_axis=PLANAR, input_mem_order=ROW_MAJOR, block_rows=1) -> None:
     """Complex float matrices -> fp8 planes [batch][2][rows][pitch] and block scales
     [batch][ceil(k / 128)][ceil(rows / block_rows)] (see include/ccglib_b200.h)."""
-    desc = QuantizeDesc(batch, rows, k, type_in, type_out, input_complex_axis, input_mem_order,
-                        block_rows)
-    _check(lib().ccglib_b200_quantize_run(ctypes.byref(desc), d_in, d_out, d_scale, stream))
+    status = lib().ccglib_b200_quantize_run(
+        _quantize_desc(batch, rows, k, type_in, type_out, input_complex_axis, input_mem_order,
+                       block_rows), d_in, d_out, d_scale, stream)
+    if status != OK:
+        _check(status)
+
+
+@functools.lru_cache(maxsize=64)
+def _quantize_desc(*fields):
+    """The call is short enough for building its description to be seen; it is read only."""
+    return ctypes.byref(QuantizeDesc(*fields))
 
 
 def operand_pitch(k: int) -> int:

@@ -55,6 +55,24 @@ int make_map(CUtensorMap *tm, const void *base, uint64_t row_bytes, uint64_t row
              uint64_t row_pitch, uint64_t slice_pitch, uint32_t sw, uint32_t box_rows,
              uint32_t box_slices);
 
+// Launch with programmatic stream serialisation: the kernel may be set up while the one before it on
+// the stream finishes, and waits for it (griddepcontrol.wait) before it touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_programmatic(void (*kernel)(Params...), unsigned grid, unsigned threads,
+                                size_t smem, cudaStream_t stream, const Args &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Launchers implemented in the individual .cu files (host side, no extern "C").
 int launch_expand_bits(const void *d_in, void *d_out, size_t batch, size_t rows, size_t k_bits,
                        size_t out_row_bytes, int planes_out, bool tiled, size_t blk, size_t k_c_bits,

@@ -10,6 +10,7 @@
 // mirror image.  X is never transposed: where a product contracts over rows, its operand is read with
 // the rows as K (the MN-major form of the shared-memory descriptor).  b S and a X are added in the
 // epilogue; the last update writes the caller's type and layout.
+// The launches are programmatic: a product's CTAs set up while the one before it drains.
 //
 // Between products X, S and P are float16.  All three are bounded (singular values stay near or below
 // one), X is kept times a power of two near sqrt(long side) so that its entries are near one, and float16
@@ -92,15 +93,6 @@ __device__ __forceinline__ TileCoord orth_tile(const OrthParams &p, uint32_t til
   t.mt = r / width;
   t.nt = first_n + (r - t.mt * width);
   return t;
-}
-
-// Products follow one another with programmatic launch: a product's CTAs may set up (barriers, tensor
-// memory, descriptors) while the product before it drains, and wait here before they touch memory.
-__device__ __forceinline__ void wait_for_previous() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_start() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi, bool bf16) {
@@ -918,6 +910,9 @@ struct ccglib_b200_orthogonalize_plan {
   size_t scratch_bytes;
   __half *x[2], *s, *p;  // [batch][2][m][cols_p], [batch][2][n][n_p]
   double *sums;
+  // tensor maps of the workspace: X as either operand of the Gram product and as the operand of the
+  // update, S as either operand, P as the operand of the update, and all three as results
+  CUtensorMap gram_a[2], gram_b[2], update_x[2], x_out[2], s_a, s_b, update_p, s_out, p_out;
 };
 
 namespace {
@@ -932,6 +927,7 @@ struct Operand {
 
 struct Product {
   Operand a, b;
+  const CUtensorMap *tm_a, *tm_b, *tm_c;
   size_t m, n;  // n: columns written
   ProductShape shape;
   bool hermitian, conj;
@@ -943,9 +939,43 @@ struct Product {
   bool boxes, bf16;
 };
 
+// Map of an operand whose tile has `tile` rows of the result's.
 int operand_map(CUtensorMap *tm, const Operand &o, size_t batch, int tile) {
   const uint32_t box = o.by_rows ? kOrthK : static_cast<uint32_t>(tile);
   return make_map(tm, o.data, o.cols * 2, o.rows, 2 * batch, o.pitch * 2, o.rows * o.pitch * 2, 128, box, 2);
+}
+
+// Map of a result: planes of rows x cols 16-bit values.
+int result_map(CUtensorMap *tm, const void *out, size_t batch, size_t rows, size_t cols) {
+  return make_map(tm, out, cols * 2, rows, 2 * batch, cols * 2, rows * cols * 2, 64, 32, 1);
+}
+
+// X as an operand: contracted over the long side in S, over the short side in the update.
+Operand x_operand(const ccglib_b200_orthogonalize_plan &plan, int which, bool over_long) {
+  return {plan.x[which], plan.desc.m, plan.cols_p, plan.cols_p, plan.tall == over_long};
+}
+Operand square_operand(const ccglib_b200_orthogonalize_plan &plan, const __half *data) {
+  return {data, plan.n, plan.n_p, plan.n_p, false};
+}
+
+int make_maps(ccglib_b200_orthogonalize_plan &plan) {
+  const size_t batch = plan.desc.batch;
+  const Operand s = square_operand(plan, plan.s), p = square_operand(plan, plan.p);
+  int rc = operand_map(&plan.s_a, s, batch, kBlockM);
+  if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.s_b, s, batch, plan.square.bn);
+  if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.update_p, p, batch, plan.tall ? plan.update.bn : kBlockM);
+  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.s_out, plan.s, batch, plan.n, plan.n_p);
+  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.p_out, plan.p, batch, plan.n, plan.n_p);
+  for (int i = 0; i < 2; ++i) {
+    const Operand x_long = x_operand(plan, i, true), x_short = x_operand(plan, i, false);
+    if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.gram_a[i], x_long, batch, kBlockM);
+    if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.gram_b[i], x_long, batch, plan.square.bn);
+    if (rc == CCGLIB_B200_OK) {
+      rc = operand_map(&plan.update_x[i], x_short, batch, plan.tall ? kBlockM : plan.update.bn);
+    }
+    if (rc == CCGLIB_B200_OK) rc = result_map(&plan.x_out[i], plan.x[i], batch, plan.desc.m, plan.cols_p);
+  }
+  return rc;
 }
 
 int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q, cudaStream_t stream) {
@@ -972,30 +1002,9 @@ int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q,
   g.n_out = static_cast<uint32_t>(q.out_pitch);
   g.status = plan.status;
   g.wait_cycles = plan.wait_cycles;
-  CUtensorMap tm_a, tm_b, tm_c;
-  int rc = operand_map(&tm_a, q.a, batch, kBlockM);
-  if (rc != CCGLIB_B200_OK) return rc;
-  rc = operand_map(&tm_b, q.b, batch, q.shape.bn);
-  if (rc != CCGLIB_B200_OK) return rc;
-  tm_c = tm_a;  // placeholder
-  if (q.boxes) {
-    rc = make_map(&tm_c, q.out, q.out_pitch * 2, q.m, 2 * batch, q.out_pitch * 2, q.m * q.out_pitch * 2,
-                  64, 32, 1);
-    if (rc != CCGLIB_B200_OK) return rc;
-  }
   const unsigned grid = g.num_tiles < static_cast<uint32_t>(plan.sms) ? g.num_tiles : plan.sms;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = orth_smem(q.shape.bn);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  CCGLIB_CUDA_TRY(cudaLaunchKernelEx(&cfg, orth_kernel(q.shape.bn, q.a.by_rows, q.b.by_rows), tm_a, tm_b,
-                                     tm_c, g));
+  CCGLIB_CUDA_TRY(launch_programmatic(orth_kernel(q.shape.bn, q.a.by_rows, q.b.by_rows), grid, kThreads,
+                                      orth_smem(q.shape.bn), stream, *q.tm_a, *q.tm_b, *q.tm_c, g));
   return CCGLIB_B200_OK;
 }
 
@@ -1156,6 +1165,11 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.s = reinterpret_cast<__half *>(take(s_bytes));
   plan.p = reinterpret_cast<__half *>(take(s_bytes));
   plan.sums = reinterpret_cast<double *>(at);
+  rc = make_maps(plan);
+  if (rc != CCGLIB_B200_OK) {
+    cudaFree(plan.scratch);
+    return rc;
+  }
   *out = new (std::nothrow) ccglib_b200_orthogonalize_plan(plan);
   if (*out == nullptr) {
     cudaFree(plan.scratch);
@@ -1215,27 +1229,34 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
   const size_t n = plan->n, n_p = plan->n_p, cols_p = plan->cols_p;
   const bool tall = plan->tall;
   const float unscale = 1.0f / (plan->scale * plan->scale);
-  const Operand s{plan->s, n, n_p, n_p, false}, p{plan->p, n, n_p, n_p, false};
   for (int step = 0; rc == CCGLIB_B200_OK && step < d.steps; ++step) {
     const bool last = step + 1 == d.steps;
-    // X as an operand: contracted over the long side in S, over the short side in the update
-    const Operand x_long{plan->x[step & 1], d.m, cols_p, cols_p, tall};
-    Operand x_short = x_long;
-    x_short.by_rows = !tall;
-    rc = launch_product(*plan, {x_long, x_long, n, n_p, plan->square, true, true, unscale, 0.0f, 1.0f,
-                                nullptr, 0, plan->s, n_p, true, false}, stream);
+    const int now = step & 1;
+    const Operand x_long = x_operand(*plan, now, true), x_short = x_operand(*plan, now, false);
+    const Operand s = square_operand(*plan, plan->s), p = square_operand(*plan, plan->p);
+    rc = launch_product(*plan, {x_long, x_long, &plan->gram_a[now], &plan->gram_b[now], &plan->s_out, n, n_p,
+                                plan->square, true, true, unscale, 0.0f, 1.0f, nullptr, 0, plan->s, n_p,
+                                true, false}, stream);
     if (rc != CCGLIB_B200_OK) break;
-    rc = launch_product(*plan, {s, s, n, n_p, plan->square, true, true, d.c, d.b, 1.0f, plan->s, n_p,
-                                plan->p, n_p, true, false}, stream);
+    rc = launch_product(*plan, {s, s, &plan->s_a, &plan->s_b, &plan->p_out, n, n_p, plan->square, true, true,
+                                d.c, d.b, 1.0f, plan->s, n_p, plan->p, n_p, true, false}, stream);
     if (rc != CCGLIB_B200_OK) break;
-    Product update{tall ? x_short : p, tall ? p : x_short, d.m, cols_p, plan->update, false, false, 1.0f,
-                   d.a, 1.0f, plan->x[step & 1], cols_p, plan->x[(step & 1) ^ 1], cols_p, true, false};
+    const CUtensorMap *tm_x = &plan->update_x[now], *tm_p = &plan->update_p;
+    Product update{tall ? x_short : p, tall ? p : x_short, tall ? tm_x : tm_p, tall ? tm_p : tm_x,
+                   &plan->x_out[now ^ 1], d.m, cols_p, plan->update, false, false, 1.0f, d.a, 1.0f,
+                   plan->x[now], cols_p, plan->x[now ^ 1], cols_p, true, false};
+    CUtensorMap tm_out;
     if (last) {
       update.gain = 1.0f / plan->scale;
       update.out = d_out;
       update.out_pitch = d.n;
       update.boxes = d.n % 8 == 0 && aligned16(d_out);
       update.bf16 = d.type_out == CCGLIB_B200_BFLOAT16;
+      if (update.boxes) {
+        rc = result_map(&tm_out, d_out, d.batch, d.m, d.n);
+        if (rc != CCGLIB_B200_OK) break;
+        update.tm_c = &tm_out;
+      }
     }
     rc = launch_product(*plan, update, stream);
   }

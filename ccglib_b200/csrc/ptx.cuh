@@ -104,6 +104,19 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
                : "memory");
 }
 
+// ---- programmatic launch ----------------------------------------------------------------------
+
+// Wait until the kernels this launch depends on have finished and their writes are visible.  With
+// programmatic stream serialisation a CTA may be set up before that; nothing it does ahead of this may
+// touch global memory.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// Let the next kernel's CTAs be set up as this one's leave.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---- tcgen05 / TMEM ---------------------------------------------------------------------------
 
 __device__ __forceinline__ void tmem_alloc(uint32_t slot_smem, uint32_t ncols) {

@@ -418,6 +418,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  let_next_start();
 
   if (warp < C::kFirstEpiWarp) {
   if constexpr (C::kSplitRegs) regs_dec<40>();
@@ -425,6 +426,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   Segment seg;
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
+    wait_for_previous();
     uint32_t stage = 0, phase = 0, issued = 0;
     bool ok = true;
     while (ok && walk.next(p, seg)) {
@@ -514,6 +516,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   } else {
     // ------------------------------------------------------------------ epilogue warps
     if constexpr (C::kSplitRegs) regs_inc<232>();
+    wait_for_previous();
     Walk walk(p);
     Segment seg;
     const uint32_t quad = warp & 3;                       // tensor-memory lanes of this warp
@@ -903,9 +906,9 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
   const size_t ctas = plan->runs > 0 ? plan->runs
                       : plan->tiles < static_cast<size_t>(plan->sms) ? plan->tiles
                                                                      : plan->sms;
-  plan->kernel.fn<<<static_cast<unsigned>(ctas), plan->kernel.threads, plan->kernel.smem,
-                    static_cast<cudaStream_t>(stream_v)>>>(tm_a, tm_b, tm_c, p);
-  CCGLIB_CUDA_TRY(cudaGetLastError());
+  CCGLIB_CUDA_TRY(launch_programmatic(plan->kernel.fn, static_cast<unsigned>(ctas), plan->kernel.threads,
+                                      plan->kernel.smem, static_cast<cudaStream_t>(stream_v), tm_a, tm_b,
+                                      tm_c, p));
   return CCGLIB_B200_OK;
 }
 
