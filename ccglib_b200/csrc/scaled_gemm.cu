@@ -51,10 +51,10 @@ template <int BN> struct ScaledCfg {
   static constexpr int kCols = BN / 2;
   static constexpr int kEpiWarps = 4 * BN / kCols;
   // 128 sums per thread need a register split: 384 threads start with 168 each (64512 in all); the
-  // first warpgroup (two warps of it idle) hands back all but 40, the others take 232: 128 * 40 +
+  // first warpgroup (one warp of it idle) hands back all but 40, the others take 232: 128 * 40 +
   // 256 * 232 = 64512.
   static constexpr bool kSplitRegs = BN == 128;
-  static constexpr int kFirstEpiWarp = kSplitRegs ? 4 : 2;
+  static constexpr int kFirstEpiWarp = kSplitRegs ? 4 : 3;  // 0 loads, 1 and 2 multiply
   static constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
   static constexpr int kStagingBytes = kEpiWarps * kStoreTile;
   static constexpr int kBarrierBytes = 256;
@@ -388,7 +388,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   const uint32_t bar_empty = bar_full + 8 * kStages;
   const uint32_t bar_acc_full = bar_empty + 8 * kStages;
   const uint32_t bar_acc_empty = bar_acc_full + 8 * kAccBuffers;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 2 * kAccBuffers);
+  const uint32_t bar_turn = bar_acc_empty + 8 * kAccBuffers;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 2 * kAccBuffers + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   volatile unsigned *last_flag = tmem_slot + 2;
   const uint32_t smem_base = smem_u32(smem);
@@ -404,6 +405,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       mbar_init(bar_acc_full + 8 * s, 1);
       mbar_init(bar_acc_empty + 8 * s, C::kEpiWarps);
     }
+    mbar_init(bar_turn, 1);
+    mbar_init(bar_turn + 8, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tensormap(&tm_a);
@@ -467,15 +470,25 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------ MMA issuers
+    // Two warps take the blocks in turn, each its own accumulator buffer.  Issuing blocks while the tensor
+    // core's short queue is full, so one warp alone leaves the tensor core idle while it waits for the
+    // barriers of the next block (350 clocks of 1900); the other has done that when its turn comes.
+    const uint32_t acc = warp - 1;
     const uint64_t blocks = walk.blocks(p);
-    for (uint64_t i = 0; i < blocks; ++i) {
-      if (!mbar_wait(bar_acc_empty + 8 * acc, acc_phase ^ 1, abort_flag, p.g.status, kDevTimeoutMma,
+    uint32_t stage = acc, phase = 0, turn = 0;
+    static_assert(kStages > 2 && kAccBuffers == 2, "a stage and a buffer for either warp");
+    for (uint64_t i = acc; i < blocks; i += 2, ++turn) {
+      if (!mbar_wait(bar_acc_empty + 8 * acc, (turn & 1) ^ 1, abort_flag, p.g.status, kDevTimeoutMma,
                      p.g.wait_cycles) ||
           !mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.g.status, kDevTimeoutMma,
                      p.g.wait_cycles)) {
+        break;
+      }
+      // the other warp has issued block i - 1
+      if (i > 0 && !mbar_wait(bar_turn + 8 * acc, (acc == 0 ? turn - 1 : turn) & 1, abort_flag, p.g.status,
+                              kDevTimeoutMma, p.g.wait_cycles)) {
         break;
       }
       tc_fence_after();
@@ -499,17 +512,15 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             tc_mma<kKindF8F6F4>(d, a_im, b_im, p.g.idesc_neg_a, 1u);
           }
         }
+        if (i + 1 < blocks) mbar_arrive(bar_turn + 8 * (acc ^ 1));
         tc_commit(bar_empty + 8 * stage);
         tc_commit(bar_acc_full + 8 * acc);
       }
       __syncwarp();
-      if (++stage == kStages) {
-        stage = 0;
+      stage += 2;
+      if (stage >= kStages) {
+        stage -= kStages;
         phase ^= 1;
-      }
-      if (++acc == kAccBuffers) {
-        acc = 0;
-        acc_phase ^= 1;
       }
     }
   }
