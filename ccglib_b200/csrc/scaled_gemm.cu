@@ -30,7 +30,8 @@ namespace {
 constexpr int kBlockK = 128;
 constexpr int kAccBuffers = 2;
 constexpr int kStoreBytes = 64;                // bytes of a row in one TMA store
-constexpr int kStoreTile = 32 * kStoreBytes;  // 32 rows of them: an epilogue warp's staging
+constexpr int kStoreTile = 32 * kStoreBytes;  // 32 rows of them
+constexpr int kStoreTiles = 2;                 // staging of an epilogue warp: two stores in flight
 
 struct ScaledParams {
   GemmParams g;  // M, N, tiles, layout of C, alpha, beta, waits; row side = tile rows
@@ -56,7 +57,7 @@ template <int BN> struct ScaledCfg {
   static constexpr bool kSplitRegs = BN == 128;
   static constexpr int kFirstEpiWarp = kSplitRegs ? 4 : 3;  // 0 loads, 1 and 2 multiply
   static constexpr int kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
-  static constexpr int kStagingBytes = kEpiWarps * kStoreTile;
+  static constexpr int kStagingBytes = kEpiWarps * kStoreTiles * kStoreTile;
   static constexpr int kBarrierBytes = 256;
   static constexpr int kRaw = (kMaxSmem - 1024 - kBarrierBytes - kStagingBytes) / kStageBytes;
   static constexpr int kStages = kRaw > 6 ? 6 : kRaw;
@@ -288,7 +289,7 @@ __device__ __forceinline__ void row_words(bool inter, const float (&re)[COLS],
   }
 }
 
-// One box through the warp's staging tile (written the way a 64-byte-swizzled TMA store reads it: 16-byte
+// One box through one of the warp's staging tiles (written the way a 64-byte-swizzled TMA store reads it: 16-byte
 // piece j of row r at j ^ ((r >> 1) & 3)) and out.
 template <typename OutT, int COLS, int T>
 __device__ __forceinline__ void store_box(const GemmParams &p, const CUtensorMap *tm_c,
@@ -298,12 +299,17 @@ __device__ __forceinline__ void store_box(const GemmParams &p, const CUtensorMap
   using B = Boxes<OutT, COLS>;
   const bool inter = p.c_layout == kInterRow;
   const uint32_t first = n0 + (inter ? T * 8 * B::kPer : (T % B::kPlane) * 16 * B::kPer);
-  if (first >= p.N || m0 >= p.M) return;  // uniform over the warp
+  if (first >= p.N || m0 >= p.M) {  // uniform over the warp
+    // an empty group keeps the count: a staging tile is free when all but the newest group are done
+    if (lane == 0) bulk_commit_group();
+    return;
+  }
   uint32_t w[16];
   row_words<OutT, COLS, T>(inter, re, im, w);
-  if (lane == 0) bulk_wait_group_read<0>();
+  if (lane == 0) bulk_wait_group_read<kStoreTiles - 1>();
   __syncwarp();
-  const uint32_t row = staging + lane * kStoreBytes;
+  const uint32_t tile = staging + (T % kStoreTiles) * kStoreTile;
+  const uint32_t row = tile + lane * kStoreBytes;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     st_shared_v4(row + ((j ^ ((lane >> 1) & 3)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2],
@@ -314,7 +320,7 @@ __device__ __forceinline__ void store_box(const GemmParams &p, const CUtensorMap
   if (lane == 0) {
     const int32_t x = static_cast<int32_t>(first * sizeof(OutT) * (inter ? 2 : 1));
     const int32_t z = static_cast<int32_t>(inter ? b : 2 * b + (T < B::kPlane ? 0 : 1));
-    tma_store_3d(tm_c, staging, x, static_cast<int32_t>(m0), z);
+    tma_store_3d(tm_c, tile, x, static_cast<int32_t>(m0), z);
     bulk_commit_group();
   }
 }
@@ -533,10 +539,10 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     const uint32_t quad = warp & 3;                       // tensor-memory lanes of this warp
     const uint32_t first_col = ((warp - C::kFirstEpiWarp) >> 2) * COLS;  // columns of this warp
     const uint32_t staging =
-        smem_base + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * kStoreTile;
+        smem_base + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * (kStoreTiles * kStoreTile);
     // the column scales of the block (two buffers) at the head of the staging tile
     float *col_buf = reinterpret_cast<float *>(
-        smem + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * kStoreTile);
+        smem + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * (kStoreTiles * kStoreTile));
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
     while (walk.next(p, seg)) {
