@@ -535,7 +535,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
     if constexpr (C::kSplitRegs) regs_inc<232>();
     wait_for_previous();
     Walk walk(p);
-    Segment seg;
+    Segment seg{};
     const uint32_t quad = warp & 3;                       // tensor-memory lanes of this warp
     const uint32_t first_col = ((warp - C::kFirstEpiWarp) >> 2) * COLS;  // columns of this warp
     const uint32_t staging =
@@ -545,44 +545,61 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         smem + kStages * C::kStageBytes + (warp - C::kFirstEpiWarp) * (kStoreTiles * kStoreTile));
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
-    while (walk.next(p, seg)) {
+    // the scales of the next block: this lane's row, and two of the warp's columns
+    const float *rs = nullptr, *cs = nullptr;
+    float s_next = 0.0f, t0_next = 0.0f, t1_next = 0.0f;
+    uint32_t ri = 0, i0 = 0, i1 = 0;
+    bool row_in = false, in0 = false, in1 = false;
+    auto load_scales = [&]() {
+      s_next = row_in ? __ldg(rs + ri) : 0.0f;
+      t0_next = in0 ? __ldg(cs + i0) : 0.0f;
+      t1_next = in1 ? __ldg(cs + i1) : 0.0f;
+    };
+    auto first_scales = [&](const Segment &of) {
+      const TileCoord t = decode_tile(p.g, of.tile);
+      const uint32_t m = t.mt * kBlockM + quad * 32 + lane, c0 = t.nt * BN + first_col + 2 * lane;
+      const size_t block = static_cast<size_t>(t.b) * p.g.k_blocks + of.k0;
+      rs = p.row_scale + block * p.row_blocks;
+      cs = p.col_scale + block * p.col_blocks;
+      row_in = m < p.g.M;
+      in0 = 2 * lane < COLS && c0 < p.g.N;
+      in1 = 2 * lane < COLS && c0 + 1 < p.g.N;
+      ri = m >> p.row_shift;
+      i0 = c0 >> p.col_shift;
+      i1 = (c0 + 1) >> p.col_shift;
+      load_scales();
+    };
+    bool more = walk.next(p, seg);
+    if (more) first_scales(seg);
+    while (more) {
       float sum[2][COLS];  // Re, Im
       const TileCoord t = decode_tile(p.g, seg.tile);
       const uint32_t m = t.mt * kBlockM + quad * 32 + lane;
       const uint32_t n0 = t.nt * BN + first_col;
-      // this lane's row scale, and the scales of two of the warp's columns
-      const float *rs = p.row_scale + (static_cast<size_t>(t.b) * p.g.k_blocks + seg.k0) * p.row_blocks;
-      const float *cs = p.col_scale + (static_cast<size_t>(t.b) * p.g.k_blocks + seg.k0) * p.col_blocks;
-      const uint32_t c0 = n0 + 2 * lane, c1 = c0 + 1;
-      const bool row_in = m < p.g.M;
-      const bool in0 = 2 * lane < COLS && c0 < p.g.N, in1 = 2 * lane < COLS && c1 < p.g.N;
-      const uint32_t ri = m >> p.row_shift, i0 = c0 >> p.col_shift, i1 = c1 >> p.col_shift;
-      float s_next = row_in ? __ldg(rs + ri) : 0.0f;
-      float t0_next = in0 ? __ldg(cs + i0) : 0.0f;
-      float t1_next = in1 ? __ldg(cs + i1) : 0.0f;
 #pragma unroll
       for (int j = 0; j < COLS; ++j) sum[0][j] = sum[1][j] = 0.0f;
-      // the column scales go through the staging tile: its last store must have read it
-      if (lane == 0) bulk_wait_group_read<0>();
-      __syncwarp();
       for (uint32_t kb = seg.k0; ok && kb < seg.k1; ++kb) {
         const float s = s_next;
         // any column's scale stands for the block's where one covers 128 columns
-        const float t = __shfl_sync(0xFFFFFFFFu, t0_next, 0);
+        const float col = __shfl_sync(0xFFFFFFFFu, t0_next, 0);
         const bool tame = __all_sync(0xFFFFFFFFu, fabsf(s) <= kTame && fabsf(t0_next) <= kTame &&
                                                       fabsf(t1_next) <= kTame);
+        const bool one_factor = tame && p.col_shift != 0;
         float *cols = col_buf + (kb & 1) * COLS;
-        if (2 * lane < COLS) {
-          *reinterpret_cast<float2 *>(cols + 2 * lane) = make_float2(t0_next, t1_next);
+        if (!one_factor) {
+          // through the staging tile, once the last stores have read it
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+          if (2 * lane < COLS) {
+            *reinterpret_cast<float2 *>(cols + 2 * lane) = make_float2(t0_next, t1_next);
+          }
+          __syncwarp();
         }
         if (kb + 1 < seg.k1) {
           rs += p.row_blocks;
           cs += p.col_blocks;
-          s_next = row_in ? __ldg(rs + ri) : 0.0f;
-          t0_next = in0 ? __ldg(cs + i0) : 0.0f;
-          t1_next = in1 ? __ldg(cs + i1) : 0.0f;
+          load_scales();
         }
-        __syncwarp();  // the column scales are in place
         ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.g.status,
                        kDevTimeoutEpilogue, p.g.wait_cycles);
         ok = __all_sync(0xFFFFFFFFu, ok);
@@ -593,8 +610,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         const uint32_t done = bar_acc_empty + 8 * acc;
         if (!tame) {
           add_block<BN, kTwoSteps>(taddr, done, lane, cols, s, 0.0f, sum);
-        } else if (p.col_shift != 0) {
-          add_block<BN, kOneFactor>(taddr, done, lane, cols, s, t, sum);
+        } else if (one_factor) {
+          add_block<BN, kOneFactor>(taddr, done, lane, cols, s, col, sum);
         } else {
           add_block<BN, kColumnFactors>(taddr, done, lane, cols, s, 0.0f, sum);
         }
@@ -603,6 +620,10 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
           acc_phase ^= 1;
         }
       }
+      // the next tile's first scales are on their way while this tile is stored
+      Segment next{};
+      more = walk.next(p, next);
+      if (more) first_scales(next);
       float(&re)[COLS] = sum[0], (&im)[COLS] = sum[1];
       bool finish = ok;
       if (seg.k1 - seg.k0 < p.g.k_blocks) {
@@ -660,6 +681,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         }
         if (!stored) store_direct<OutT, COLS>(p.g, t.b, m, n0, re, im);
       }
+      seg = next;
     }
     if (p.g.epi_tma && lane == 0) bulk_wait_group<0>();
     __syncwarp();
