@@ -20,6 +20,7 @@
 // equal runs of 128-k blocks instead of whole tiles: a CTA that holds part of a tile's blocks writes
 // its sums to the plan's workspace, and the CTA that completes the tile adds the parts in the order
 // of k, whoever that is, so results do not depend on timing.
+#include <cstdlib>
 #include <new>
 
 #include "gemm_kernels.cuh"
@@ -338,35 +339,62 @@ __device__ __forceinline__ void store_boxes(const GemmParams &p, const CUtensorM
   }
 }
 
-// Row m, COLS columns from n0, straight from registers.
+// Row m (m0 + lane), COLS columns from n0, without the TMA unit.  Row-major rows that start anywhere turn in
+// the warp's staging tiles, kTurn columns of one plane at a time, so that lanes store along the row
+// (a lane to a row, a store touched 32 rows: 3 x 1000 x 2501 x 1984 took 180 us).
 template <typename OutT, int COLS>
-__device__ __forceinline__ void store_direct(const GemmParams &p, uint32_t b, uint32_t m, uint32_t n0,
-                                             const float (&re)[COLS], const float (&im)[COLS]) {
-  if (m >= p.M || n0 >= p.N) return;
+__device__ __forceinline__ void store_direct(const GemmParams &p, float *turn, uint32_t lane, uint32_t b,
+                                             uint32_t m0, uint32_t n0, const float (&re)[COLS],
+                                             const float (&im)[COLS]) {
+  if (m0 >= p.M || n0 >= p.N) return;  // uniform over the warp
   using Tr = OutTraits<OutT>;
   OutT *C = static_cast<OutT *>(p.c);
-  const COffsets o = c_offsets(p, b, m, n0);
-  const int valid = static_cast<int>(min(static_cast<uint32_t>(COLS), p.N - n0));
-  if (p.vec_ok && valid == COLS && p.c_layout == kPlanarRow) {
-    store_run<OutT, COLS>(C + o.base_re, re, valid, true);
-    store_run<OutT, COLS>(C + o.base_re + o.off_im, im, valid, true);
+  if (p.c_layout == kPlanarRow || p.c_layout == kInterRow) {
+    constexpr int kTurn = COLS < 32 ? COLS : 32;
+    static_assert(32 * kTurn * sizeof(float) <= kStoreTiles * kStoreTile, "staging");
+    constexpr uint32_t kRows = 32 / kTurn;  // rows stored by one instruction
+    const COffsets o = c_offsets(p, b, m0, n0);
+    const size_t pitch = (p.c_layout == kInterRow ? 2 : 1) * static_cast<size_t>(p.N);
+    const uint32_t rows = min(32u, p.M - m0), col = lane % kTurn, sub = lane / kTurn;
+#pragma unroll
+    for (int c = 0; c < COLS; c += kTurn) {
+#pragma unroll
+      for (int plane = 0; plane < 2; ++plane) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kTurn; ++j) {
+          turn[lane * kTurn + (j ^ (lane & (kTurn - 1)))] = plane == 0 ? re[c + j] : im[c + j];
+        }
+        __syncwarp();
+        OutT *dst = C + o.base_re + (plane == 0 ? 0 : o.off_im) + (c + col) * o.stride_j;
+        if (n0 + c + col < p.N) {
+          for (uint32_t r = sub; r < rows; r += kRows) {
+            dst[r * pitch] = Tr::to_out(turn[r * kTurn + (col ^ (r & (kTurn - 1)))]);
+          }
+        }
+      }
+    }
+    __syncwarp();
     return;
   }
-  if (p.c_layout == kInterRow || p.c_layout == kInterCol) {
+  // column-major: consecutive lanes hold consecutive rows
+  const uint32_t m = m0 + lane;
+  if (m >= p.M) return;
+  const COffsets o = c_offsets(p, b, m, n0);
+  const int valid = static_cast<int>(min(static_cast<uint32_t>(COLS), p.N - n0));
+  if (p.c_layout == kInterCol && p.pair_ok) {
     // one store per complex value
     struct alignas(2 * sizeof(OutT)) Pair {
       OutT re, im;
     };
-    if (p.pair_ok) {
 #pragma unroll
-      for (int j = 0; j < COLS; ++j) {
-        if (j < valid) {
-          *reinterpret_cast<Pair *>(C + o.base_re + j * o.stride_j) =
-              Pair{Tr::to_out(re[j]), Tr::to_out(im[j])};
-        }
+    for (int j = 0; j < COLS; ++j) {
+      if (j < valid) {
+        *reinterpret_cast<Pair *>(C + o.base_re + j * o.stride_j) =
+            Pair{Tr::to_out(re[j]), Tr::to_out(im[j])};
       }
-      return;
     }
+    return;
   }
 #pragma unroll
   for (int j = 0; j < COLS; ++j) {
@@ -633,12 +661,15 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         constexpr size_t kPart = 2 * BN * kBlockM;
         const uint64_t units = static_cast<uint64_t>(p.g.num_tiles) * p.g.k_blocks;
         const uint64_t base = static_cast<uint64_t>(seg.tile) * p.g.k_blocks;
-        const uint32_t at = first_col * kBlockM + quad * 32 + lane;
+        // [plane][column / 4][row][column % 4]: a lane moves four columns of its row at a time
+        const uint32_t at = (first_col * kBlockM + (quad * 32 + lane) * 4);
         float *mine = p.parts + (2 * static_cast<size_t>(blockIdx.x) + (seg.k0 == 0 ? 1 : 0)) * kPart + at;
 #pragma unroll
-        for (int j = 0; j < COLS; ++j) {
-          __stcg(mine + j * kBlockM, re[j]);
-          __stcg(mine + (BN + j) * kBlockM, im[j]);
+        for (int j = 0; j < COLS; j += 4) {
+          __stcg(reinterpret_cast<float4 *>(mine + j * kBlockM),
+                 make_float4(re[j], re[j + 1], re[j + 2], re[j + 3]));
+          __stcg(reinterpret_cast<float4 *>(mine + (BN + j) * kBlockM),
+                 make_float4(im[j], im[j + 1], im[j + 2], im[j + 3]));
         }
         __threadfence();
         epi_sync<32 * C::kEpiWarps>();
@@ -662,9 +693,11 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             const uint32_t slot = run_start(units, gridDim.x, c) > base ? 0 : 1;
             const float *part = p.parts + (2 * static_cast<size_t>(c) + slot) * kPart + at;
 #pragma unroll
-            for (int j = 0; j < COLS; ++j) {
-              re[j] += __ldcg(part + j * kBlockM);
-              im[j] += __ldcg(part + (BN + j) * kBlockM);
+            for (int j = 0; j < COLS; j += 4) {
+              const float4 x = __ldcg(reinterpret_cast<const float4 *>(part + j * kBlockM));
+              const float4 y = __ldcg(reinterpret_cast<const float4 *>(part + (BN + j) * kBlockM));
+              re[j] += x.x; re[j + 1] += x.y; re[j + 2] += x.z; re[j + 3] += x.w;
+              im[j] += y.x; im[j + 1] += y.y; im[j + 2] += y.z; im[j + 3] += y.w;
             }
           }
         }
@@ -679,7 +712,9 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
             stored = true;
           }
         }
-        if (!stored) store_direct<OutT, COLS>(p.g, t.b, m, n0, re, im);
+        if (!stored) {
+          store_direct<OutT, COLS>(p.g, col_buf, lane, t.b, t.mt * kBlockM + quad * 32, n0, re, im);
+        }
       }
       seg = next;
     }
@@ -799,18 +834,50 @@ extern "C" int ccglib_b200_scaled_gemm_plan_create(const ccglib_b200_scaled_gemm
   plan.swapped = d.m <= 64 && d.m < d.n;
   plan.rows = plan.swapped ? d.n : d.m;
   plan.cols = plan.swapped ? d.m : d.n;
-  plan.bn = plan.cols <= 16 ? 16 : plan.cols <= 32 ? 32 : plan.cols <= 64 ? 64 : 128;
-  plan.tiles = d.batch * ceil_div<size_t>(plan.rows, kBlockM) * ceil_div<size_t>(plan.cols, plan.bn);
+  const size_t sms = static_cast<size_t>(plan.sms);
+  const int narrowest = plan.cols <= 16 ? 16 : plan.cols <= 32 ? 32 : plan.cols <= 64 ? 64 : 0;
+  const char *env = std::getenv("CCGLIB_B200_SCALED_BN");
+  const int forced_bn = env != nullptr ? std::atoi(env) : 0;
+  env = std::getenv("CCGLIB_B200_SCALED_RUNS");
+  const int forced_runs = env != nullptr && *env != '\0' ? std::atoi(env) : -1;
+  // Whole tiles, or all blocks in equal runs?  And 128 or 64 columns where there is a choice?  Estimated
+  // in clocks; on 16 shapes from 256 x 256 x 256 to 4096 x 4096 x 4096 the choice is within 6 % of the
+  // best of the four forms (1024 x 1024 x 1024: 10.4 us, the others 13 to 18; 256 x 256 x 4096: 16.7,
+  // the others 23 to 32; 2048 x 2048 x 2048: 38, the others 49 to 53).
+  const size_t col_block = plan.swapped ? d.a_block_rows : d.b_block_rows;
+  double least = 0.0;
+  for (int bn : {128, 64, 32, 16}) {
+    if (narrowest != 0 ? bn != narrowest : bn < 64) continue;
+    if (forced_bn != 0 && narrowest == 0 && bn != forced_bn) continue;
+    const size_t tiles = d.batch * ceil_div<size_t>(plan.rows, kBlockM) * ceil_div<size_t>(plan.cols, bn);
+    const size_t units = tiles * plan.k_blocks;
+    // clocks of one block, of storing a tile, and of adding a shared tile's parts, measured
+    const bool one = col_block == 1;  // a factor for every column
+    const double block = bn == 128 ? (one ? 2200.0 : 1600.0) : bn == 64 ? (one ? 1450.0 : 1150.0) : 800.0;
+    const double store = 40.0 * bn, part = 350.0 * bn;
+    const double whole = static_cast<double>(ceil_div(tiles, sms)) *
+                         (static_cast<double>(plan.k_blocks) * block + store);
+    const size_t ctas = units / 4 < sms ? units / 4 : sms;
+    const double shared = ctas > 0 ? static_cast<double>(units) / static_cast<double>(ctas) * block +
+                                         store + part
+                                   : 0.0;
+    const bool may_share = plan.k_blocks > 1 && ctas > 1 && ceil_div(tiles, sms) <= 4;
+    const bool runs = may_share && (forced_runs >= 0 ? forced_runs != 0 : shared < whole);
+    const double cost = runs ? shared : whole;
+    if (plan.tiles == 0 || cost < least) {
+      least = cost;
+      plan.bn = bn;
+      plan.tiles = tiles;
+      plan.runs = runs ? ctas : 0;
+    }
+  }
+  if (plan.tiles == 0) {
+    set_last_error("CCGLIB_B200_SCALED_BN must be 64 or 128");
+    return CCGLIB_B200_INVALID_ARGUMENT;
+  }
   if (plan.tiles > 0x7FFFFFFFull) {
     set_last_error("scaled_gemm_plan_create: too many tiles");
     return CCGLIB_B200_INVALID_ARGUMENT;
-  }
-  const size_t sms = static_cast<size_t>(plan.sms);
-  const size_t waves = ceil_div(plan.tiles, sms);
-  const size_t units = plan.tiles * plan.k_blocks;
-  if (waves <= 4 && plan.k_blocks > 1 && plan.tiles * 10 < waves * sms * 9) {
-    const size_t ctas = units / 4 < sms ? units / 4 : sms;
-    if (ctas > plan.tiles) plan.runs = ctas;
   }
   switch (d.type_out) {
   case CCGLIB_B200_FLOAT32:
