@@ -5,6 +5,8 @@
 //   ccglib::transpose::Transpose     (reference include/ccglib/transpose/transpose.h:14-54)
 //   ccglib::packing::Packing         (reference include/ccglib/packing/packing.h:25-54)
 //   ccglib::pipeline::Pipeline       (reference include/ccglib/pipeline/pipeline.h:28-73)
+//   ccglib::quantize::Quantize, ccglib::mma::ScaledGEMM, ccglib::orthogonalize::Orthogonalize
+//                                    (no counterpart there; same constructor and Run conventions)
 //   value types / enums              (reference include/ccglib/common/*.h, gemm/mem_order.h,
 //                                     gemm/variant.h)
 //
@@ -199,7 +201,233 @@ private:
   CUstream stream_;
 };
 
+// Block-scaled fp8 GEMM: A and B as quantize::Quantize writes them, one float32 scale per
+// a_block_rows (b_block_rows) rows x 128 k; A and B may have different fp8 types.
+class ScaledGEMM {
+public:
+  ScaledGEMM(size_t B, size_t M, size_t N, size_t K, CUdevice &device, CUstream &stream,
+             ValuePrecision a_precision, ValuePrecision b_precision,
+             ValuePrecision output_precision = ValueType::float32, size_t a_block_rows = 1,
+             size_t b_block_rows = 128,
+             ComplexAxisLocation c_complex_axis_location = ComplexAxisLocation::complex_planar,
+             MemOrder c_mem_order = MemOrder::row_major, std::complex<float> alpha = {1, 0},
+             std::complex<float> beta = {0, 0})
+      : ScaledGEMM(FromHandles{}, B, M, N, K, device, stream, a_precision, b_precision,
+                   output_precision, a_block_rows, b_block_rows, c_complex_axis_location,
+                   c_mem_order, alpha, beta) {}
+  ~ScaledGEMM() { ccglib_b200_scaled_gemm_plan_destroy(plan_); }
+  ScaledGEMM(const ScaledGEMM &) = delete;
+  ScaledGEMM &operator=(const ScaledGEMM &) = delete;
+
+  // Asynchronous on the stream given at construction; no allocation, no synchronisation.
+  void Run(CUdeviceptr d_a, CUdeviceptr d_a_scale, CUdeviceptr d_b, CUdeviceptr d_b_scale,
+           CUdeviceptr d_c) {
+    detail::check(ccglib_b200_scaled_gemm_run(
+        plan_, detail::ptr(d_a), static_cast<const float *>(detail::ptr(d_a_scale)),
+        detail::ptr(d_b), static_cast<const float *>(detail::ptr(d_b_scale)), detail::ptr(d_c),
+        stream_));
+  }
+
+  // The stream this object enqueues on (the handle given at construction).
+  CUstream stream() const { return stream_; }
+
+#ifdef CCGLIB_B200_HAVE_CUDAWRAPPERS
+  ScaledGEMM(size_t B, size_t M, size_t N, size_t K, cu::Device &device, cu::Stream &stream,
+             ValuePrecision a_precision, ValuePrecision b_precision,
+             ValuePrecision output_precision = ValueType::float32, size_t a_block_rows = 1,
+             size_t b_block_rows = 128,
+             ComplexAxisLocation c_complex_axis_location = ComplexAxisLocation::complex_planar,
+             MemOrder c_mem_order = MemOrder::row_major, std::complex<float> alpha = {1, 0},
+             std::complex<float> beta = {0, 0})
+      : ScaledGEMM(FromHandles{}, B, M, N, K, static_cast<CUdevice>(device),
+                   static_cast<CUstream>(stream), a_precision, b_precision, output_precision,
+                   a_block_rows, b_block_rows, c_complex_axis_location, c_mem_order, alpha, beta) {}
+  void Run(cu::DeviceMemory &d_a, cu::DeviceMemory &d_a_scale, cu::DeviceMemory &d_b,
+           cu::DeviceMemory &d_b_scale, cu::DeviceMemory &d_c) {
+    Run(static_cast<CUdeviceptr>(d_a), static_cast<CUdeviceptr>(d_a_scale),
+        static_cast<CUdeviceptr>(d_b), static_cast<CUdeviceptr>(d_b_scale),
+        static_cast<CUdeviceptr>(d_c));
+  }
+#endif
+
+private:
+  struct FromHandles {};
+  ScaledGEMM(FromHandles, size_t B, size_t M, size_t N, size_t K, CUdevice device, CUstream stream,
+             ValuePrecision a, ValuePrecision b, ValuePrecision out, size_t a_block_rows,
+             size_t b_block_rows, ComplexAxisLocation c_axis, MemOrder c_order,
+             std::complex<float> alpha, std::complex<float> beta)
+      : stream_(stream) {
+    (void)device;  // the current context's device is used, as with the other classes
+    ccglib_b200_scaled_gemm_desc d{};
+    d.batch = B;
+    d.m = M;
+    d.n = N;
+    d.k = K;
+    d.type_a = static_cast<ValueType>(a);
+    d.type_b = static_cast<ValueType>(b);
+    d.type_out = static_cast<ValueType>(out);
+    d.a_block_rows = a_block_rows;
+    d.b_block_rows = b_block_rows;
+    d.c_complex_axis = c_axis;
+    d.c_mem_order = c_order;
+    d.alpha_re = alpha.real();
+    d.alpha_im = alpha.imag();
+    d.beta_re = beta.real();
+    d.beta_im = beta.imag();
+    detail::check(ccglib_b200_scaled_gemm_plan_create(&d, &plan_));
+  }
+
+  ccglib_b200_scaled_gemm_plan *plan_ = nullptr;
+  CUstream stream_;
+};
+
 } // namespace mma
+
+// ---- Quantize -----------------------------------------------------------------------------------
+
+namespace quantize {
+
+// Complex float16 / bfloat16 / float32 matrices -> fp8 planes [B][2][rows][Pitch(K)] and float32
+// scales [B][ceil(K / 128)][ceil(rows / block_rows)]: the operands of mma::ScaledGEMM.
+class Quantize {
+public:
+  Quantize(size_t B, size_t rows, size_t K, CUdevice &device, CUstream &stream,
+           ValuePrecision input_precision, ValuePrecision output_precision, size_t block_rows = 1,
+           ComplexAxisLocation input_complex_axis_location = ComplexAxisLocation::complex_planar,
+           mma::MemOrder input_mem_order = mma::MemOrder::row_major)
+      : Quantize(FromHandles{}, B, rows, K, device, stream, input_precision, output_precision,
+                 block_rows, input_complex_axis_location, input_mem_order) {}
+
+  // Asynchronous on the stream given at construction; no allocation, no synchronisation.
+  void Run(CUdeviceptr d_input, CUdeviceptr d_output, CUdeviceptr d_scale) {
+    detail::check(ccglib_b200_quantize_run(&desc_, detail::ptr(d_input), detail::ptr(d_output),
+                                           static_cast<float *>(detail::ptr(d_scale)), stream_));
+  }
+
+  // The stream this object enqueues on (the handle given at construction).
+  CUstream stream() const { return stream_; }
+
+  static size_t Pitch(size_t K) { return helper::ceildiv(K, size_t{16}) * 16; }
+  size_t OutputBytes() const { return desc_.batch * 2 * desc_.rows * Pitch(desc_.k); }
+  size_t ScaleBytes() const {
+    return desc_.batch * helper::ceildiv(desc_.k, size_t{128}) *
+           helper::ceildiv(desc_.rows, desc_.block_rows) * sizeof(float);
+  }
+
+#ifdef CCGLIB_B200_HAVE_CUDAWRAPPERS
+  Quantize(size_t B, size_t rows, size_t K, cu::Device &device, cu::Stream &stream,
+           ValuePrecision input_precision, ValuePrecision output_precision, size_t block_rows = 1,
+           ComplexAxisLocation input_complex_axis_location = ComplexAxisLocation::complex_planar,
+           mma::MemOrder input_mem_order = mma::MemOrder::row_major)
+      : Quantize(FromHandles{}, B, rows, K, static_cast<CUdevice>(device),
+                 static_cast<CUstream>(stream), input_precision, output_precision, block_rows,
+                 input_complex_axis_location, input_mem_order) {}
+  void Run(cu::DeviceMemory &d_input, cu::DeviceMemory &d_output, cu::DeviceMemory &d_scale) {
+    Run(static_cast<CUdeviceptr>(d_input), static_cast<CUdeviceptr>(d_output),
+        static_cast<CUdeviceptr>(d_scale));
+  }
+#endif
+
+private:
+  struct FromHandles {};
+  Quantize(FromHandles, size_t B, size_t rows, size_t K, CUdevice device, CUstream stream,
+           ValuePrecision in, ValuePrecision out, size_t block_rows, ComplexAxisLocation axis,
+           mma::MemOrder order)
+      : stream_(stream) {
+    (void)device;
+    if (block_rows != 1 && block_rows != 128) {
+      throw std::runtime_error("a block has 1 or 128 rows");
+    }
+    desc_.batch = B;
+    desc_.rows = rows;
+    desc_.k = K;
+    desc_.type_in = static_cast<ValueType>(in);
+    desc_.type_out = static_cast<ValueType>(out);
+    desc_.input_complex_axis = axis;
+    desc_.input_mem_order = order;
+    desc_.block_rows = block_rows;
+  }
+
+  ccglib_b200_quantize_desc desc_{};
+  CUstream stream_;
+};
+
+} // namespace quantize
+
+// ---- Orthogonalize ------------------------------------------------------------------------------
+
+namespace orthogonalize {
+
+// Coefficients (a, b, c) of a step X <- a X + (b S + c S^2) X, S = X X^H.
+struct Coefficients {
+  float a, b, c;
+};
+// Steep at zero; five steps bring the singular values of any full-rank matrix to about 0.7 .. 1.2.
+constexpr Coefficients quintic{3.4445f, -4.7750f, 2.0315f};
+// Newton-Schulz of fifth order: converges to orthonormal rows (columns).
+constexpr Coefficients convergent{1.875f, -1.25f, 0.375f};
+
+// Newton-Schulz orthogonalisation of B complex M x N matrices; output planar float16 or bfloat16.
+class Orthogonalize {
+public:
+  Orthogonalize(size_t B, size_t M, size_t N, CUdevice &device, CUstream &stream,
+                ValuePrecision input_precision, ValuePrecision output_precision, int steps = 5,
+                Coefficients coefficients = quintic,
+                ComplexAxisLocation input_complex_axis_location = ComplexAxisLocation::complex_planar)
+      : Orthogonalize(FromHandles{}, B, M, N, device, stream, input_precision, output_precision,
+                      steps, coefficients, input_complex_axis_location) {}
+  ~Orthogonalize() { ccglib_b200_orthogonalize_plan_destroy(plan_); }
+  Orthogonalize(const Orthogonalize &) = delete;
+  Orthogonalize &operator=(const Orthogonalize &) = delete;
+
+  // Asynchronous on the stream given at construction; no allocation, no synchronisation.
+  void Run(CUdeviceptr d_input, CUdeviceptr d_output) {
+    detail::check(ccglib_b200_orthogonalize_run(plan_, detail::ptr(d_input), detail::ptr(d_output),
+                                                stream_));
+  }
+
+  // The stream this object enqueues on (the handle given at construction).
+  CUstream stream() const { return stream_; }
+
+#ifdef CCGLIB_B200_HAVE_CUDAWRAPPERS
+  Orthogonalize(size_t B, size_t M, size_t N, cu::Device &device, cu::Stream &stream,
+                ValuePrecision input_precision, ValuePrecision output_precision, int steps = 5,
+                Coefficients coefficients = quintic,
+                ComplexAxisLocation input_complex_axis_location = ComplexAxisLocation::complex_planar)
+      : Orthogonalize(FromHandles{}, B, M, N, static_cast<CUdevice>(device),
+                      static_cast<CUstream>(stream), input_precision, output_precision, steps,
+                      coefficients, input_complex_axis_location) {}
+  void Run(cu::DeviceMemory &d_input, cu::DeviceMemory &d_output) {
+    Run(static_cast<CUdeviceptr>(d_input), static_cast<CUdeviceptr>(d_output));
+  }
+#endif
+
+private:
+  struct FromHandles {};
+  Orthogonalize(FromHandles, size_t B, size_t M, size_t N, CUdevice device, CUstream stream,
+                ValuePrecision in, ValuePrecision out, int steps, Coefficients coefficients,
+                ComplexAxisLocation axis)
+      : stream_(stream) {
+    (void)device;
+    ccglib_b200_orthogonalize_desc d{};
+    d.batch = B;
+    d.m = M;
+    d.n = N;
+    d.type_in = static_cast<ValueType>(in);
+    d.type_out = static_cast<ValueType>(out);
+    d.input_complex_axis = axis;
+    d.steps = steps;
+    d.a = coefficients.a;
+    d.b = coefficients.b;
+    d.c = coefficients.c;
+    detail::check(ccglib_b200_orthogonalize_plan_create(&d, &plan_));
+  }
+
+  ccglib_b200_orthogonalize_plan *plan_ = nullptr;
+  CUstream stream_;
+};
+
+} // namespace orthogonalize
 
 // ---- Transpose ----------------------------------------------------------------------------------
 
