@@ -56,20 +56,25 @@ int make_map(CUtensorMap *tm, const void *base, uint64_t row_bytes, uint64_t row
              uint32_t box_slices);
 
 // Launch with programmatic stream serialisation: the kernel may be set up while the one before it on
-// the stream finishes, and waits for it (griddepcontrol.wait) before it touches memory.
+// the stream finishes, and waits for it (griddepcontrol.wait) before it touches memory.  `cluster` CTAs
+// form a cluster (1: none).
 template <typename... Params, typename... Args>
 cudaError_t launch_programmatic(void (*kernel)(Params...), unsigned grid, unsigned threads,
-                                size_t smem, cudaStream_t stream, const Args &...args) {
+                                size_t smem, int cluster, cudaStream_t stream, const Args &...args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attrs[2]{};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

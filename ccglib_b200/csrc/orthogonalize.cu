@@ -215,6 +215,111 @@ __device__ __forceinline__ void orth_store(const OrthParams &p, const CUtensorMa
   }
 }
 
+constexpr uint32_t kAtom = 2 * kOrthK * 128;  // 64 values along M or N of both planes, MN-major
+
+// Loads of one stage: block kb of K of tile t.
+template <int BN, bool A_MN, bool B_MN>
+__device__ __forceinline__ void load_stage(const CUtensorMap *tm_a, const CUtensorMap *tm_b,
+                                           const TileCoord &t, uint32_t kb, uint32_t dst, uint32_t full) {
+  using C = OrthCfg<BN>;
+  const int32_t k = static_cast<int32_t>(kb * kOrthK), z = static_cast<int32_t>(2 * t.b);
+  const int32_t m0 = static_cast<int32_t>(t.mt * kBlockM), n0 = static_cast<int32_t>(t.nt * BN);
+  mbar_arrive_expect_tx(full, C::kStageBytes);
+  if constexpr (A_MN) {
+#pragma unroll
+    for (int i = 0; i < kBlockM / 64; ++i) tma_load_3d(dst + i * kAtom, tm_a, (m0 + 64 * i) * 2, k, z, full);
+  } else {
+    tma_load_3d(dst, tm_a, k * 2, m0, z, full);
+  }
+  if constexpr (B_MN) {
+#pragma unroll
+    for (int i = 0; i < BN / 64; ++i) {
+      tma_load_3d(dst + C::kABytes + i * kAtom, tm_b, (n0 + 64 * i) * 2, k, z, full);
+    }
+  } else {
+    tma_load_3d(dst + C::kABytes, tm_b, k * 2, n0, z, full);
+  }
+}
+
+// MMAs of one stage into the accumulators at d; more: add to what is there.
+template <int BN, bool A_MN, bool B_MN>
+__device__ __forceinline__ void issue_stage(uint32_t a_base, uint32_t d, bool conj_b, bool more) {
+  using C = OrthCfg<BN>;
+  // descriptor: fp32 sums, f16 operands, bit 13 negates A, bits 15 / 16 say that A / B is MN-major
+  constexpr uint32_t kIdesc = (1u << 4) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) |
+                              (static_cast<uint32_t>((C::kStacked ? 2 * BN : BN) >> 3) << 17) |
+                              (static_cast<uint32_t>(kBlockM >> 4) << 24);
+  constexpr uint32_t kNegA = kIdesc | (1u << 13);
+  // A x B^T: Re = Ar.Br - Ai.Bi, Im = Ar.Bi + Ai.Br; with conj(B): Re = Ar.Br + Ai.Bi, Im = Ai.Br - Ar.Bi
+  const uint32_t ar_bi = conj_b ? kNegA : kIdesc, ai_bi = conj_b ? kIdesc : kNegA;
+  const uint32_t b_base = a_base + C::kABytes;
+#pragma unroll
+  for (int k = 0; k < kOrthK / 16; ++k) {
+    // plane of 64 x 64 values of an MN-major atom: 8 KiB; 16 rows of K: 2 KiB
+    const uint64_t a_re = A_MN ? smem_desc_mn(a_base + k * 2048, kAtom) : smem_desc<128>(a_base + k * 32);
+    const uint64_t a_im = A_MN ? smem_desc_mn(a_base + kAtom / 2 + k * 2048, kAtom)
+                               : smem_desc<128>(a_base + kBlockM * 128 + k * 32);
+    const uint32_t add = more || k != 0 ? 1u : 0u;
+    if constexpr (C::kStacked) {
+      // both B planes lie one behind the other: [Ar.Br | Ar.Bi], [Ai.Br | Ai.Bi]
+      const uint64_t b_both = B_MN ? smem_desc_mn(b_base + k * 2048, kAtom / 2)
+                                   : smem_desc<128>(b_base + k * 32);
+      tc_mma<kKindF16>(d, a_re, b_both, kIdesc, add);
+      tc_mma<kKindF16>(d + 2 * BN, a_im, b_both, kIdesc, add);
+    } else {
+      const uint64_t b_re = B_MN ? smem_desc_mn(b_base + k * 2048, kAtom) : smem_desc<128>(b_base + k * 32);
+      const uint64_t b_im = B_MN ? smem_desc_mn(b_base + kAtom / 2 + k * 2048, kAtom)
+                                 : smem_desc<128>(b_base + BN * 128 + k * 32);
+      tc_mma<kKindF16>(d, a_re, b_re, kIdesc, add);
+      tc_mma<kKindF16>(d + BN, a_re, b_im, ar_bi, add);
+      tc_mma<kKindF16>(d + BN, a_im, b_re, kIdesc, 1u);
+      tc_mma<kKindF16>(d, a_im, b_im, ai_bi, 1u);
+    }
+  }
+}
+
+// 32 columns of the accumulators at taddr as Re and Im.
+template <int BN>
+__device__ __forceinline__ void read_chunk(uint32_t taddr, bool conj_b, float (&re)[32], float (&im)[32]) {
+  uint32_t r[32], i[32];
+  tmem_ld_32x32b_x32(taddr, r);
+  tmem_ld_32x32b_x32(taddr + BN, i);
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    re[j] = __uint_as_float(r[j]);
+    im[j] = __uint_as_float(i[j]);
+  }
+  if constexpr (OrthCfg<BN>::kStacked) {
+    tmem_ld_32x32b_x32(taddr + 2 * BN, i);  // Ai.Br
+    tmem_ld_32x32b_x32(taddr + 3 * BN, r);  // Ai.Bi
+    tmem_wait_ld();
+    const float sign = conj_b ? -1.0f : 1.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      re[j] -= sign * __uint_as_float(r[j]);
+      im[j] = sign * im[j] + __uint_as_float(i[j]);
+    }
+  }
+}
+
+// After an abort: our own copies must land before the CTA leaves (or reuses its stages).
+template <int STAGES>
+__device__ __forceinline__ void drain_loads(uint32_t bar_full, uint32_t issued, uint32_t stage,
+                                            uint32_t phase, const OrthParams &p) {
+  for (int s = 0; s < STAGES; ++s) {
+    if (!(issued & (1u << s))) continue;
+    const uint32_t parity = (static_cast<uint32_t>(s) < stage) ? phase : (phase ^ 1);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar_full + 8 * s, parity)) {
+      if (clock64() - t0 > p.wait_cycles) {
+        atomicOr(p.status, kDevTimeoutDrain);
+        break;
+      }
+    }
+  }
+}
+
 // result = gain * (alpha * A x op(B)^T + beta * c0), tiles of 128 x BN.  An operand that is MN-major is
 // stored [K][M or N]; the others are stored [M or N][K].  Roles as in cgemm_tcgen05_kernel.
 template <int BN, bool A_MN, bool B_MN>
@@ -224,7 +329,6 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const __grid_constant__ CUtensorMap tm_c, const OrthParams p) {
   using C = OrthCfg<BN>;
   constexpr int kStages = C::kStages;
-  constexpr uint32_t kAtom = 2 * kOrthK * 128;  // 64 values along M or N of both planes
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
@@ -278,27 +382,8 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
           break;
         }
         if (lane == 0) {
-          const uint32_t full = bar_full + 8 * stage;
-          const uint32_t dst = smem_base + stage * C::kStageBytes;
-          const int32_t k = static_cast<int32_t>(kb * kOrthK), z = static_cast<int32_t>(2 * t.b);
-          const int32_t m0 = static_cast<int32_t>(t.mt * kBlockM), n0 = static_cast<int32_t>(t.nt * BN);
-          mbar_arrive_expect_tx(full, C::kStageBytes);
-          if constexpr (A_MN) {
-#pragma unroll
-            for (int i = 0; i < kBlockM / 64; ++i) {
-              tma_load_3d(dst + i * kAtom, &tm_a, (m0 + 64 * i) * 2, k, z, full);
-            }
-          } else {
-            tma_load_3d(dst, &tm_a, k * 2, m0, z, full);
-          }
-          if constexpr (B_MN) {
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i) {
-              tma_load_3d(dst + C::kABytes + i * kAtom, &tm_b, (n0 + 64 * i) * 2, k, z, full);
-            }
-          } else {
-            tma_load_3d(dst + C::kABytes, &tm_b, k * 2, n0, z, full);
-          }
+          load_stage<BN, A_MN, B_MN>(&tm_a, &tm_b, t, kb, smem_base + stage * C::kStageBytes,
+                                     bar_full + 8 * stage);
         }
         __syncwarp();
         issued |= 1u << stage;
@@ -308,29 +393,9 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
         }
       }
     }
-    if (*abort_flag) {
-      // our own copies must land before the CTA leaves
-      for (int s = 0; s < kStages; ++s) {
-        if (!(issued & (1u << s))) continue;
-        const uint32_t parity = (static_cast<uint32_t>(s) < stage) ? phase : (phase ^ 1);
-        const long long t0 = clock64();
-        while (!mbar_try_wait(bar_full + 8 * s, parity)) {
-          if (clock64() - t0 > p.wait_cycles) {
-            atomicOr(p.status, kDevTimeoutDrain);
-            break;
-          }
-        }
-      }
-    }
+    if (*abort_flag) drain_loads<kStages>(bar_full, issued, stage, phase, p);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    // descriptor: fp32 sums, f16 operands, bit 13 negates A, bits 15 / 16 say that A / B is MN-major
-    constexpr uint32_t kIdesc = (1u << 4) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) |
-                                (static_cast<uint32_t>((C::kStacked ? 2 * BN : BN) >> 3) << 17) |
-                                (static_cast<uint32_t>(kBlockM >> 4) << 24);
-    constexpr uint32_t kNegA = kIdesc | (1u << 13);
-    // A x B^T: Re = Ar.Br - Ai.Bi, Im = Ar.Bi + Ai.Br; with conj(B): Re = Ar.Br + Ai.Bi, Im = Ai.Br - Ar.Bi
-    const uint32_t ar_bi = p.conj_b ? kNegA : kIdesc, ai_bi = p.conj_b ? kIdesc : kNegA;
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
     bool ok = true;
     for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
@@ -348,33 +413,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
         }
         tc_fence_after();
         if (lane == 0) {
-          const uint32_t a_base = smem_base + stage * C::kStageBytes;
-          const uint32_t b_base = a_base + C::kABytes;
-#pragma unroll
-          for (int k = 0; k < kOrthK / 16; ++k) {
-            // plane of 64 x 64 values of an MN-major atom: 8 KiB; 16 rows of K: 2 KiB
-            const uint64_t a_re = A_MN ? smem_desc_mn(a_base + k * 2048, kAtom)
-                                       : smem_desc<128>(a_base + k * 32);
-            const uint64_t a_im = A_MN ? smem_desc_mn(a_base + kAtom / 2 + k * 2048, kAtom)
-                                       : smem_desc<128>(a_base + kBlockM * 128 + k * 32);
-            const uint32_t more = (kb | static_cast<uint32_t>(k)) != 0 ? 1u : 0u;
-            if constexpr (C::kStacked) {
-              // both B planes lie one behind the other: [Ar.Br | Ar.Bi], [Ai.Br | Ai.Bi]
-              const uint64_t b_both = B_MN ? smem_desc_mn(b_base + k * 2048, kAtom / 2)
-                                           : smem_desc<128>(b_base + k * 32);
-              tc_mma<kKindF16>(d, a_re, b_both, kIdesc, more);
-              tc_mma<kKindF16>(d + 2 * BN, a_im, b_both, kIdesc, more);
-            } else {
-              const uint64_t b_re = B_MN ? smem_desc_mn(b_base + k * 2048, kAtom)
-                                         : smem_desc<128>(b_base + k * 32);
-              const uint64_t b_im = B_MN ? smem_desc_mn(b_base + kAtom / 2 + k * 2048, kAtom)
-                                         : smem_desc<128>(b_base + BN * 128 + k * 32);
-              tc_mma<kKindF16>(d, a_re, b_re, kIdesc, more);
-              tc_mma<kKindF16>(d + BN, a_re, b_im, ar_bi, more);
-              tc_mma<kKindF16>(d + BN, a_im, b_re, kIdesc, 1u);
-              tc_mma<kKindF16>(d, a_im, b_im, ai_bi, 1u);
-            }
-          }
+          issue_stage<BN, A_MN, B_MN>(smem_base + stage * C::kStageBytes, d, p.conj_b != 0, kb != 0);
           tc_commit(bar_empty + 8 * stage);
           if (kb + 1 == p.k_blocks) tc_commit(bar_acc_full + 8 * acc);
         }
@@ -408,27 +447,8 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
         const uint32_t n0 = t.nt * BN + c0;
         if (n0 >= p.n) break;
         if (m0 >= p.m || (p.hermitian && n0 < m0)) continue;  // comes from the mirror image
-        uint32_t r[32], i[32];
         float re[32], im[32];
-        tmem_ld_32x32b_x32(taddr + c0, r);
-        tmem_ld_32x32b_x32(taddr + BN + c0, i);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          re[j] = __uint_as_float(r[j]);
-          im[j] = __uint_as_float(i[j]);
-        }
-        if constexpr (C::kStacked) {
-          tmem_ld_32x32b_x32(taddr + 2 * BN + c0, i);  // Ai.Br
-          tmem_ld_32x32b_x32(taddr + 3 * BN + c0, r);  // Ai.Bi
-          tmem_wait_ld();
-          const float sign = p.conj_b ? -1.0f : 1.0f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            re[j] -= sign * __uint_as_float(r[j]);
-            im[j] = sign * im[j] + __uint_as_float(i[j]);
-          }
-        }
+        read_chunk<BN>(taddr + c0, p.conj_b != 0, re, im);
         orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
       }
       tc_fence_before();
@@ -452,37 +472,229 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
   }
 }
 
+// The same for problems whose tiles leave most SMs idle: a cluster of SPLIT CTAs shares the K of one
+// tile and every CTA finishes BN / SPLIT of its columns.  Partial sums travel through distributed shared
+// memory into the (by then unused) stages, and are added in the order of the CTAs.  1024 x 1024 on
+// 72 CTAs of 128 x 64 spent 15.5 k clocks per product loading 48 KiB per block of K through one SM's port to
+// L2; shared, a CTA loads half or a quarter of that.
+template <int BN, bool A_MN, bool B_MN, int SPLIT>
+__global__ void __launch_bounds__(kThreads, 1)
+orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                  const __grid_constant__ CUtensorMap tm_c, const OrthParams p) {
+  using C = OrthCfg<BN>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kChunks = BN / SPLIT / 32;  // 32-column pieces a CTA finishes
+  static_assert(BN % (32 * SPLIT) == 0, "whole pieces");
+  static_assert((SPLIT - 1) * 2 * kChunks * 4 * kStagingTile <= kStages * C::kStageBytes,
+                "partial sums exceed the stages");
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~static_cast<uintptr_t>(1023u));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * C::kStageBytes + kOrthStaging);
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_acc_full = bar_empty + 8 * kStages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_acc_full, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+    prefetch_tensormap(&tm_c);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  let_next_start();
+
+  const TileCoord t = orth_tile<BN>(p, cluster_id_x());
+  const uint32_t kb0 = p.k_blocks * rank / SPLIT, kb1 = p.k_blocks * (rank + 1) / SPLIT;
+  bool done = false;  // epilogue warps: this CTA's sums are complete
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    wait_for_previous();
+    uint32_t stage = 0, phase = 0, issued = 0;
+    for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, kDevTimeoutProducer,
+                     p.wait_cycles)) {
+        break;
+      }
+      if (lane == 0) {
+        load_stage<BN, A_MN, B_MN>(&tm_a, &tm_b, t, kb, smem_base + stage * C::kStageBytes,
+                                   bar_full + 8 * stage);
+      }
+      __syncwarp();
+      issued |= 1u << stage;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (*abort_flag) drain_loads<kStages>(bar_full, issued, stage, phase, p);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    uint32_t stage = 0, phase = 0;
+    for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, kDevTimeoutMma, p.wait_cycles)) {
+        break;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        issue_stage<BN, A_MN, B_MN>(smem_base + stage * C::kStageBytes, tmem_base, p.conj_b != 0, kb != kb0);
+        tc_commit(bar_empty + 8 * stage);
+        if (kb + 1 == kb1) tc_commit(bar_acc_full);
+      }
+      __syncwarp();
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  } else {
+    wait_for_previous();
+    done = mbar_wait(bar_acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue, p.wait_cycles);
+    done = __all_sync(0xFFFFFFFFu, done);
+  }
+  __syncwarp();
+
+  // every CTA of the cluster has read its stages (or given up): they may receive partial sums
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t quad = warp & 3;
+  const uint32_t taddr = tmem_base + ((quad * 32) << 16);
+  // 4 KiB for 32 rows x 32 columns of one plane from source i (of the SPLIT - 1 others)
+  auto recv = [&](uint32_t i, uint32_t plane, uint32_t c) {
+    return smem_base + ((((i * 2 + plane) * kChunks + c) * 4 + quad) * kStagingTile) + lane * 128;
+  };
+  if (warp >= 2 && done) {
+    for (uint32_t step = 1; step < SPLIT; ++step) {
+      const uint32_t dest = (rank + step) % SPLIT;
+      const uint32_t idx = rank - (rank > dest ? 1u : 0u);  // our place among dest's sources
+#pragma unroll 1
+      for (uint32_t c = 0; c < kChunks; ++c) {
+        float re[32], im[32];
+        read_chunk<BN>(taddr + (dest * kChunks + c) * 32, p.conj_b != 0, re, im);
+        const uint32_t to_re = map_to_cta(recv(idx, 0, c), dest), to_im = map_to_cta(recv(idx, 1, c), dest);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t off = (j ^ (lane & 7)) << 4;  // no bank is hit twice
+          st_shared_cluster_v4(to_re + off, __float_as_uint(re[4 * j]), __float_as_uint(re[4 * j + 1]),
+                               __float_as_uint(re[4 * j + 2]), __float_as_uint(re[4 * j + 3]));
+          st_shared_cluster_v4(to_im + off, __float_as_uint(im[4 * j]), __float_as_uint(im[4 * j + 1]),
+                               __float_as_uint(im[4 * j + 2]), __float_as_uint(im[4 * j + 3]));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();  // all partial sums are in place
+
+  if (warp >= 2 && done && !*abort_flag) {
+    const uint32_t staging = smem_base + kStages * C::kStageBytes + quad * (4 * kOrthBox);
+    const uint32_t m0 = t.mt * kBlockM + quad * 32;
+#pragma unroll 1
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      const uint32_t col = (rank * kChunks + c) * 32, n0 = t.nt * BN + col;
+      if (n0 >= p.n || m0 >= p.m || (p.hermitian && n0 < m0)) continue;
+      float re[32], im[32];
+      read_chunk<BN>(taddr + col, p.conj_b != 0, re, im);
+#pragma unroll 1
+      for (uint32_t i = 0; i + 1 < SPLIT; ++i) {
+        const uint32_t from_re = recv(i, 0, c), from_im = recv(i, 1, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t off = (j ^ (lane & 7)) << 4;
+          uint32_t x[4], y[4];
+          ld_shared_v4(from_re + off, x[0], x[1], x[2], x[3]);
+          ld_shared_v4(from_im + off, y[0], y[1], y[2], y[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            re[4 * j + e] += __uint_as_float(x[e]);
+            im[4 * j + e] += __uint_as_float(y[e]);
+          }
+        }
+      }
+      orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
+    }
+    if (lane == 0) bulk_wait_group<0>();
+  }
+  __syncwarp();
+
+  // ------------------------------------------------------------------ tear-down
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
 using OrthFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const OrthParams);
 
-template <int BN> OrthFn orth_kernel(bool a_mn, bool b_mn) {
-  return a_mn ? orth_product_kernel<BN, true, true>
-         : b_mn ? orth_product_kernel<BN, false, true>
-                : orth_product_kernel<BN, false, false>;
+template <int BN, bool A_MN, bool B_MN> OrthFn orth_kernel(int split) {
+  if constexpr (BN == 128) {
+    if (split == 4) return orth_split_kernel<BN, A_MN, B_MN, 4>;
+  }
+  return split == 2 ? orth_split_kernel<BN, A_MN, B_MN, 2> : orth_product_kernel<BN, A_MN, B_MN>;
 }
-OrthFn orth_kernel(int bn, bool a_mn, bool b_mn) {
-  return bn == 128 ? orth_kernel<128>(a_mn, b_mn) : orth_kernel<64>(a_mn, b_mn);
+template <int BN> OrthFn orth_kernel(int split, bool a_mn, bool b_mn) {
+  return a_mn   ? orth_kernel<BN, true, true>(split)
+         : b_mn ? orth_kernel<BN, false, true>(split)
+                : orth_kernel<BN, false, false>(split);
+}
+OrthFn orth_kernel(int bn, int split, bool a_mn, bool b_mn) {
+  return bn == 128 ? orth_kernel<128>(split, a_mn, b_mn) : orth_kernel<64>(split, a_mn, b_mn);
 }
 int orth_smem(int bn) { return bn == 128 ? OrthCfg<128>::kSmemBytes : OrthCfg<64>::kSmemBytes; }
 
-// Tiles of one product, of the width that finishes sooner: waves x tensor time of a tile.  (A 64-wide
-// tile takes half the MMAs of a 128-wide one.)
+// Tiles of one product: the width, and how many CTAs share the K of a tile.
 struct ProductShape {
-  int bn;
+  int bn, split;
   size_t per_batch;
 };
 
-ProductShape pick_shape(size_t batch, size_t m, size_t n, bool hermitian, size_t sms) {
-  ProductShape best{0, 0};
+// Estimated clocks: a block of K costs what its bytes take through the SM's port to L2 (64 KiB resp. 48 KiB,
+// 128 resp. 64 columns), a tile its epilogue, an exchange of partial sums 60 per column.
+ProductShape pick_shape(size_t batch, size_t m, size_t n, size_t k, bool hermitian, size_t sms) {
+  ProductShape best{0, 1, 0};
   double least = 0.0;
+  const size_t k_blocks = ceil_div<size_t>(k, kOrthK);
+  const char *env = std::getenv("CCGLIB_B200_ORTH_SPLIT");  // 1, 2 or 4: by hand, where it fits
+  const int forced = env != nullptr ? std::atoi(env) : 0;
   for (int bn : {128, 64}) {
     const size_t rows = ceil_div<size_t>(m, kBlockM), cols = ceil_div<size_t>(n, bn);
     size_t tiles = 0;
     for (size_t i = 0; i < rows; ++i) tiles += cols - (hermitian ? i * kBlockM / bn : 0);
-    const double cost =
-        static_cast<double>(ceil_div(batch * tiles, sms)) * (bn == 128 ? 1.0 : 0.6);
-    if (best.bn == 0 || cost < least) {
-      best = {bn, tiles};
-      least = cost;
+    for (int split : {1, 2, 4}) {
+      const size_t ctas = batch * tiles * split;
+      // (clusters of four do not fill the processor groups: at most 32 of them run at once)
+      if (split > 1 && (ctas > (split == 4 ? sms * 86 / 100 : sms) || k_blocks < static_cast<size_t>(split) || bn < 32 * split)) continue;
+      const double blocks = static_cast<double>(ceil_div<size_t>(k_blocks, split));
+      double cost = static_cast<double>(ceil_div(ctas, sms)) *
+                        (blocks * (bn == 128 ? 1250.0 : 950.0) + 25.0 * bn / split) +
+                    (split > 1 ? 60.0 * bn : 0.0);
+      if (forced != 0 && split == forced) cost *= 1e-3;
+      if (best.bn == 0 || cost < least) {
+        best = {bn, split, tiles};
+        least = cost;
+      }
     }
   }
   return best;
@@ -900,7 +1112,7 @@ struct ccglib_b200_orthogonalize_plan {
   size_t n_p, cols_p;   // row pitches of S and P, and of X: multiples of eight
   bool tall;            // m > n
   float scale;          // power of two near sqrt(long side)
-  ProductShape square, update;
+  ProductShape gram, poly, update;
   bool small;           // the whole iteration in one launch, a CTA per matrix
   size_t chunks;
   int device, sms;
@@ -962,14 +1174,14 @@ int make_maps(ccglib_b200_orthogonalize_plan &plan) {
   const size_t batch = plan.desc.batch;
   const Operand s = square_operand(plan, plan.s), p = square_operand(plan, plan.p);
   int rc = operand_map(&plan.s_a, s, batch, kBlockM);
-  if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.s_b, s, batch, plan.square.bn);
+  if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.s_b, s, batch, plan.poly.bn);
   if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.update_p, p, batch, plan.tall ? plan.update.bn : kBlockM);
   if (rc == CCGLIB_B200_OK) rc = result_map(&plan.s_out, plan.s, batch, plan.n, plan.n_p);
   if (rc == CCGLIB_B200_OK) rc = result_map(&plan.p_out, plan.p, batch, plan.n, plan.n_p);
   for (int i = 0; i < 2; ++i) {
     const Operand x_long = x_operand(plan, i, true), x_short = x_operand(plan, i, false);
     if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.gram_a[i], x_long, batch, kBlockM);
-    if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.gram_b[i], x_long, batch, plan.square.bn);
+    if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.gram_b[i], x_long, batch, plan.gram.bn);
     if (rc == CCGLIB_B200_OK) {
       rc = operand_map(&plan.update_x[i], x_short, batch, plan.tall ? kBlockM : plan.update.bn);
     }
@@ -1002,9 +1214,11 @@ int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q,
   g.n_out = static_cast<uint32_t>(q.out_pitch);
   g.status = plan.status;
   g.wait_cycles = plan.wait_cycles;
-  const unsigned grid = g.num_tiles < static_cast<uint32_t>(plan.sms) ? g.num_tiles : plan.sms;
-  CCGLIB_CUDA_TRY(launch_programmatic(orth_kernel(q.shape.bn, q.a.by_rows, q.b.by_rows), grid, kThreads,
-                                      orth_smem(q.shape.bn), stream, *q.tm_a, *q.tm_b, *q.tm_c, g));
+  unsigned grid = g.num_tiles < static_cast<uint32_t>(plan.sms) ? g.num_tiles : plan.sms;
+  if (q.shape.split > 1) grid = g.num_tiles * q.shape.split;  // one cluster per tile
+  CCGLIB_CUDA_TRY(launch_programmatic(
+      orth_kernel(q.shape.bn, q.shape.split, q.a.by_rows, q.b.by_rows), grid, kThreads,
+      orth_smem(q.shape.bn), q.shape.split, stream, *q.tm_a, *q.tm_b, *q.tm_c, g));
   return CCGLIB_B200_OK;
 }
 
@@ -1101,8 +1315,9 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.wait_cycles = wait_limit_cycles();
   int rc = device_status_address(&plan.status);
   if (rc != CCGLIB_B200_OK) return rc;
-  plan.square = pick_shape(d.batch, plan.n, plan.n_p, true, plan.sms);
-  plan.update = pick_shape(d.batch, d.m, plan.cols_p, false, plan.sms);
+  plan.gram = pick_shape(d.batch, plan.n, plan.n_p, plan.l, true, plan.sms);
+  plan.poly = pick_shape(d.batch, plan.n, plan.n_p, plan.n, true, plan.sms);
+  plan.update = pick_shape(d.batch, d.m, plan.cols_p, plan.n, false, plan.sms);
   // One launch with a CTA per matrix, or three launches per step?  Estimates in microseconds per step,
   // within 40 % of what both forms take on short sides 1 .. 64, long sides to 1600, batches to 1024:
   // 33 x 70 x 64 51 against 106 for five steps, 64 x 64 150 against 95, 16 x 32 x 1024 92 against 211.
@@ -1113,7 +1328,7 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     const size_t sms = static_cast<size_t>(plan.sms);
     const double turns = static_cast<double>(ceil_div(d.batch, sms));
     const double one = turns * (1.5 + 4e-5 * macs);
-    const double waves = 2.0 * static_cast<double>(ceil_div(d.batch * plan.square.per_batch, sms)) +
+    const double waves = 2.0 * static_cast<double>(ceil_div(d.batch * plan.gram.per_batch, sms)) +
                          static_cast<double>(ceil_div(d.batch * plan.update.per_batch, sms));
     const double three = 3 * 4.8 + 2.5 * (waves - 3.0);
     plan.small = one < three;
@@ -1132,16 +1347,16 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     }
     return CCGLIB_B200_OK;
   }
-  if (d.batch * plan.square.per_batch > 0x7FFFFFFFull ||
+  if (d.batch * plan.gram.per_batch > 0x7FFFFFFFull ||
       d.batch * plan.update.per_batch > 0x7FFFFFFFull) {
     set_last_error("orthogonalize_plan_create: too many tiles");
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
-  for (int bn : {64, 128}) {
+  for (const ProductShape &shape : {plan.gram, plan.poly, plan.update}) {
     for (int form = 0; form < 3; ++form) {
       CCGLIB_CUDA_TRY(cudaFuncSetAttribute(
-          reinterpret_cast<const void *>(orth_kernel(bn, form == 2, form >= 1)),
-          cudaFuncAttributeMaxDynamicSharedMemorySize, orth_smem(bn)));
+          reinterpret_cast<const void *>(orth_kernel(shape.bn, shape.split, form == 2, form >= 1)),
+          cudaFuncAttributeMaxDynamicSharedMemorySize, orth_smem(shape.bn)));
     }
   }
   plan.chunks = ceil_div<size_t>(2 * d.m * d.n, kNormChunk);
@@ -1235,10 +1450,10 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
     const Operand x_long = x_operand(*plan, now, true), x_short = x_operand(*plan, now, false);
     const Operand s = square_operand(*plan, plan->s), p = square_operand(*plan, plan->p);
     rc = launch_product(*plan, {x_long, x_long, &plan->gram_a[now], &plan->gram_b[now], &plan->s_out, n, n_p,
-                                plan->square, true, true, unscale, 0.0f, 1.0f, nullptr, 0, plan->s, n_p,
+                                plan->gram, true, true, unscale, 0.0f, 1.0f, nullptr, 0, plan->s, n_p,
                                 true, false}, stream);
     if (rc != CCGLIB_B200_OK) break;
-    rc = launch_product(*plan, {s, s, &plan->s_a, &plan->s_b, &plan->p_out, n, n_p, plan->square, true, true,
+    rc = launch_product(*plan, {s, s, &plan->s_a, &plan->s_b, &plan->p_out, n, n_p, plan->poly, true, true,
                                 d.c, d.b, 1.0f, plan->s, n_p, plan->p, n_p, true, false}, stream);
     if (rc != CCGLIB_B200_OK) break;
     const CUtensorMap *tm_x = &plan->update_x[now], *tm_p = &plan->update_p;

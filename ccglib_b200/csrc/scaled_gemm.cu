@@ -1013,7 +1013,7 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
                       : plan->tiles < static_cast<size_t>(plan->sms) ? plan->tiles
                                                                      : plan->sms;
   CCGLIB_CUDA_TRY(launch_programmatic(plan->kernel.fn, static_cast<unsigned>(ctas), plan->kernel.threads,
-                                      plan->kernel.smem, static_cast<cudaStream_t>(stream_v), tm_a, tm_b,
+                                      plan->kernel.smem, 1, static_cast<cudaStream_t>(stream_v), tm_a, tm_b,
                                       tm_c, p));
   return CCGLIB_B200_OK;
 }
