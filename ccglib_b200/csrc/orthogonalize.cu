@@ -859,17 +859,21 @@ void launch_first_form(const FirstParams &p, bool il, bool vec, unsigned grid, c
   }
 }
 
-// ---- small matrices: the whole iteration in one CTA ------------------------------------------------
+// ---- small matrices: the whole iteration in one launch ---------------------------------------------
 //
-// X (twice), S and P in shared memory, float32 throughout, one launch: for matrices whose products are
-// too small for 128-row tiles and a launch each.  X is kept transposed, V[l][i]: with S and P
-// Hermitian, every product then reads rows of four consecutive values,
+// X, S and P in shared memory, float32 throughout: for matrices whose products are too small for
+// 128-row tiles and a launch each.  X is kept transposed, V[l][i]: with S and P Hermitian, every product
+// then reads rows of neighbouring values,
 //   S_ij = sum_l V[l][i] conj(V[l][j]),  (S S)_ij = sum_k conj(S[k][i]) S[k][j],
 //   V'[l][i] = a V[l][i] + sum_j conj(P[j][i]) V[l][j].
+// A cluster of up to eight CTAs shares a matrix by rows of V where one CTA cannot hold it or SMs would
+// stay idle: each adds up its rows' share of S, the shares go to all through distributed shared memory
+// and are added in the order of the CTAs, and P is computed by each for itself.
 
 constexpr int kSmallThreads = 512;
 constexpr int kSmallRows = 2;  // rows of V' per thread in the update
 constexpr size_t kSmallMaxSide = 64;
+constexpr uint32_t kSmallMaxParts = 8;
 constexpr int kSmallSmem = kMaxSmem - 2048;  // dynamic; the rest is static
 
 struct SmallParams {
@@ -877,14 +881,16 @@ struct SmallParams {
   void *out;
   size_t batch, m, n;  // as the caller holds them
   uint32_t s, l, sp;   // short and long side, short side rounded up to four
+  uint32_t parts;      // CTAs per matrix (the cluster)
   bool tall;
   int type_in, bf16, inter, steps;
   float a, b, c;
 };
 
-size_t small_smem(size_t s, size_t l) {
+// V's share, S, P, and the others' shares of S (twice: one set is read while the next may arrive).
+size_t small_smem(size_t s, size_t l, size_t parts) {
   const size_t sp = ceil_div<size_t>(s, 4) * 4;
-  return (2 * 2 * l * sp + 2 * 2 * sp * sp) * sizeof(float);
+  return (2 * ceil_div(l, parts) * sp + 2 * 2 * sp * sp + 2 * (parts - 1) * 2 * sp * sp) * sizeof(float);
 }
 
 // Four rows' worth of complex values.
@@ -966,31 +972,42 @@ __device__ __forceinline__ uint32_t lanes_for(uint32_t pairs, uint32_t rows) {
   return lanes;
 }
 
+__device__ __forceinline__ void st_shared_cluster_f64(uint32_t addr_cluster, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr_cluster), "d"(v) : "memory");
+}
+
 __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams p) {
   extern __shared__ __align__(16) float small_smem_raw[];
   __shared__ double part[kSmallThreads / 32];
+  __shared__ double squares[kSmallMaxParts];  // sums of squares of the cluster's CTAs
   // the 2 x 2 blocks on and above the diagonal, row by row: (row << 8) + column
   __shared__ uint16_t blocks[(kSmallMaxSide / 2) * (kSmallMaxSide / 2 + 1) / 2];
-  const uint32_t sp = p.sp, l = p.l;
-  const uint32_t x_size = l * sp;
-  float *x0 = small_smem_raw, *x1 = x0 + 2 * x_size;  // Re, Im of V, twice
-  float *at = x1 + 2 * x_size;
-  float *s_re = at, *s_im = at + sp * sp, *p_re = at + 2 * sp * sp, *p_im = at + 3 * sp * sp;
+  const uint32_t parts = p.parts, rank = parts > 1 ? cluster_ctarank() : 0;
+  // this CTA's rows of V
+  const uint32_t l_first = static_cast<uint32_t>(static_cast<uint64_t>(p.l) * rank / parts);
+  const uint32_t sp = p.sp, l = static_cast<uint32_t>(static_cast<uint64_t>(p.l) * (rank + 1) / parts) - l_first;
+  const uint32_t square = sp * sp;
+  float *x_re = small_smem_raw, *x_im = x_re + l * sp;
+  float *s_re = small_smem_raw + 2 * ceil_div(p.l, parts) * sp, *s_im = s_re + square;
+  float *p_re = s_im + square, *p_im = p_re + square;
+  float *others = p_im + square;  // [2][parts - 1][2][sp][sp]
   const uint32_t nb = sp / 4, pairs = (sp / 2) * (sp / 2 + 1) / 2;
   const uint32_t lanes_l = lanes_for(pairs, l), lanes_s = lanes_for(pairs, sp);
   for (uint32_t i = threadIdx.x; i < sp / 2; i += kSmallThreads) {
     uint32_t at_block = i * (sp / 2) - i * (i - 1) / 2;
     for (uint32_t j = i; j < sp / 2; ++j) blocks[at_block++] = static_cast<uint16_t>(i << 8 | j);
   }
-  // the update deals (row group, column group) pairs to the threads: this thread's first and the stride
-  const uint32_t row_0 = threadIdx.x / nb, col_0 = threadIdx.x % nb;
-  const uint32_t row_step = kSmallThreads / nb, col_step = kSmallThreads % nb;
+  // the update deals (row group, column group) pairs to the threads, whole row groups at a time
+  const uint32_t groups = kSmallThreads / nb, row_0 = threadIdx.x / nb, i0 = threadIdx.x % nb * 4;
   const size_t plane = p.m * p.n;
-  for (size_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
+  uint32_t turn = 0;  // which set of shares the next exchange uses
+  __syncwarp();
+  if (parts > 1) cluster_sync();  // the others have started
+  for (size_t b = blockIdx.x / parts; b < p.batch; b += gridDim.x / parts) {
     // X and its norm (float64: no input overflows or vanishes in it)
     double sum = 0.0;
     for (uint32_t i = threadIdx.x; i < l * sp; i += kSmallThreads) {
-      const uint32_t row = i / sp, col = i - row * sp;  // V[row][col]
+      const uint32_t r = i / sp, col = i - r * sp, row = l_first + r;  // V[row][col]
       float re = 0.0f, im = 0.0f;
       if (col < p.s) {
         const size_t e = p.tall ? static_cast<size_t>(row) * p.n + col : static_cast<size_t>(col) * p.n + row;
@@ -998,8 +1015,8 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
         re = load_value(p.in, base + (p.inter ? 2 * e : e), p.type_in);
         im = load_value(p.in, base + (p.inter ? 2 * e + 1 : e + plane), p.type_in);
       }
-      x0[i] = re;
-      x0[i + x_size] = im;
+      x_re[i] = re;
+      x_im[i] = im;
       sum += static_cast<double>(re) * re + static_cast<double>(im) * im;
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -1007,16 +1024,23 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < kSmallThreads / 32; ++w) sum += part[w];
+    if (parts > 1) {
+      if (threadIdx.x < parts) {
+        st_shared_cluster_f64(map_to_cta(smem_u32(&squares[rank]), threadIdx.x), sum);
+      }
+      __syncwarp();
+      cluster_sync();
+      sum = 0.0;
+      for (uint32_t i = 0; i < parts; ++i) sum += squares[i];
+    }
     const double factor = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
     for (uint32_t i = threadIdx.x; i < l * sp; i += kSmallThreads) {
-      x0[i] = static_cast<float>(x0[i] * factor);
-      x0[i + x_size] = static_cast<float>(x0[i + x_size] * factor);
+      x_re[i] = static_cast<float>(x_re[i] * factor);
+      x_im[i] = static_cast<float>(x_im[i] * factor);
     }
     __syncthreads();
     for (int step = 0; step < p.steps; ++step) {
-      const float *xr = (step & 1) ? x1 : x0, *xi = xr + x_size;
-      float *yr = (step & 1) ? x0 : x1, *yi = yr + x_size;
-      gram_blocks(xr, xi, l, sp, lanes_l, blocks, [&](uint32_t i, uint32_t j, float re, float im) {
+      gram_blocks(x_re, x_im, l, sp, lanes_l, blocks, [&](uint32_t i, uint32_t j, float re, float im) {
         // S_ij = conj(H_ij)
         const uint32_t ij = i * sp + j, ji = j * sp + i;
         im = i == j ? 0.0f : im;
@@ -1026,6 +1050,31 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
         s_im[ji] = im;
       });
       __syncthreads();
+      if (parts > 1) {
+        // A share goes to place `rank` (less one behind the receiver's own) of the set of this turn.  The
+        // set is free: whoever read it last turn but one has been at last turn's barrier since.
+        float *set = others + static_cast<size_t>(turn) * (parts - 1) * 2 * square;
+        for (uint32_t peer = 0; peer < parts; ++peer) {
+          if (peer == rank) continue;
+          const uint32_t to = map_to_cta(smem_u32(set + (rank - (rank > peer ? 1 : 0)) * 2 * square), peer);
+          for (uint32_t i = threadIdx.x * 4; i < 2 * square; i += kSmallThreads * 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(s_re + i);
+            st_shared_cluster_v4(to + i * 4, __float_as_uint(v.x), __float_as_uint(v.y),
+                                 __float_as_uint(v.z), __float_as_uint(v.w));
+          }
+        }
+        __syncwarp();
+        cluster_sync();
+        for (uint32_t i = threadIdx.x; i < 2 * square; i += kSmallThreads) {
+          float all = 0.0f;
+          for (uint32_t r = 0; r < parts; ++r) {
+            all += r == rank ? s_re[i] : set[(r - (r > rank ? 1 : 0)) * 2 * square + i];
+          }
+          s_re[i] = all;
+        }
+        turn ^= 1;
+        __syncthreads();
+      }
       gram_blocks(s_re, s_im, sp, sp, lanes_s, blocks, [&](uint32_t i, uint32_t j, float re, float im) {
         const uint32_t ij = i * sp + j, ji = j * sp + i;
         re = p.b * s_re[ij] + p.c * re;
@@ -1036,66 +1085,73 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
         p_im[ji] = -im;
       });
       __syncthreads();
-      // kSmallRows rows of V' x four columns
+      // kSmallRows rows of V' x four columns per thread; a pass reads its rows before any is written
       const uint32_t lb = ceil_div<uint32_t>(l, kSmallRows);
-      for (uint32_t row = row_0, col = col_0; row < lb;) {
-        const uint32_t i0 = col * 4, l0 = row * kSmallRows;
-        row += row_step;
-        col += col_step;
-        if (col >= nb) {
-          col -= nb;
-          ++row;
-        }
+      for (uint32_t first = 0; first < lb; first += groups) {
+        const uint32_t l0 = (first + row_0) * kSmallRows;
+        const bool on = row_0 < groups && l0 < l;
         float vr[kSmallRows][4], vi[kSmallRows][4];
-#pragma unroll
-        for (int r = 0; r < kSmallRows; ++r) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vr[r][i] = vi[r][i] = 0.0f;
-        }
-#pragma unroll 1
-        for (uint32_t j = 0; j < sp; j += 4) {
-          Quad x[kSmallRows];
+        if (on) {
 #pragma unroll
           for (int r = 0; r < kSmallRows; ++r) {
-            const uint32_t from = min(l0 + r, l - 1) * sp + j;
-            x[r] = load_quad(xr + from, xi + from);
-          }
+            const uint32_t at = min(l0 + r, l - 1) * sp + i0;
+            const Quad q = load_quad(x_re + at, x_im + at);
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            const Quad q = load_quad(p_re + (j + jj) * sp + i0, p_im + (j + jj) * sp + i0);
+            for (int i = 0; i < 4; ++i) {
+              vr[r][i] = p.a * q.re[i];
+              vi[r][i] = p.a * q.im[i];
+            }
+          }
+#pragma unroll 1
+          for (uint32_t j = 0; j < sp; j += 4) {
+            Quad x[kSmallRows];
 #pragma unroll
             for (int r = 0; r < kSmallRows; ++r) {
-              const float cr = x[r].re[jj], ci = x[r].im[jj];
+              const uint32_t from = min(l0 + r, l - 1) * sp + j;
+              x[r] = load_quad(x_re + from, x_im + from);
+            }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                vr[r][i] = fmaf(q.re[i], cr, fmaf(q.im[i], ci, vr[r][i]));
-                vi[r][i] = fmaf(q.re[i], ci, fmaf(-q.im[i], cr, vi[r][i]));
+            for (int jj = 0; jj < 4; ++jj) {
+              const Quad q = load_quad(p_re + (j + jj) * sp + i0, p_im + (j + jj) * sp + i0);
+#pragma unroll
+              for (int r = 0; r < kSmallRows; ++r) {
+                const float cr = x[r].re[jj], ci = x[r].im[jj];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  vr[r][i] = fmaf(q.re[i], cr, fmaf(q.im[i], ci, vr[r][i]));
+                  vi[r][i] = fmaf(q.re[i], ci, fmaf(-q.im[i], cr, vi[r][i]));
+                }
               }
             }
           }
         }
+        __syncthreads();
+        if (on) {
 #pragma unroll
-        for (int r = 0; r < kSmallRows; ++r) {
-          if (l0 + r < l) {
-            Quad q = load_quad(xr + (l0 + r) * sp + i0, xi + (l0 + r) * sp + i0);
+          for (int r = 0; r < kSmallRows; ++r) {
+            if (l0 + r < l) {
+              Quad q;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              q.re[i] = fmaf(p.a, q.re[i], vr[r][i]);
-              q.im[i] = fmaf(p.a, q.im[i], vi[r][i]);
+              for (int i = 0; i < 4; ++i) {
+                q.re[i] = vr[r][i];
+                q.im[i] = vi[r][i];
+              }
+              store_quad(x_re + (l0 + r) * sp + i0, x_im + (l0 + r) * sp + i0, q);
             }
-            store_quad(yr + (l0 + r) * sp + i0, yi + (l0 + r) * sp + i0, q);
           }
         }
       }
       __syncthreads();
     }
-    const float *xr = (p.steps & 1) ? x1 : x0, *xi = xr + x_size;
+    // every CTA of the cluster has read the input: d_out may be d_in
     uint16_t *out = static_cast<uint16_t *>(p.out) + b * 2 * plane;
-    for (uint32_t e = threadIdx.x; e < plane; e += kSmallThreads) {
-      const uint32_t row = e / static_cast<uint32_t>(p.n), col = e - row * static_cast<uint32_t>(p.n);
-      const uint32_t i = p.tall ? row * sp + col : col * sp + row;
-      out[e] = round_half(xr[i], p.bf16);
-      out[e + plane] = round_half(xi[i], p.bf16);
+    for (uint32_t e = threadIdx.x; e < l * p.s; e += kSmallThreads) {
+      // along the rows of the output
+      const uint32_t row = p.tall ? e / p.s : e % l, col = p.tall ? e - row * p.s : e / l;  // V[row][col]
+      const size_t to = p.tall ? static_cast<size_t>(l_first + row) * p.n + col
+                               : static_cast<size_t>(col) * p.n + l_first + row;
+      out[to] = round_half(x_re[row * sp + col], p.bf16);
+      out[to + plane] = round_half(x_im[row * sp + col], p.bf16);
     }
     __syncthreads();
   }
@@ -1113,7 +1169,7 @@ struct ccglib_b200_orthogonalize_plan {
   bool tall;            // m > n
   float scale;          // power of two near sqrt(long side)
   ProductShape gram, poly, update;
-  bool small;           // the whole iteration in one launch, a CTA per matrix
+  uint32_t small;       // > 0: the whole iteration in one launch, so many CTAs per matrix
   size_t chunks;
   int device, sms;
   long long wait_cycles;
@@ -1318,23 +1374,31 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.gram = pick_shape(d.batch, plan.n, plan.n_p, plan.l, true, plan.sms);
   plan.poly = pick_shape(d.batch, plan.n, plan.n_p, plan.n, true, plan.sms);
   plan.update = pick_shape(d.batch, d.m, plan.cols_p, plan.n, false, plan.sms);
-  // One launch with a CTA per matrix, or three launches per step?  Estimates in microseconds per step,
-  // within 40 % of what both forms take on short sides 1 .. 64, long sides to 1600, batches to 1024:
-  // 33 x 70 x 64 51 against 106 for five steps, 64 x 64 150 against 95, 16 x 32 x 1024 92 against 211.
-  plan.small = plan.n <= kSmallMaxSide && small_smem(plan.n, plan.l) <= static_cast<size_t>(kSmallSmem);
-  if (plan.small) {
+  // One launch (with how many CTAs per matrix), or three launches per step?  Estimates in microseconds
+  // per step, within 40 % of what the forms take on short sides 1 .. 64, long sides to 1600, batches to
+  // 1024: 64 x 64 x 64 150 us in one launch against 95 for five steps, 16 x 32 x 1024 92 against 211.
+  const size_t sms = static_cast<size_t>(plan.sms);
+  const double waves = static_cast<double>(ceil_div(d.batch * plan.gram.per_batch, sms)) +
+                       static_cast<double>(ceil_div(d.batch * plan.poly.per_batch, sms)) +
+                       static_cast<double>(ceil_div(d.batch * plan.update.per_batch, sms));
+  double least = 3 * 4.8 + 2.5 * (waves - 3.0);
+  // CCGLIB_B200_ORTH_SMALL: 0 for three launches, 1, 2, 4 or 8 for one with so many CTAs (where it fits)
+  const char *env = std::getenv("CCGLIB_B200_ORTH_SMALL");
+  const int forced = env != nullptr && *env != '\0' ? std::atoi(env) : -1;
+  for (uint32_t parts = 1; parts <= kSmallMaxParts && plan.n <= kSmallMaxSide; parts *= 2) {
+    if (small_smem(plan.n, plan.l, parts) > static_cast<size_t>(kSmallSmem) || parts > plan.l) continue;
     const double side = static_cast<double>(ceil_div<size_t>(plan.n, 4) * 4);
-    const double macs = side * side * (2.0 * static_cast<double>(plan.l) + side);
-    const size_t sms = static_cast<size_t>(plan.sms);
-    const double turns = static_cast<double>(ceil_div(d.batch, sms));
-    const double one = turns * (1.5 + 4e-5 * macs);
-    const double waves = 2.0 * static_cast<double>(ceil_div(d.batch * plan.gram.per_batch, sms)) +
-                         static_cast<double>(ceil_div(d.batch * plan.update.per_batch, sms));
-    const double three = 3 * 4.8 + 2.5 * (waves - 3.0);
-    plan.small = one < three;
-    // CCGLIB_B200_ORTH_SMALL = 0 or 1 chooses by hand (where the matrices fit)
-    const char *v = std::getenv("CCGLIB_B200_ORTH_SMALL");
-    if (v != nullptr && *v != '\0') plan.small = std::atoi(v) != 0;
+    const double macs = side * side * (2.0 * static_cast<double>(plan.l) / parts + side);
+    // (clusters of four and eight leave some SMs of a processor group over)
+    const size_t room = parts >= 4 ? sms * 86 / 100 : sms;
+    const double turns = static_cast<double>(ceil_div(d.batch * parts, room));
+    const double exchange = parts > 1 ? 0.5 + 0.1 * parts + 5e-4 * (parts - 1) * side * side : 0.0;
+    double cost = turns * (1.5 + 4e-5 * macs + exchange);
+    if (forced >= 0) cost = static_cast<int>(parts) == forced ? -1.0 : 1e30;
+    if (cost < least) {
+      least = cost;
+      plan.small = parts;
+    }
   }
   if (plan.small) {
     CCGLIB_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void *>(small_kernel),
@@ -1432,10 +1496,21 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
     q.a = d.a;
     q.b = d.b;
     q.c = d.c;
+    q.parts = plan->small;
     const size_t cap = static_cast<size_t>(plan->sms) * 8;
-    small_kernel<<<static_cast<unsigned>(d.batch < cap ? d.batch : cap), kSmallThreads,
-                   small_smem(plan->n, plan->l), stream>>>(q);
-    CCGLIB_CUDA_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((d.batch < cap ? d.batch : cap) * plan->small));
+    cfg.blockDim = dim3(kSmallThreads);
+    cfg.dynamicSmemBytes = small_smem(plan->n, plan->l, plan->small);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = plan->small;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = plan->small > 1 ? 1 : 0;
+    CCGLIB_CUDA_TRY(cudaLaunchKernelEx(&cfg, small_kernel, q));
     return CCGLIB_B200_OK;
   }
   int rc = d.type_in == CCGLIB_B200_FLOAT32   ? launch_first<float>(*plan, d_in, stream)

@@ -122,6 +122,32 @@ def test_shapes(batch, m, n, steps, coefficients):
     _check(x, _run(plan, x, F32, F16, capi.PLANAR), steps, coefficients, F16)
 
 
+@pytest.mark.parametrize("form", ["0", "1", "2", "4", "8"])
+def test_every_form_of_small_matrices(form, monkeypatch):
+    """Three launches per step, or one with 1 .. 8 CTAs per matrix (the plan's choice by hand)."""
+    rng = np.random.default_rng(18)
+    monkeypatch.setenv("CCGLIB_B200_ORTH_SMALL", form)
+    for batch, m, n in ((3, 4, 8), (2, 9, 200), (5, 200, 33), (2, 31, 90), (300, 8, 12), (2, 3, 5000)):
+        x = _input(rng, batch, m, n, F16)
+        plan = capi.OrthogonalizePlan(batch, m, n, F16, F16, 4, QUINTIC)
+        got = _run(plan, x, F16, F16, capi.PLANAR)
+        _check(x[-3:], got[-3:], 4, QUINTIC, F16)
+        import torch
+
+        assert torch.equal(_run(plan, x, F16, F16, capi.PLANAR, in_place=True), got)
+
+
+@pytest.mark.parametrize("split", ["1", "2", "4"])
+def test_every_split_of_large_matrices(split, monkeypatch):
+    """CTAs that share the K of a tile (the plan's choice by hand)."""
+    rng = np.random.default_rng(19)
+    monkeypatch.setenv("CCGLIB_B200_ORTH_SPLIT", split)
+    for batch, m, n in ((1, 150, 600), (1, 600, 150), (2, 260, 260)):
+        x = _input(rng, batch, m, n, BF16)
+        plan = capi.OrthogonalizePlan(batch, m, n, BF16, BF16, 3, QUINTIC)
+        _check(x, _run(plan, x, BF16, BF16, capi.PLANAR), 3, QUINTIC, BF16)
+
+
 @pytest.mark.parametrize("type_out", [F16, BF16])
 @pytest.mark.parametrize("axis", [capi.PLANAR, capi.INTERLEAVED])
 @pytest.mark.parametrize("type_in", [F16, BF16, F32])
