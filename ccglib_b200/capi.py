@@ -63,7 +63,7 @@ class QuantizeDesc(ctypes.Structure):
     _fields_ = [("batch", ctypes.c_size_t), ("rows", ctypes.c_size_t), ("k", ctypes.c_size_t),
                 ("type_in", ctypes.c_int), ("type_out", ctypes.c_int),
                 ("input_complex_axis", ctypes.c_int), ("input_mem_order", ctypes.c_int),
-                ("block_rows", ctypes.c_size_t)]
+                ("block_rows", ctypes.c_size_t), ("conjugate", ctypes.c_int)]
 
 
 class ScaledGemmDesc(ctypes.Structure):
@@ -420,12 +420,13 @@ def pack(n, direction, input_complex_axis, d_in, d_out, stream: int = 0) -> None
 
 
 def quantize(batch, rows, k, type_in, type_out, d_in, d_out, d_scale, stream: int = 0,
-             input_complex_axis=PLANAR, input_mem_order=ROW_MAJOR, block_rows=1) -> None:
+             input_complex_axis=PLANAR, input_mem_order=ROW_MAJOR, block_rows=1,
+             conjugate=False) -> None:
     """Complex float matrices -> fp8 planes [batch][2][rows][pitch] and block scales
     [batch][ceil(k / 128)][ceil(rows / block_rows)] (see include/ccglib_b200.h)."""
     status = lib().ccglib_b200_quantize_run(
         _quantize_desc(batch, rows, k, type_in, type_out, input_complex_axis, input_mem_order,
-                       block_rows), d_in, d_out, d_scale, stream)
+                       block_rows, int(conjugate)), d_in, d_out, d_scale, stream)
     if status != OK:
         _check(status)
 

@@ -1412,6 +1412,7 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     return CCGLIB_B200_OK;
   }
   if (d.batch * plan.gram.per_batch > 0x7FFFFFFFull ||
+      d.batch * plan.poly.per_batch > 0x7FFFFFFFull ||
       d.batch * plan.update.per_batch > 0x7FFFFFFFull) {
     set_last_error("orthogonalize_plan_create: too many tiles");
     return CCGLIB_B200_INVALID_ARGUMENT;

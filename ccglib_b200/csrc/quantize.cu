@@ -32,6 +32,7 @@ struct QuantizeParams {
   float *scale;   // [batch][blocks_k][blocks_rows]
   size_t batch, rows, k, pitch;
   size_t blocks_k, blocks_rows;
+  float im_sign;  // -1: the conjugate is written
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -211,7 +212,7 @@ quantize_rows_kernel(const QuantizeParams p) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const float s = block_scale<E5M2>(top[i]);
-      const float inv = __fdiv_rn(1.0f, s);
+      const float inv = __fdiv_rn(1.0f, s), inv_im = p.im_sign * inv;
       if constexpr (kTile) {
         if (i == 0 && threadIdx.x == 0) scale_row[group] = s;
       } else {
@@ -223,7 +224,7 @@ quantize_rows_kernel(const QuantizeParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           a[j] = re[i][j] * inv;
-          c[j] = im[i][j] * inv;
+          c[j] = im[i][j] * inv_im;
         }
         uint8_t *dst = p.out + ((b * 2) * p.rows + r) * p.pitch + k0;
         uint32_t w_re = pack4<E5M2>(a), w_im = pack4<E5M2>(c);
@@ -374,7 +375,7 @@ quantize_cols_kernel(const QuantizeParams p) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float inv = TILE ? inv_tile : row_inv[32 * j + lane];
+      const float inv = TILE ? inv_tile : row_inv[32 * j + lane], inv_im = p.im_sign * inv;
       const uint32_t at = (32 * j + lane) * kColPitch + warp * kColK;
       uint32_t w[4];
 #pragma unroll
@@ -384,7 +385,7 @@ quantize_cols_kernel(const QuantizeParams p) {
         for (int i = 0; i < 4; ++i) {
           const float2 v = x[j][4 * h + i].value();
           a[i] = v.x * inv;
-          c[i] = v.y * inv;
+          c[i] = v.y * inv_im;
         }
         w[h] = pack4<E5M2>(a);
         w[2 + h] = pack4<E5M2>(c);
@@ -501,6 +502,10 @@ extern "C" int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *desc, c
                    d.input_complex_axis, d.input_mem_order);
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
+  if (d.conjugate != 0 && d.conjugate != 1) {
+    set_last_error("quantize_run: conjugate must be 0 or 1 (got %d)", d.conjugate);
+    return CCGLIB_B200_INVALID_ARGUMENT;
+  }
   if (!aligned16(d_in) || !aligned16(d_out) || (reinterpret_cast<uintptr_t>(d_scale) & 3u) != 0) {
     set_last_error("quantize_run: input and output must be 16-byte aligned, scales 4-byte aligned");
     return CCGLIB_B200_INVALID_ARGUMENT;
@@ -516,6 +521,7 @@ extern "C" int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *desc, c
   p.pitch = ceil_div<size_t>(d.k, 16) * 16;
   p.blocks_k = ceil_div<size_t>(d.k, kBlockK);
   p.blocks_rows = ceil_div<size_t>(d.rows, d.block_rows);
+  p.im_sign = d.conjugate ? -1.0f : 1.0f;
   const bool il = d.input_complex_axis == CCGLIB_B200_INTERLEAVED;
   const bool e5m2 = d.type_out == CCGLIB_B200_FLOAT8E5M2;
   const bool col = d.input_mem_order == CCGLIB_B200_COL_MAJOR;

@@ -294,9 +294,10 @@ public:
   Quantize(size_t B, size_t rows, size_t K, CUdevice &device, CUstream &stream,
            ValuePrecision input_precision, ValuePrecision output_precision, size_t block_rows = 1,
            ComplexAxisLocation input_complex_axis_location = ComplexAxisLocation::complex_planar,
-           mma::MemOrder input_mem_order = mma::MemOrder::row_major)
+           mma::MemOrder input_mem_order = mma::MemOrder::row_major,
+           bool conjugate = false)
       : Quantize(FromHandles{}, B, rows, K, device, stream, input_precision, output_precision,
-                 block_rows, input_complex_axis_location, input_mem_order) {}
+                 block_rows, input_complex_axis_location, input_mem_order, conjugate) {}
 
   // Asynchronous on the stream given at construction; no allocation, no synchronisation.
   void Run(CUdeviceptr d_input, CUdeviceptr d_output, CUdeviceptr d_scale) {
@@ -318,10 +319,11 @@ public:
   Quantize(size_t B, size_t rows, size_t K, cu::Device &device, cu::Stream &stream,
            ValuePrecision input_precision, ValuePrecision output_precision, size_t block_rows = 1,
            ComplexAxisLocation input_complex_axis_location = ComplexAxisLocation::complex_planar,
-           mma::MemOrder input_mem_order = mma::MemOrder::row_major)
+           mma::MemOrder input_mem_order = mma::MemOrder::row_major,
+           bool conjugate = false)
       : Quantize(FromHandles{}, B, rows, K, static_cast<CUdevice>(device),
                  static_cast<CUstream>(stream), input_precision, output_precision, block_rows,
-                 input_complex_axis_location, input_mem_order) {}
+                 input_complex_axis_location, input_mem_order, conjugate) {}
   void Run(cu::DeviceMemory &d_input, cu::DeviceMemory &d_output, cu::DeviceMemory &d_scale) {
     Run(static_cast<CUdeviceptr>(d_input), static_cast<CUdeviceptr>(d_output),
         static_cast<CUdeviceptr>(d_scale));
@@ -332,7 +334,7 @@ private:
   struct FromHandles {};
   Quantize(FromHandles, size_t B, size_t rows, size_t K, CUdevice device, CUstream stream,
            ValuePrecision in, ValuePrecision out, size_t block_rows, ComplexAxisLocation axis,
-           mma::MemOrder order)
+           mma::MemOrder order, bool conjugate)
       : stream_(stream) {
     (void)device;
     if (block_rows != 1 && block_rows != 128) {
@@ -346,6 +348,7 @@ private:
     desc_.input_complex_axis = axis;
     desc_.input_mem_order = order;
     desc_.block_rows = block_rows;
+    desc_.conjugate = conjugate ? 1 : 0;
   }
 
   ccglib_b200_quantize_desc desc_{};

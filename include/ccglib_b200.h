@@ -170,6 +170,10 @@ CCGLIB_B200_API int ccglib_b200_pack_run(size_t n, int direction, int input_comp
  *   q = x * (1 / scale) rounded to nearest even, FMAX = 448 (e4m3) or 57344 (e5m2),
  * in float32.  NaN stays NaN; an infinity becomes an infinity in e5m2 and NaN in e4m3.
  * Asynchronous on `stream`, one launch, no scratch.
+ *
+ * The products of a backward pass of C = A x B^T are products of the same kind, over operands quantised
+ * along their other axis: dA = dC x conj(B) contracts over n (rows = K of the col-major, conjugated B),
+ * dB = dC^T x conj(A) over m (col-major dC and col-major, conjugated A); dC is commonly e5m2.
  */
 typedef struct ccglib_b200_quantize_desc {
   size_t batch;
@@ -180,6 +184,7 @@ typedef struct ccglib_b200_quantize_desc {
   int input_complex_axis; /* CCGLIB_B200_PLANAR / CCGLIB_B200_INTERLEAVED */
   int input_mem_order;    /* CCGLIB_B200_ROW_MAJOR (k contiguous) / CCGLIB_B200_COL_MAJOR */
   size_t block_rows;      /* 1 or 128 */
+  int conjugate;          /* 1: the conjugate is written, e.g. for A x B^H or a gradient */
 } ccglib_b200_quantize_desc;
 
 CCGLIB_B200_API int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *desc, const void *d_in,

@@ -23,6 +23,7 @@ def _status(call, *args, **kw):
     ((1, 1, 1, F16, E4M3, 256, 512, 768), {"block_rows": 64}, capi.INVALID_ARGUMENT, "1 or 128 rows"),
     ((1, 1, 1, F16, E4M3, 256, 512, 768), {"input_complex_axis": 2}, capi.INVALID_ARGUMENT, "axis"),
     ((1, 1, 1, F16, E4M3, 256, 512, 768), {"input_mem_order": 2}, capi.INVALID_ARGUMENT, "order"),
+    ((1, 1, 1, F16, E4M3, 256, 512, 768), {"conjugate": 2}, capi.INVALID_ARGUMENT, "conjugate"),
     ((1, 1, 1, F16, E4M3, 0, 512, 768), {}, capi.INVALID_ARGUMENT, "null"),
     ((1, 1, 1, F16, E4M3, 256, 0, 768), {}, capi.INVALID_ARGUMENT, "null"),
     ((1, 1, 1, F16, E4M3, 256, 512, 0), {}, capi.INVALID_ARGUMENT, "null"),

@@ -223,6 +223,23 @@ def test_same_bits_in_place_on_a_side_stream_and_from_a_graph():
             assert torch.equal(out, first)
 
 
+def test_buffers_aligned_to_their_elements_only():
+    import torch
+
+    rng = np.random.default_rng(22)
+    for m, n in ((40, 72), (200, 136)):
+        x = _input(rng, 1, m, n, F16)
+        plan = capi.OrthogonalizePlan(1, m, n, F16, F16, 3)
+        want = _run(plan, x, F16, F16, capi.PLANAR)
+        d_in = torch.zeros(2 * m * n + 8, dtype=torch.float16, device="cuda")
+        out = torch.zeros(2 * m * n + 8, dtype=torch.float16, device="cuda")
+        d_in[1:1 + 2 * m * n] = x.cuda().reshape(-1)
+        plan.run(d_in.data_ptr() + 2, out.data_ptr() + 2, gu.stream_handle())
+        torch.cuda.synchronize()
+        assert torch.equal(out[1:1 + 2 * m * n].view(want.shape), want)
+        assert out[0] == 0 and not out[1 + 2 * m * n:].any()
+
+
 def test_weights_orthogonalised_quantised_and_multiplied():
     """The operators as they are used together: an orthonormal set of weights, quantised with one
     scale per 128 x 128 block, applied to samples quantised with one scale per row and block."""

@@ -109,6 +109,28 @@ def test_ties_round_to_even():
         _check(x, code, 1, got, scale)
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("order", [capi.ROW_MAJOR, capi.COL_MAJOR])
+def test_conjugate_is_the_same_with_the_other_sign(order, block_rows):
+    import torch
+
+    rng = np.random.default_rng(20)
+    batch, rows, k = 2, 70, 300
+    x = _signal(rng, batch, rows, k, F32)
+    d_in = bu.lay_out(x, capi.PLANAR, order).cuda()
+    got = []
+    for conjugate in (False, True):
+        q = torch.empty((batch, 2, rows, capi.operand_pitch(k)), dtype=torch.uint8, device="cuda")
+        s = torch.empty((batch, 3, bu.ceil(rows, block_rows)), device="cuda")
+        capi.quantize(batch, rows, k, F32, E4M3, d_in.data_ptr(), q.data_ptr(), s.data_ptr(),
+                      gu.stream_handle(), input_mem_order=order, block_rows=block_rows,
+                      conjugate=conjugate)
+        got.append((q.view(torch.float8_e4m3fn).float(), s))
+    assert torch.equal(got[0][1], got[1][1])
+    assert torch.equal(got[0][0][:, 0], got[1][0][:, 0])
+    assert torch.equal(got[0][0][:, 1], -got[1][0][:, 1])
+
+
 def test_side_stream_and_replayed_graph():
     import torch
 

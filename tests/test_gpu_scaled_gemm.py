@@ -248,3 +248,60 @@ def test_quantise_and_multiply():
         assert (np.abs(got[:, i] - v) <= bound).all()
         rms = np.sqrt(np.mean((got[:, i] - v) ** 2) / np.mean(v ** 2))
         assert rms < 2 * 2.0 ** -4
+
+
+def test_backward_products():
+    """Gradients of a real loss L = Re sum conj(G) C of C = A B^T: dA = G conj(B), dB = G^T conj(A), from
+    the same two operators with the operands quantised along their other axis.  Against the formula in
+    64 bits on the dequantised operands, and the formula against differences of L."""
+    import torch
+
+    rng = np.random.default_rng(21)
+    m, n, k = 90, 140, 200
+    a, b = (torch.from_numpy(rng.standard_normal((1, 2, r, k))).float() for r in (m, n))
+    g = torch.from_numpy(rng.standard_normal((1, 2, m, n))).float()
+
+    def quantised(x, rows, kk, code, order, conjugate):
+        """-> (tensors for the GEMM, complex values [rows][kk] that they stand for)"""
+        d_in = x.cuda()
+        q = torch.empty((1, 2, rows, capi.operand_pitch(kk)), dtype=torch.uint8, device="cuda")
+        s = torch.empty((1, bu.ceil(kk, 128), rows), device="cuda")
+        capi.quantize(1, rows, kk, F32, code, d_in.data_ptr(), q.data_ptr(), s.data_ptr(),
+                      gu.stream_handle(), input_mem_order=order, conjugate=conjugate)
+        v = q.view(bu.torch_type(code))[..., :kk].double().cpu().numpy()
+        return (q, s), v, s.cpu().numpy()
+
+    def product(x, xv, xs, y, yv, ys, rows, cols, kk, ta):
+        plan = capi.ScaledGemmPlan(1, rows, cols, kk, ta, E4M3, F32, 1, 1)
+        c = torch.empty((1, 2, rows, cols), device="cuda")
+        plan.run(x[0].data_ptr(), x[1].data_ptr(), y[0].data_ptr(), y[1].data_ptr(), c.data_ptr(),
+                 gu.stream_handle())
+        torch.cuda.synchronize()
+        want, s_re, s_im = bu.scaled_product(xv, xs, 1, yv, ys, 1)
+        _check(c, want, s_re, s_im, kk, F32)
+        got = c.double().cpu().numpy()
+        return got[0, 0] + 1j * got[0, 1]
+
+    # dA [m][k]: over n.  B is [n][k]: for rows of k it is col-major.
+    d_a = product(*quantised(g, m, n, E5M2, ROW, False), *quantised(b, k, n, E4M3, COL, True),
+                  m, k, n, E5M2)
+    # dB [n][k]: over m
+    d_b = product(*quantised(g, n, m, E5M2, COL, False), *quantised(a, k, m, E4M3, COL, True),
+                  n, k, m, E5M2)
+    av, bv, gv = ((x[0, 0] + 1j * x[0, 1]).numpy().astype(np.complex128) for x in (a, b, g))
+    exact_a, exact_b = gv @ bv.conj(), gv.T @ av.conj()
+    # e5m2 rounds by at most 2^-3, e4m3 by 2^-4; errors of the terms are independent
+    for got, want in ((d_a, exact_a), (d_b, exact_b)):
+        assert np.linalg.norm(got - want) <= (2.0 ** -3 + 2.0 ** -4) * np.linalg.norm(want)
+
+    def loss(x, y):
+        return float(np.sum(gv.conj() * (x @ y.T)).real)
+
+    # L is linear in either operand: differences are exact up to rounding
+    for _ in range(3):
+        e = rng.standard_normal((m, k)) + 1j * rng.standard_normal((m, k))
+        f = rng.standard_normal((n, k)) + 1j * rng.standard_normal((n, k))
+        da = (loss(av + e, bv) - loss(av - e, bv)) / 2
+        db = (loss(av, bv + f) - loss(av, bv - f)) / 2
+        assert abs(da - np.sum(exact_a.conj() * e).real) <= 1e-9 * np.linalg.norm(exact_a) * np.linalg.norm(e)
+        assert abs(db - np.sum(exact_b.conj() * f).real) <= 1e-9 * np.linalg.norm(exact_b) * np.linalg.norm(f)
