@@ -6,20 +6,26 @@
 // either operand: the operands quantize.cu writes.
 //
 // The scales differ from block to block, so a block's product cannot stay in the tensor-memory
-// accumulator while the next one is added to it.  Per 128 k the MMA warp fills one of two tensor-memory
-// buffers (Re and Im, BN columns each) and eight epilogue warps move the other one into float32
-// sums in registers, acc += (d * sA) * sB in packed pairs.  A 128 x 128 block is 16 MMAs of 64 clocks
-// = 1024 clocks of tensor pipe; moving it takes 256 packed instructions per scheduler beside 64
-// columns of tensor-memory loads, so the sums hide behind the MMAs.  The float32 sums of a 128 x 128
-// complex tile are 128 registers in each of 256 threads, which is what bounds the tile: no wider
-// tile fits the register file.
+// accumulator while the next one is added to it.  Per 128 k the MMA warps fill one of two tensor-memory
+// buffers (Re and Im, BN columns each) while eight epilogue warps add the other one to float32 sums in
+// registers, sum += d * (sA sB).  The sums of a 128 x 128 complex tile are 128 registers in each of 256
+// threads, which is what bounds the tile: no wider tile fits the register file.
+//
+// What bounds it at 4096 x 4096 x 16384, measured in clocks per 128 x 128 x 128 block: the 16 MMAs take
+// 1570 (a 128-column MMA reads 8 KiB of operands from shared memory beside the 64 KiB that TMA brings in
+// per block; their arithmetic alone is 1024), adding a block to the sums takes 600 of an epilogue
+// warp's time and hides behind them.  With normally distributed operands the 1 kW power cap takes the
+// clock to 1.25 .. 1.45 GHz: 1.95 to 2.06 PFLOP/s, against 2.31 of the unscaled kernel with the same
+// tile and 2.69 with 256 columns.  Tried and dropped: sixteen epilogue warps (2640 clocks), packed
+// two-value arithmetic (more register moves than it saves), Re and Im handed over apart (2500).
 //
 // Either operand may be the 128-row side of the tile (the product is symmetric in A and B); the
 // plan takes the one that wastes fewer rows, so one row of A against many rows of B is a
-// 128 x 16 tile that reads B once.  Problems whose tiles do not fill the device evenly are cut into
-// equal runs of 128-k blocks instead of whole tiles: a CTA that holds part of a tile's blocks writes
-// its sums to the plan's workspace, and the CTA that completes the tile adds the parts in the order
-// of k, whoever that is, so results do not depend on timing.
+// 128 x 16 tile that reads B once: memory-bound, 1 x 8192 x 8192 in 31 us (134 MB, 4.3 TB/s; a set-up of
+// 3 us and the last exchange of 2 us are in it).  Problems whose tiles do not fill the device evenly may
+// be cut into equal runs of 128-k blocks instead of whole tiles: a CTA that holds part of a tile's blocks
+// writes its sums to the plan's workspace, and the CTA that completes the tile adds the parts in the
+// order of k, whoever that is, so results do not depend on timing.
 #include <cstdlib>
 #include <new>
 
