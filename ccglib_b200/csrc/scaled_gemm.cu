@@ -174,10 +174,6 @@ template <> __device__ __forceinline__ void tmem_ld_cols<16>(uint32_t taddr, uin
       : "memory");
 }
 
-template <> __device__ __forceinline__ void tmem_ld_cols<32>(uint32_t taddr, uint32_t *r) {
-  tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
-}
-
 // How a block's sums are scaled.  s * t is formed first, once per row and column, unless a scale is
 // so large that the product could overflow where d * s * t does not (d may be zero): then d * s
 // comes first.
@@ -464,106 +460,106 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
   let_next_start();
 
   if (warp < C::kFirstEpiWarp) {
-  if constexpr (C::kSplitRegs) regs_dec<40>();
-  Walk walk(p);
-  Segment seg;
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    wait_for_previous();
-    uint32_t stage = 0, phase = 0, issued = 0;
-    bool ok = true;
-    while (ok && walk.next(p, seg)) {
-      const TileCoord t = decode_tile(p.g, seg.tile);
-      for (uint32_t kb = seg.k0; kb < seg.k1; ++kb) {
-        if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.g.status,
-                       kDevTimeoutProducer, p.g.wait_cycles)) {
-          ok = false;
+    if constexpr (C::kSplitRegs) regs_dec<40>();
+    Walk walk(p);
+    Segment seg;
+    if (warp == 0) {
+      // ------------------------------------------------------------------ TMA producer
+      wait_for_previous();
+      uint32_t stage = 0, phase = 0, issued = 0;
+      bool ok = true;
+      while (ok && walk.next(p, seg)) {
+        const TileCoord t = decode_tile(p.g, seg.tile);
+        for (uint32_t kb = seg.k0; kb < seg.k1; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.g.status,
+                         kDevTimeoutProducer, p.g.wait_cycles)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            const uint32_t full = bar_full + 8 * stage;
+            const uint32_t dst = smem_base + stage * C::kStageBytes;
+            const int32_t x = static_cast<int32_t>(kb * kBlockK), z = static_cast<int32_t>(2 * t.b);
+            mbar_arrive_expect_tx(full, C::kStageBytes);
+            tma_load_3d(dst, &tm_a, x, static_cast<int32_t>(t.mt * kBlockM), z, full);
+            tma_load_3d(dst + C::kABytes, &tm_b, x, static_cast<int32_t>(t.nt * BN), z, full);
+          }
+          __syncwarp();
+          issued |= 1u << stage;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (*abort_flag) {
+        // our own copies must land before the CTA leaves
+        for (int s = 0; s < kStages; ++s) {
+          if (!(issued & (1u << s))) continue;
+          const uint32_t parity = (static_cast<uint32_t>(s) < stage) ? phase : (phase ^ 1);
+          const long long t0 = clock64();
+          while (!mbar_try_wait(bar_full + 8 * s, parity)) {
+            if (clock64() - t0 > p.g.wait_cycles) {
+              atomicOr(p.g.status, kDevTimeoutDrain);
+              break;
+            }
+          }
+        }
+      }
+    } else if (warp <= 2) {
+      // ------------------------------------------------------------------ MMA issuers
+      // Two warps take the blocks in turn, each its own accumulator buffer.  Issuing blocks while the tensor
+      // core's short queue is full, so one warp alone leaves the tensor core idle while it waits for the
+      // barriers of the next block (350 clocks of 1900); the other has done that when its turn comes.
+      const uint32_t acc = warp - 1;
+      const uint64_t blocks = walk.blocks(p);
+      uint32_t stage = acc, phase = 0, turn = 0;
+      static_assert(kStages > 2 && kAccBuffers == 2, "a stage and a buffer for either warp");
+      for (uint64_t i = acc; i < blocks; i += 2, ++turn) {
+        if (!mbar_wait(bar_acc_empty + 8 * acc, (turn & 1) ^ 1, abort_flag, p.g.status, kDevTimeoutMma,
+                       p.g.wait_cycles) ||
+            !mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.g.status, kDevTimeoutMma,
+                       p.g.wait_cycles)) {
           break;
         }
+        // the other warp has issued block i - 1
+        if (i > 0 && !mbar_wait(bar_turn + 8 * acc, (acc == 0 ? turn - 1 : turn) & 1, abort_flag, p.g.status,
+                                kDevTimeoutMma, p.g.wait_cycles)) {
+          break;
+        }
+        tc_fence_after();
         if (lane == 0) {
-          const uint32_t full = bar_full + 8 * stage;
-          const uint32_t dst = smem_base + stage * C::kStageBytes;
-          const int32_t x = static_cast<int32_t>(kb * kBlockK), z = static_cast<int32_t>(2 * t.b);
-          mbar_arrive_expect_tx(full, C::kStageBytes);
-          tma_load_3d(dst, &tm_a, x, static_cast<int32_t>(t.mt * kBlockM), z, full);
-          tma_load_3d(dst + C::kABytes, &tm_b, x, static_cast<int32_t>(t.nt * BN), z, full);
+          const uint32_t a_base = smem_base + stage * C::kStageBytes;
+          const uint32_t b_base = a_base + C::kABytes;
+          const uint32_t d = tmem_base + acc * C::kAccCols;
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k) {
+            const uint64_t a_re = smem_desc<128>(a_base + k * 32);
+            const uint64_t a_im = smem_desc<128>(a_base + C::kAPlane + k * 32);
+            const uint64_t b_re = smem_desc<128>(b_base + k * 32);
+            if constexpr (C::kStacked) {
+              tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
+              tc_mma<kKindF8F6F4>(d + 2 * BN, a_im, b_re, p.g.idesc, k != 0);
+            } else {
+              const uint64_t b_im = smem_desc<128>(b_base + C::kBPlane + k * 32);
+              tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
+              tc_mma<kKindF8F6F4>(d + BN, a_re, b_im, p.g.idesc, k != 0);
+              tc_mma<kKindF8F6F4>(d + BN, a_im, b_re, p.g.idesc, 1u);
+              tc_mma<kKindF8F6F4>(d, a_im, b_im, p.g.idesc_neg_a, 1u);
+            }
+          }
+          if (i + 1 < blocks) mbar_arrive(bar_turn + 8 * (acc ^ 1));
+          tc_commit(bar_empty + 8 * stage);
+          tc_commit(bar_acc_full + 8 * acc);
         }
         __syncwarp();
-        issued |= 1u << stage;
-        if (++stage == kStages) {
-          stage = 0;
+        stage += 2;
+        if (stage >= kStages) {
+          stage -= kStages;
           phase ^= 1;
         }
       }
     }
-    if (*abort_flag) {
-      // our own copies must land before the CTA leaves
-      for (int s = 0; s < kStages; ++s) {
-        if (!(issued & (1u << s))) continue;
-        const uint32_t parity = (static_cast<uint32_t>(s) < stage) ? phase : (phase ^ 1);
-        const long long t0 = clock64();
-        while (!mbar_try_wait(bar_full + 8 * s, parity)) {
-          if (clock64() - t0 > p.g.wait_cycles) {
-            atomicOr(p.g.status, kDevTimeoutDrain);
-            break;
-          }
-        }
-      }
-    }
-  } else if (warp <= 2) {
-    // ------------------------------------------------------------------ MMA issuers
-    // Two warps take the blocks in turn, each its own accumulator buffer.  Issuing blocks while the tensor
-    // core's short queue is full, so one warp alone leaves the tensor core idle while it waits for the
-    // barriers of the next block (350 clocks of 1900); the other has done that when its turn comes.
-    const uint32_t acc = warp - 1;
-    const uint64_t blocks = walk.blocks(p);
-    uint32_t stage = acc, phase = 0, turn = 0;
-    static_assert(kStages > 2 && kAccBuffers == 2, "a stage and a buffer for either warp");
-    for (uint64_t i = acc; i < blocks; i += 2, ++turn) {
-      if (!mbar_wait(bar_acc_empty + 8 * acc, (turn & 1) ^ 1, abort_flag, p.g.status, kDevTimeoutMma,
-                     p.g.wait_cycles) ||
-          !mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.g.status, kDevTimeoutMma,
-                     p.g.wait_cycles)) {
-        break;
-      }
-      // the other warp has issued block i - 1
-      if (i > 0 && !mbar_wait(bar_turn + 8 * acc, (acc == 0 ? turn - 1 : turn) & 1, abort_flag, p.g.status,
-                              kDevTimeoutMma, p.g.wait_cycles)) {
-        break;
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t a_base = smem_base + stage * C::kStageBytes;
-        const uint32_t b_base = a_base + C::kABytes;
-        const uint32_t d = tmem_base + acc * C::kAccCols;
-#pragma unroll
-        for (int k = 0; k < kBlockK / 32; ++k) {
-          const uint64_t a_re = smem_desc<128>(a_base + k * 32);
-          const uint64_t a_im = smem_desc<128>(a_base + C::kAPlane + k * 32);
-          const uint64_t b_re = smem_desc<128>(b_base + k * 32);
-          if constexpr (C::kStacked) {
-            tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
-            tc_mma<kKindF8F6F4>(d + 2 * BN, a_im, b_re, p.g.idesc, k != 0);
-          } else {
-            const uint64_t b_im = smem_desc<128>(b_base + C::kBPlane + k * 32);
-            tc_mma<kKindF8F6F4>(d, a_re, b_re, p.g.idesc, k != 0);
-            tc_mma<kKindF8F6F4>(d + BN, a_re, b_im, p.g.idesc, k != 0);
-            tc_mma<kKindF8F6F4>(d + BN, a_im, b_re, p.g.idesc, 1u);
-            tc_mma<kKindF8F6F4>(d, a_im, b_im, p.g.idesc_neg_a, 1u);
-          }
-        }
-        if (i + 1 < blocks) mbar_arrive(bar_turn + 8 * (acc ^ 1));
-        tc_commit(bar_empty + 8 * stage);
-        tc_commit(bar_acc_full + 8 * acc);
-      }
-      __syncwarp();
-      stage += 2;
-      if (stage >= kStages) {
-        stage -= kStages;
-        phase ^= 1;
-      }
-    }
-  }
   } else {
     // ------------------------------------------------------------------ epilogue warps
     if constexpr (C::kSplitRegs) regs_inc<232>();
