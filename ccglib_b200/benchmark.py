@@ -1,4 +1,4 @@
-"""Command-line micro-benchmarks of the three operators, with the flags, method and output columns
+"""Command-line micro-benchmarks of the operators, with the flags, method and output columns
 of the reference's benchmark programs (benchmark/benchmark_gemm.cpp:14-50,255-323,
 benchmark_transpose.cpp, benchmark_packing.cpp): one probe run to estimate the iteration count for
 `--benchmark_duration` seconds, a warm-up of the same length, then CUDA-event timing of back-to-back
@@ -7,6 +7,9 @@ runs with the operands resident on the device.
     python -m ccglib_b200.benchmark gemm --b 8 --m 8192 --n 8192 --k 8192 --precision_in float16
     python -m ccglib_b200.benchmark transpose --b 8 --m 8192 --n 8192 --precision float16
     python -m ccglib_b200.benchmark packing --n 1073741824 --direction pack
+    python -m ccglib_b200.benchmark quantize --b 4 --m 4096 --k 16384 --precision_in float32
+    python -m ccglib_b200.benchmark scaled_gemm --b 4 --m 4096 --n 4096 --k 16384
+    python -m ccglib_b200.benchmark orthogonalize --b 8 --m 4096 --n 1024 --steps 8
     python -m ccglib_b200.benchmark gemm --gpus 8 --b 64 --m 8192 --n 8192 --k 8192 --precision_in float16
 
 Several sizes may be given (`--m 1024,2048 --n ... --k ...`).  `--pad` rounds M, N, K up to the
@@ -239,6 +242,99 @@ def bench_packing(args) -> None:
             del byte_side, word_side
 
 
+def _report(args, values, ms, rate, unit, watts) -> None:
+    if args.csv:
+        print(",".join(["%d" % v for v in values] + ["%g" % ms, "%g" % rate]) +
+              (",%g" % watts if watts is not None else ""))
+    else:
+        print("%20s %7.4g ms, %7.4g %s" % ("x".join("%d" % v for v in values), ms, rate, unit) +
+              (", %7.4g W" % watts if watts is not None else ""))
+
+
+def _header(args, labels, rate) -> None:
+    if args.csv:
+        print("#%s,runtime_ms,%s" % (",".join(labels), rate) + (",watt" if args.measure_power else ""))
+
+
+def bench_quantize(args) -> None:
+    import torch
+
+    tin, tout = PRECISIONS[args.precision_in], PRECISIONS[args.precision_out]
+    axis = capi.INTERLEAVED if args.complex_axis == "interleaved" else capi.PLANAR
+    order = capi.COL_MAJOR if args.mem_order == "col" else capi.ROW_MAJOR
+    stream = int(torch.cuda.current_stream().cuda_stream)
+    meter = _EnergyMeter(args.device) if args.measure_power else None
+    _header(args, ("M", "K"), "gbytes_per_s")
+    first = True
+    for _ in range(args.nr_benchmarks):
+        for M, K in zip(_sizes(args.m), _sizes(args.k)):
+            d_in = torch.full((args.b * 2 * M * K * BITS[tin] // 8,), 0x3C, dtype=torch.uint8,
+                              device="cuda")
+            d_out = torch.empty(args.b * 2 * M * capi.operand_pitch(K), dtype=torch.uint8, device="cuda")
+            d_scale = torch.empty(args.b * _ceil(K, 128) * _ceil(M, args.block_rows), device="cuda")
+            ms, _, watts = _time(
+                lambda: capi.quantize(args.b, M, K, tin, tout, d_in.data_ptr(), d_out.data_ptr(),
+                                      d_scale.data_ptr(), stream, input_complex_axis=axis,
+                                      input_mem_order=order, block_rows=args.block_rows),
+                args.benchmark_duration, first, meter)
+            first = False
+            moved = d_in.numel() + d_out.numel() + 4 * d_scale.numel()
+            _report(args, (M, K), ms, 1e-6 * moved / ms, "GByte/s", watts)
+            del d_in, d_out, d_scale
+
+
+def bench_scaled_gemm(args) -> None:
+    import torch
+
+    ta, tb, tout = (PRECISIONS[x] for x in (args.precision_a, args.precision_b, args.precision_out))
+    stream = int(torch.cuda.current_stream().cuda_stream)
+    meter = _EnergyMeter(args.device) if args.measure_power else None
+    _header(args, ("M", "N", "K"), "tops")
+    first = True
+    for _ in range(args.nr_benchmarks):
+        for M, N, K in zip(_sizes(args.m), _sizes(args.n), _sizes(args.k)):
+            pitch, kb = capi.operand_pitch(K), _ceil(K, 128)
+            a, b = (torch.full((args.b * 2 * rows * pitch,), 0x3C, dtype=torch.uint8, device="cuda")
+                    for rows in (M, N))
+            sa = torch.ones(args.b * kb * _ceil(M, args.a_block_rows), device="cuda")
+            sb = torch.ones(args.b * kb * _ceil(N, args.b_block_rows), device="cuda")
+            c = torch.empty(args.b * 2 * M * N * BITS[tout] // 8, dtype=torch.uint8, device="cuda")
+            plan = capi.ScaledGemmPlan(args.b, M, N, K, ta, tb, tout, args.a_block_rows,
+                                       args.b_block_rows)
+            ms, _, watts = _time(
+                lambda: plan.run(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(),
+                                 c.data_ptr(), stream), args.benchmark_duration, first, meter)
+            first = False
+            _report(args, (M, N, K), ms, 8e-9 * args.b * M * N * K / ms, "TOps/s",
+                    watts)
+            del plan, a, b, c
+
+
+def bench_orthogonalize(args) -> None:
+    import torch
+
+    tin, tout = PRECISIONS[args.precision_in], PRECISIONS[args.precision_out]
+    stream = int(torch.cuda.current_stream().cuda_stream)
+    meter = _EnergyMeter(args.device) if args.measure_power else None
+    _header(args, ("M", "N"), "tops")
+    first = True
+    dtype = {capi.FLOAT32: torch.float32, capi.FLOAT16: torch.float16,
+             capi.BFLOAT16: torch.bfloat16}[tin]
+    for _ in range(args.nr_benchmarks):
+        for M, N in zip(_sizes(args.m), _sizes(args.n)):
+            x = torch.randn((args.b, 2, M, N), device="cuda").to(dtype)
+            y = torch.empty(args.b * 2 * M * N, dtype=torch.float16, device="cuda")
+            plan = capi.OrthogonalizePlan(args.b, M, N, tin, tout, args.steps)
+            ms, _, watts = _time(lambda: plan.run(x.data_ptr(), y.data_ptr(), stream),
+                                 args.benchmark_duration, first, meter)
+            first = False
+            short, long = min(M, N), max(M, N)
+            # S and S^2 are Hermitian: half of each
+            ops = args.b * args.steps * (12 * short * short * long + 4 * short ** 3)
+            _report(args, (M, N), ms, 1e-9 * ops / ms, "TOps/s", watts)
+            del plan, x, y
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m ccglib_b200.benchmark")
     sub = ap.add_subparsers(dest="what", required=True)
@@ -275,6 +371,36 @@ def main(argv=None) -> int:
     p.add_argument("--n", required=True)
     p.add_argument("--direction", default="pack", choices=["pack", "unpack"])
     common(p)
+    floats, fp8 = ["bfloat16", "float16", "float32"], ["float8e4m3", "float8e5m2"]
+    q = sub.add_parser("quantize")
+    q.add_argument("--b", type=int, default=1)
+    q.add_argument("--m", required=True)
+    q.add_argument("--k", required=True)
+    q.add_argument("--precision_in", default="float32", choices=floats)
+    q.add_argument("--precision_out", default="float8e4m3", choices=fp8)
+    q.add_argument("--complex_axis", default="planar", choices=["planar", "interleaved"])
+    q.add_argument("--mem_order", default="row", choices=["row", "col"])
+    q.add_argument("--block_rows", type=int, default=1, choices=[1, 128])
+    common(q)
+    s = sub.add_parser("scaled_gemm")
+    s.add_argument("--b", type=int, default=1)
+    s.add_argument("--m", required=True)
+    s.add_argument("--n", required=True)
+    s.add_argument("--k", required=True)
+    s.add_argument("--precision_a", default="float8e4m3", choices=fp8)
+    s.add_argument("--precision_b", default="float8e4m3", choices=fp8)
+    s.add_argument("--precision_out", default="float32", choices=floats)
+    s.add_argument("--a_block_rows", type=int, default=1, choices=[1, 128])
+    s.add_argument("--b_block_rows", type=int, default=128, choices=[1, 128])
+    common(s)
+    o = sub.add_parser("orthogonalize")
+    o.add_argument("--b", type=int, default=1)
+    o.add_argument("--m", required=True)
+    o.add_argument("--n", required=True)
+    o.add_argument("--steps", type=int, default=5)
+    o.add_argument("--precision_in", default="float32", choices=floats)
+    o.add_argument("--precision_out", default="float16", choices=["bfloat16", "float16"])
+    common(o)
     args = ap.parse_args(argv)
 
     import torch
@@ -283,7 +409,9 @@ def main(argv=None) -> int:
         print("a CUDA device is required", file=sys.stderr)
         return 1
     torch.cuda.set_device(args.device)
-    {"gemm": bench_gemm, "transpose": bench_transpose, "packing": bench_packing}[args.what](args)
+    {"gemm": bench_gemm, "transpose": bench_transpose, "packing": bench_packing,
+     "quantize": bench_quantize, "scaled_gemm": bench_scaled_gemm,
+     "orthogonalize": bench_orthogonalize}[args.what](args)
     return 0
 
 
