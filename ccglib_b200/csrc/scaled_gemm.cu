@@ -211,19 +211,28 @@ __device__ __forceinline__ void add_block(uint32_t taddr, uint32_t done, uint32_
       if (lane == 0) mbar_arrive(done);
     }
 #pragma unroll
-    for (int j = 0; j < kStep; ++j) {
-      float f = s;
-      if constexpr (MODE == kColumnFactors) f = s * cols[c + j];
-      if constexpr (MODE == kTwoSteps) f = cols[c + j];
+    for (int j = 0; j < kStep; j += 4) {
+      float f[4] = {s, s, s, s};
+      if constexpr (MODE != kOneFactor) {
+        const float4 t = *reinterpret_cast<const float4 *>(cols + c + j);
+        f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
+        if constexpr (MODE == kColumnFactors) {
 #pragma unroll
-      for (int plane = 0; plane < 2; ++plane) {
-        float x = __uint_as_float(v[plane][j]);
-        // Re = Ar.Br - Ai.Bi, Im = Ar.Bi + Ai.Br
-        if constexpr (C::kStacked) {
-          fma_to(x, __uint_as_float(v[kAccs - 1 - plane][j]), plane == 0 ? -1.0f : 1.0f);
+          for (int e = 0; e < 4; ++e) f[e] *= s;
         }
-        if constexpr (MODE == kTwoSteps) x *= s;
-        fma_to(sum[plane][c + j], x, f);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane) {
+          float x = __uint_as_float(v[plane][j + e]);
+          // Re = Ar.Br - Ai.Bi, Im = Ar.Bi + Ai.Br
+          if constexpr (C::kStacked) {
+            fma_to(x, __uint_as_float(v[kAccs - 1 - plane][j + e]), plane == 0 ? -1.0f : 1.0f);
+          }
+          if constexpr (MODE == kTwoSteps) x *= s;
+          fma_to(sum[plane][c + j + e], x, f[e]);
+        }
       }
     }
   }
