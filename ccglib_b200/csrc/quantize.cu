@@ -3,10 +3,14 @@
 //
 //   amax  = max(|re|, |im|) over the finite entries of the block
 //   scale = max(amax / FMAX, 2^-126)         FMAX = 448 (e4m3), 57344 (e5m2)
-//   q     = fp8_rne(x * (1 / scale))         every step a correctly rounded float32 operation
+//   q     = fp8_rne(x * (FMAX / amax))       every step a correctly rounded float32 operation
+//
+// (x * 2^126 where the scale is at its floor.)  FMAX / amax is one rounding away from the exact factor,
+// 1 / scale would be two: with 16-bit input exact ties between two fp8 values are common, and after a second
+// rounding they fall to either side.
 //
 // A block is 128 consecutive k of one row, or 128 x 128 (rows x k); re and im share the scale, so a
-// phase survives.  The floor 2^-126 keeps 1 / scale finite; a silent block gets it and quantises to
+// phase survives.  The floor 2^-126 keeps the factor finite; a silent block gets it and quantises to
 // zeros.  A NaN stays a NaN and an infinity becomes what the format has for it (e5m2: infinity,
 // e4m3: NaN); neither enters amax, so one bad sample does not cost its block the other samples.
 //
@@ -59,6 +63,12 @@ __device__ __forceinline__ uint32_t finite_abs_bits(float x) {
 template <bool E5M2> __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
   const float s = __fdiv_rn(__uint_as_float(amax_bits), E5M2 ? 57344.0f : 448.0f);
   return fmaxf(s, kMinScale);
+}
+
+// What the values of a block with this maximum and scale are multiplied by.
+template <bool E5M2> __device__ __forceinline__ float block_factor(uint32_t amax_bits, float scale) {
+  return scale > kMinScale ? __fdiv_rn(E5M2 ? 57344.0f : 448.0f, __uint_as_float(amax_bits))
+                           : 8.507059e37f;  // 2^126
 }
 
 // Four scaled values -> four fp8 bytes, first value in the low byte.  SPECIAL: the values may hold
@@ -214,7 +224,7 @@ quantize_rows_kernel(const QuantizeParams p) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const float s = block_scale<E5M2>(top[i]);
-      const float inv = __fdiv_rn(1.0f, s), inv_im = p.im_sign * inv;
+      const float inv = block_factor<E5M2>(top[i], s), inv_im = p.im_sign * inv;
       if constexpr (kTile) {
         if (i == 0 && threadIdx.x == 0) scale_row[group] = s;
       } else {
@@ -365,12 +375,12 @@ quantize_cols_kernel(const QuantizeParams p) {
       uint32_t t = max(max(row_max[lane], row_max[32 + lane]), max(row_max[64 + lane], row_max[96 + lane]));
       t = __reduce_max_sync(0xFFFFFFFFu, t);
       const float s = block_scale<E5M2>(t);
-      inv_tile = __fdiv_rn(1.0f, s);
+      inv_tile = block_factor<E5M2>(t, s);
       if (tid == 0) p.scale[(b * p.blocks_k + kb) * p.blocks_rows + group] = s;
     } else {
       if (tid < 128) {
         const float s = block_scale<E5M2>(row_max[tid]);
-        row_inv[tid] = __fdiv_rn(1.0f, s);
+        row_inv[tid] = block_factor<E5M2>(row_max[tid], s);
         if (r0 + tid < p.rows) p.scale[(b * p.blocks_k + kb) * p.blocks_rows + r0 + tid] = s;
       }
       __syncthreads();

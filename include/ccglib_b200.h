@@ -167,8 +167,8 @@ CCGLIB_B200_API int ccglib_b200_pack_run(size_t n, int direction, int input_comp
  *   behind k written as zeros; scales [batch][ceil(k / 128)][ceil(rows / block_rows)] float32.
  * A block is block_rows (1 or 128) rows x 128 k, both planes together:
  *   amax = max(|re|, |im|) over its finite entries,  scale = max(amax / FMAX, 2^-126),
- *   q = x * (1 / scale) rounded to nearest even, FMAX = 448 (e4m3) or 57344 (e5m2),
- * in float32.  NaN stays NaN; an infinity becomes an infinity in e5m2 and NaN in e4m3.
+ *   q = x * (FMAX / amax), or x * 2^126 where scale is 2^-126, rounded to nearest even,
+ * in float32; FMAX = 448 (e4m3) or 57344 (e5m2).  NaN stays NaN; an infinity becomes an infinity in e5m2 and NaN in e4m3.
  * Asynchronous on `stream`, one launch, no scratch.
  *
  * The products of a backward pass of C = A x B^T are products of the same kind, over operands quantised

@@ -35,14 +35,18 @@ def round_fp8(v, code):
 
 
 def block_scales(x, code, block_rows):
-    """x: planar [batch][2][rows][k] float32 -> scales [batch][kb][rb] float32 by the definition."""
+    """x: planar [batch][2][rows][k] float32 -> (scales, factors) [batch][kb][rb] float32 by the
+    definition."""
     batch, _, rows, k = x.shape
     kb, rb = ceil(k, BLOCK), ceil(rows, block_rows)
     mag = np.zeros((batch, rb * block_rows, kb * BLOCK), np.float32)
     mag[:, :rows, :k] = np.where(np.isfinite(x), np.abs(x), np.float32(0)).max(axis=1)
     amax = mag.reshape(batch, rb, block_rows, kb, BLOCK).max(axis=(2, 4))
     scale = np.maximum(amax / np.float32(FMAX[code]), TINY)
-    return np.ascontiguousarray(scale.transpose(0, 2, 1))
+    with np.errstate(divide="ignore", over="ignore"):
+        factor = np.where(scale > TINY, np.float32(FMAX[code]) / amax, np.float32(2.0 ** 126))
+    return (np.ascontiguousarray(scale.transpose(0, 2, 1)),
+            np.ascontiguousarray(factor.transpose(0, 2, 1)))
 
 
 def per_element(scale, block_rows, rows, k):
@@ -54,10 +58,9 @@ def per_element(scale, block_rows, rows, k):
 def quantize(x, code, block_rows):
     """Planar float32 x -> (values [batch][2][rows][k] float64, scales), the definition's steps in
     float32 (numpy's division and product are correctly rounded)."""
-    scale = block_scales(x, code, block_rows)
-    inv = np.float32(1) / per_element(scale, block_rows, x.shape[2], x.shape[3])
+    scale, factor = block_scales(x, code, block_rows)
     with np.errstate(invalid="ignore", over="ignore"):
-        v = x * inv[:, None]
+        v = x * per_element(factor, block_rows, x.shape[2], x.shape[3])[:, None]
     finite = np.isfinite(v)
     q = round_fp8(np.where(finite, v, 0), code)
     special = v.astype(np.float64) if code == capi.FLOAT8E5M2 else np.full(v.shape, np.nan)

@@ -71,7 +71,7 @@ def test_matches_definition(type_in, axis, order, block_rows):
 @pytest.mark.parametrize("order", [capi.ROW_MAJOR, capi.COL_MAJOR])
 @pytest.mark.parametrize("type_out", [E4M3, E5M2])
 def test_special_values(type_out, order):
-    """NaN and infinities stay out of the maximum; tiny and huge blocks keep a finite 1 / scale."""
+    """NaN and infinities stay out of the maximum; tiny and huge blocks keep a finite factor."""
     import torch
 
     rng = np.random.default_rng(8)
