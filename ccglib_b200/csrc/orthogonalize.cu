@@ -12,9 +12,9 @@
 // epilogue; the last update writes the caller's type and layout.
 // The launches are programmatic: a product's CTAs set up while the one before it drains.
 //
-// Measured: 8 x 4096 x 1024, eight steps, 3.57 to 3.68 ms (0.97 to 1.0 PFLOP/s of the operations that the
-// Hermitian halves need, 1.3 PFLOP/s in the large products, power-capped); 1024 x 1024, five steps, 198 us
-// (a product of 1024^3 takes about 12 us: its operands' way from L2 into 144 SMs and two latencies).
+// Measured: 8 x 4096 x 1024, eight steps, 3.50 to 3.68 ms (0.97 to 1.02 PFLOP/s of the operations that the
+// Hermitian halves need, 1.3 PFLOP/s in the large products, power-capped); 1024 x 1024, five steps, 182 us
+// (a product of 1024^3 takes about 11 us: its operands' way from L2 into 144 SMs and two latencies).
 //
 // Between products X, S and P are float16.  All three are bounded (singular values stay near or below
 // one), X is kept times a power of two near sqrt(long side) so that its entries are near one, and float16
@@ -116,37 +116,46 @@ __device__ __forceinline__ void st_shared_u16(uint32_t addr, uint16_t v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
 }
 
-// 32 rows x 32 columns (one row per lane, from m0; columns from n0) of one batch item.
+// c0 of this lane's row m, 32 columns from n0: Re in c[0..3], Im in c[4..7].  Loaded well before it is used.
+__device__ __forceinline__ void load_c0(const OrthParams &p, uint32_t b, uint32_t m, uint32_t n0,
+                                        uint4 (&c)[8]) {
+  if (p.c0 == nullptr) return;
+  const size_t plane = static_cast<size_t>(p.m) * p.c0_pitch;
+  const __half *src = p.c0 + static_cast<size_t>(b) * 2 * plane + static_cast<size_t>(m) * p.c0_pitch + n0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool inside = m < p.m && n0 + 8 * j < p.c0_pitch;  // the pitch is a multiple of eight
+    c[j] = inside ? *reinterpret_cast<const uint4 *>(src + 8 * j) : make_uint4(0, 0, 0, 0);
+    c[4 + j] = inside ? *reinterpret_cast<const uint4 *>(src + plane + 8 * j) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// 32 rows x 32 columns (one row per lane, from m0; columns from n0) of one batch item; c as load_c0 left it.
 __device__ __forceinline__ void orth_store(const OrthParams &p, const CUtensorMap *tm_c,
                                            uint32_t staging, uint32_t lane, uint32_t b, uint32_t m0,
-                                           uint32_t n0, float (&re)[32], float (&im)[32]) {
+                                           uint32_t n0, const uint4 (&c)[8], float (&re)[32],
+                                           float (&im)[32]) {
   const uint32_t m = m0 + lane;
-  if (p.c0 != nullptr && m < p.m) {
-    const size_t plane = static_cast<size_t>(p.m) * p.c0_pitch;
-    const __half *src = p.c0 + static_cast<size_t>(b) * 2 * plane +
-                        static_cast<size_t>(m) * p.c0_pitch + n0;
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (n0 + j < p.c0_pitch) {  // the pitch is a multiple of eight
-        const uint4 r = *reinterpret_cast<const uint4 *>(src + j);
-        const uint4 i = *reinterpret_cast<const uint4 *>(src + plane + j);
-        const uint32_t rw[4] = {r.x, r.y, r.z, r.w}, iw[4] = {i.x, i.y, i.z, i.w};
+  for (int j = 0; j < 32; ++j) {
+    re[j] *= p.alpha;
+    im[j] *= p.alpha;
+  }
+  if (p.c0 != nullptr) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 rv = __half22float2(*reinterpret_cast<const __half2 *>(&rw[e]));
-          const float2 iv = __half22float2(*reinterpret_cast<const __half2 *>(&iw[e]));
-          re[j + 2 * e] = fmaf(p.beta, rv.x, p.alpha * re[j + 2 * e]);
-          re[j + 2 * e + 1] = fmaf(p.beta, rv.y, p.alpha * re[j + 2 * e + 1]);
-          im[j + 2 * e] = fmaf(p.beta, iv.x, p.alpha * im[j + 2 * e]);
-          im[j + 2 * e + 1] = fmaf(p.beta, iv.y, p.alpha * im[j + 2 * e + 1]);
-        }
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t rw[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
+      const uint32_t iw[4] = {c[4 + j].x, c[4 + j].y, c[4 + j].z, c[4 + j].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 rv = __half22float2(*reinterpret_cast<const __half2 *>(&rw[e]));
+        const float2 iv = __half22float2(*reinterpret_cast<const __half2 *>(&iw[e]));
+        const int at = 8 * j + 2 * e;
+        re[at] = fmaf(p.beta, rv.x, re[at]);
+        re[at + 1] = fmaf(p.beta, rv.y, re[at + 1]);
+        im[at] = fmaf(p.beta, iv.x, im[at]);
+        im[at + 1] = fmaf(p.beta, iv.y, im[at + 1]);
       }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      re[j] *= p.alpha;
-      im[j] *= p.alpha;
     }
   }
 #pragma unroll
@@ -440,20 +449,26 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
     uint32_t acc = 0, acc_phase = 0;
     for (uint32_t tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x) {
       const TileCoord t = orth_tile<BN>(p, tile);
+      const uint32_t m0 = t.mt * kBlockM + quad * 32;
+      uint4 c_next[8];  // while the tile is multiplied
+      load_c0(p, t.b, m0 + lane, t.nt * BN, c_next);
       bool ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.status,
                           kDevTimeoutEpilogue, p.wait_cycles);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       tc_fence_after();
-      const uint32_t m0 = t.mt * kBlockM + quad * 32;
       const uint32_t taddr = tmem_base + ((quad * 32) << 16) + acc * C::kAccCols;
 #pragma unroll 1
       for (uint32_t c0 = 0; c0 < BN; c0 += 32) {
         const uint32_t n0 = t.nt * BN + c0;
         if (n0 >= p.n) break;
+        uint4 c_now[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c_now[j] = c_next[j];
+        if (c0 + 32 < BN) load_c0(p, t.b, m0 + lane, n0 + 32, c_next);
         if (m0 >= p.m || (p.hermitian && n0 < m0)) continue;  // comes from the mirror image
         float re[32], im[32];
         read_chunk<BN>(taddr + c0, p.conj_b != 0, re, im);
-        orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
+        orth_store(p, &tm_c, staging, lane, t.b, m0, n0, c_now, re, im);
       }
       tc_fence_before();
       __syncwarp();
@@ -530,6 +545,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   const TileCoord t = orth_tile<BN>(p, cluster_id_x());
   const uint32_t kb0 = p.k_blocks * rank / SPLIT, kb1 = p.k_blocks * (rank + 1) / SPLIT;
   bool done = false;  // epilogue warps: this CTA's sums are complete
+  uint4 c_next[8];
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     wait_for_previous();
@@ -572,6 +588,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     }
   } else {
     wait_for_previous();
+    load_c0(p, t.b, t.mt * kBlockM + (warp & 3) * 32 + lane, t.nt * BN + rank * kChunks * 32, c_next);
     done = mbar_wait(bar_acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue, p.wait_cycles);
     done = __all_sync(0xFFFFFFFFu, done);
   }
@@ -616,7 +633,10 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll 1
     for (uint32_t c = 0; c < kChunks; ++c) {
       const uint32_t col = (rank * kChunks + c) * 32, n0 = t.nt * BN + col;
-      if (n0 >= p.n || m0 >= p.m || (p.hermitian && n0 < m0)) continue;
+      if (n0 >= p.n || m0 >= p.m || (p.hermitian && n0 < m0)) {
+        if (c + 1 < kChunks) load_c0(p, t.b, m0 + lane, n0 + 32, c_next);
+        continue;
+      }
       float re[32], im[32];
       read_chunk<BN>(taddr + col, p.conj_b != 0, re, im);
 #pragma unroll 1
@@ -635,7 +655,8 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           }
         }
       }
-      orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
+      orth_store(p, &tm_c, staging, lane, t.b, m0, n0, c_next, re, im);
+      if (c + 1 < kChunks) load_c0(p, t.b, m0 + lane, n0 + 32, c_next);
     }
     if (lane == 0) bulk_wait_group<0>();
   }
