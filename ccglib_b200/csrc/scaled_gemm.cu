@@ -26,6 +26,7 @@
 // be cut into equal runs of 128-k blocks instead of whole tiles: a CTA that holds part of a tile's blocks
 // writes its sums to the plan's workspace, and the CTA that completes the tile adds the parts in the
 // order of k, whoever that is, so results do not depend on timing.
+#include <cmath>
 #include <cstdlib>
 #include <new>
 
@@ -45,6 +46,7 @@ struct ScaledParams {
   const float *row_scale, *col_scale;  // [batch][k_blocks][row_blocks / col_blocks]
   uint32_t row_blocks, col_blocks;
   uint32_t row_shift, col_shift;  // log2 of the rows one scale covers (0 or 7)
+  uint32_t lift_limit;  // largest scale in a tile that keeps its sums times 2^64, as float32 bits
   // equal runs of blocks (null: whole tiles)
   float *parts;        // two per CTA: [2][BN][128] sums
   unsigned *counters;  // blocks added so far, one per tile; zero between runs
@@ -148,6 +150,18 @@ __device__ __forceinline__ void fma_to(float &acc, float a, float b) {
   asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(a), "f"(b));
 }
 
+__device__ __forceinline__ void mul_pair(float &a, float &b, float f) {
+  asm("{\n"
+      ".reg .b64 x, y;\n"
+      "mov.b64 x, {%0, %1};\n"
+      "mov.b64 y, {%2, %2};\n"
+      "mul.rn.f32x2 x, x, y;\n"
+      "mov.b64 {%0, %1}, x;\n"
+      "}"
+      : "+f"(a), "+f"(b)
+      : "f"(f));
+}
+
 template <int N> __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
@@ -174,20 +188,105 @@ template <> __device__ __forceinline__ void tmem_ld_cols<16>(uint32_t taddr, uin
       : "memory");
 }
 
-// How a block's sums are scaled.  s * t is formed first, once per row and column, unless a scale is
-// so large that the product could overflow where d * s * t does not (d may be zero): then d * s
-// comes first.
-enum ScaleMode { kOneFactor, kColumnFactors, kTwoSteps };
-constexpr float kTame = 1.8446744e19f;  // 2^64
+__device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// How a block's sums d are scaled by s (of the row) and t (of the column).  d is a multiple of 2^-32 below
+// 2^41, so d s t can be an ordinary float32 where s t is not; and where d is zero the result is zero.
+//   s and t in [2^-63, 2^63] or zero: s t is normal or zero, and d * (s t) is what add_block adds.
+//   Smaller ones are common (the quantiser gives a silent block 2^-126).  A tile whose first block has
+//   such scales keeps its sums times a power of two, 2^64 or, in rows that begin below 2^-63, 2^117, for
+//   t from 2^-126 and s 2^p from 2^-9: s 2^p t, at least 2^-135, is below the normal range only where
+//   s t < 2^-190 and d s t vanishes, and is not zero, so that an infinite sum stays infinite.  s 2^p
+//   up to 2^(l + 64) and t up to 2^l keep the sum of all blocks below 2^127 (2^l is lift_limit).
+//   A block with any other scale: scale_block writes d s t over d first (1.3 to 1.5 times the time where
+//   every block needs it).
+// A power of two taken out of d in add_block instead, one multiplication per value, took 3 to 12 % more time
+// where one row in 64 is silent; this takes 0 to 4 % more than d * (s t) alone, which was wrong there.
+__host__ __device__ constexpr uint32_t exponent_bits(int e) { return static_cast<uint32_t>(127 + e) << 23; }
+
+// |x| is zero or between the float32 with the bits low and that with the bits high.
+__device__ __forceinline__ bool zero_or_between(float x, uint32_t low, uint32_t high) {
+  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+  return u == 0 || u - low <= high - low;
+}
+
+// s (times the power of two that the row's sums are kept times) and t are in the ranges above.
+__device__ __forceinline__ bool in_range(float s, float t0, float t1, bool lifted, uint32_t limit) {
+  const uint32_t t_low = lifted ? exponent_bits(-126) : exponent_bits(-63);
+  const uint32_t t_high = lifted ? limit : exponent_bits(63);
+  return zero_or_between(s, lifted ? exponent_bits(-9) : exponent_bits(-63),
+                         lifted ? limit + (64u << 23) : exponent_bits(63)) &&
+         zero_or_between(t0, t_low, t_high) && zero_or_between(t1, t_low, t_high);
+}
+
+// The accumulators of one block at `taddr` -> d s t in their place, to be added as it is.  SMALL: the
+// scales are up to 2^63 and none is subnormal; a power of two moves from d to s then, such that s 2^p t is
+// below 2^127 and, as above, not zero.  Else in float64, whose range holds every s t.
+template <int BN, bool SMALL>
+__device__ __forceinline__ void scale_columns(uint32_t taddr, const float *cols, float s) {
+  using C = ScaledCfg<BN>;
+  constexpr int kAccs = C::kStacked ? 4 : 2;
+  constexpr int kStep = C::kStacked || C::kCols < 16 ? 8 : 16;
+  const bool one = fabsf(s) >= 1.0f, middle = fabsf(s) >= 0x1p-63f;
+  const float down = one ? 1.0f : middle ? 0x1p-64f : 0x1p-117f;
+  const float s_up = s * (one ? 1.0f : middle ? 0x1p64f : 0x1p117f);
+#pragma unroll 1
+  for (int c = 0; c < C::kCols; c += kStep) {
+    uint32_t v[kAccs][kStep];
+#pragma unroll
+    for (int i = 0; i < kAccs; ++i) tmem_ld_cols<kStep>(taddr + i * BN + c, v[i]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {
+      const float t = cols[c + j];
+#pragma unroll
+      for (int plane = 0; plane < 2; ++plane) {
+        float x = __uint_as_float(v[plane][j]);
+        if constexpr (C::kStacked) {
+          fma_to(x, __uint_as_float(v[kAccs - 1 - plane][j]), plane == 0 ? -1.0f : 1.0f);
+        } else {
+          asm volatile("" : "+f"(x));  // volatile like fma_to: not ahead of the wait
+        }
+        if constexpr (SMALL) {
+          x = (x * down) * (s_up * t);
+        } else {
+          x = static_cast<float>(static_cast<double>(x) * (static_cast<double>(s) * t));
+        }
+        v[plane][j] = __float_as_uint(x);
+      }
+      if constexpr (C::kStacked) v[2][j] = v[3][j] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kAccs; ++i) {
+#pragma unroll
+      for (int j = 0; j < kStep; j += 8) tmem_st_8(taddr + i * BN + c + j, v[i] + j);
+    }
+  }
+  tmem_wait_st();
+}
+// (a call, so that add_block's registers are allotted without it)
+template <int BN>
+__device__ __noinline__ void scale_block(uint32_t taddr, const float *cols, float s, bool small) {
+  if (small) {
+    scale_columns<BN, true>(taddr, cols, s);
+  } else {
+    scale_columns<BN, false>(taddr, cols, s);
+  }
+}
 
 // The accumulators of one block at `taddr` (this warp's lanes and columns) -> sum += scaled block;
-// arrives on `done` when tensor memory is read.
-template <int BN, ScaleMode MODE>
+// arrives on `done` when tensor memory is read.  ONE: one scale, `col_scale`, covers the columns; else
+// they are at `cols`.
+template <int BN, bool ONE>
 __device__ __forceinline__ void add_block(uint32_t taddr, uint32_t done, uint32_t lane,
                                           const float *cols, float row_scale, float col_scale,
                                           float (&sum)[2][ScaledCfg<BN>::kCols]) {
   using C = ScaledCfg<BN>;
-  const float s = MODE == kOneFactor ? row_scale * col_scale : row_scale;
+  const float s = ONE ? row_scale * col_scale : row_scale;
   // Steps of kStep columns of both planes; the next step's loads are on their way while this one's
   // values are added.  Stacked accumulators are [Ar.Br | Ar.Bi | Ai.Br | Ai.Bi].
   constexpr int kAccs = C::kStacked ? 4 : 2;
@@ -213,13 +312,11 @@ __device__ __forceinline__ void add_block(uint32_t taddr, uint32_t done, uint32_
 #pragma unroll
     for (int j = 0; j < kStep; j += 4) {
       float f[4] = {s, s, s, s};
-      if constexpr (MODE != kOneFactor) {
+      if constexpr (!ONE) {
         const float4 t = *reinterpret_cast<const float4 *>(cols + c + j);
         f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
-        if constexpr (MODE == kColumnFactors) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] *= s;
-        }
+        for (int e = 0; e < 4; ++e) f[e] *= s;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -230,7 +327,6 @@ __device__ __forceinline__ void add_block(uint32_t taddr, uint32_t done, uint32_
           if constexpr (C::kStacked) {
             fma_to(x, __uint_as_float(v[kAccs - 1 - plane][j + e]), plane == 0 ? -1.0f : 1.0f);
           }
-          if constexpr (MODE == kTwoSteps) x *= s;
           fma_to(sum[plane][c + j + e], x, f[e]);
         }
       }
@@ -617,27 +713,50 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       const uint32_t n0 = t.nt * BN + first_col;
 #pragma unroll
       for (int j = 0; j < COLS; ++j) sum[0][j] = sum[1][j] = 0.0f;
-      for (uint32_t kb = seg.k0; ok && kb < seg.k1; ++kb) {
-        const float s = s_next;
-        // any column's scale stands for the block's where one covers 128 columns
-        const float col = __shfl_sync(0xFFFFFFFFu, t0_next, 0);
-        const bool tame = __all_sync(0xFFFFFFFFu, fabsf(s) <= kTame && fabsf(t0_next) <= kTame &&
-                                                      fabsf(t1_next) <= kTame);
-        const bool one_factor = tame && p.col_shift != 0;
-        float *cols = col_buf + (kb & 1) * COLS;
-        if (!one_factor) {
-          // through the staging tile, once the last stores have read it
-          if (lane == 0) bulk_wait_group_read<0>();
-          __syncwarp();
-          if (2 * lane < COLS) {
-            *reinterpret_cast<float2 *>(cols + 2 * lane) = make_float2(t0_next, t1_next);
-          }
-          __syncwarp();
+      // what this row's sums are kept times
+      float up = 1.0f;
+      bool lifted = false;
+      auto lower = [&]() {
+        const float down = up == 0x1p64f ? 0x1p-64f : 0x1p-117f;
+#pragma unroll
+        for (int j = 0; j < COLS; j += 2) {
+          mul_pair(sum[0][j], sum[0][j + 1], down);
+          mul_pair(sum[1][j], sum[1][j + 1], down);
         }
+        up = 1.0f;
+        lifted = false;
+      };
+      for (uint32_t kb = seg.k0; ok && kb < seg.k1; ++kb) {
+        const float s = s_next, t0 = t0_next, t1 = t1_next;
         if (kb + 1 < seg.k1) {
           rs += p.row_blocks;
           cs += p.col_blocks;
           load_scales();
+        }
+        // any column's scale stands for the block's where one covers 128 columns
+        const float col = __shfl_sync(0xFFFFFFFFu, t0, 0);
+        bool plain = __all_sync(0xFFFFFFFFu, in_range(s * up, t0, t1, lifted, p.lift_limit));
+        if (!plain) {
+          if (kb == seg.k0) {
+            lifted = true;
+            up = s != 0.0f && fabsf(s) < 0x1p-63f ? 0x1p117f : 0x1p64f;
+            plain = __all_sync(0xFFFFFFFFu, in_range(s * up, t0, t1, true, p.lift_limit));
+          }
+          if (!plain && lifted) {
+            lower();
+            plain = __all_sync(0xFFFFFFFFu, in_range(s, t0, t1, false, p.lift_limit));
+          }
+        }
+        const bool one = plain && p.col_shift != 0;
+        float *cols = col_buf + (kb & 1) * COLS;
+        if (!one) {
+          // through the staging tile, once the last stores have read it
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+          if (2 * lane < COLS) {
+            *reinterpret_cast<float2 *>(cols + 2 * lane) = make_float2(t0, t1);
+          }
+          __syncwarp();
         }
         ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.g.status,
                        kDevTimeoutEpilogue, p.g.wait_cycles);
@@ -647,18 +766,24 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
         const uint32_t taddr =
             tmem_base + ((quad * 32) << 16) + acc * C::kAccCols + first_col;
         const uint32_t done = bar_acc_empty + 8 * acc;
-        if (!tame) {
-          add_block<BN, kTwoSteps>(taddr, done, lane, cols, s, 0.0f, sum);
-        } else if (one_factor) {
-          add_block<BN, kOneFactor>(taddr, done, lane, cols, s, col, sum);
+        if (plain && !one) {
+          add_block<BN, false>(taddr, done, lane, cols, s * up, 0.0f, sum);
         } else {
-          add_block<BN, kColumnFactors>(taddr, done, lane, cols, s, 0.0f, sum);
+          if (!plain) {
+            constexpr uint32_t kLow = exponent_bits(-126), kHigh = exponent_bits(63);
+            const bool small = __all_sync(0xFFFFFFFFu, zero_or_between(s, kLow, kHigh) &&
+                                                           zero_or_between(t0, kLow, kHigh) &&
+                                                           zero_or_between(t1, kLow, kHigh));
+            scale_block<BN>(taddr, cols, s, small);
+          }
+          add_block<BN, true>(taddr, done, lane, cols, plain ? s * up : 1.0f, plain ? col : 1.0f, sum);
         }
         if (++acc == kAccBuffers) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
+      if (lifted) lower();
       // the next tile's first scales are on their way while this tile is stored
       Segment next{};
       more = walk.next(p, next);
@@ -1005,6 +1130,12 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
   p.col_shift = col_block == 128 ? 7 : 0;
   p.parts = plan->parts;
   p.counters = plan->counters;
+  // 2^l: largest scales whose blocks, lifted by 2^64, add up to less than 2^127.  A block's sums are at
+  // most 256 products of the types' largest values (448 < 2^9, 57344 < 2^16).
+  const double most = std::log2(256.0 * static_cast<double>(plan->k_blocks)) +
+                      (d.type_a == CCGLIB_B200_FLOAT8E5M2 ? 16.0 : 9.0) +
+                      (d.type_b == CCGLIB_B200_FLOAT8E5M2 ? 16.0 : 9.0);
+  p.lift_limit = static_cast<uint32_t>(127 + static_cast<int>(std::floor((63.0 - most) / 2))) << 23;
 
   const size_t pitch = ceil_div<size_t>(d.k, 16) * 16;
   CUtensorMap tm_a, tm_b, tm_c;
