@@ -409,6 +409,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
     if (*abort_flag) drain_loads<kStages>(bar_full, issued, stage, phase, p);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
+    wait_for_previous();  // its run time is not counted against the limits below
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
     bool ok = true;
     for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
@@ -569,6 +570,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     if (*abort_flag) drain_loads<kStages>(bar_full, issued, stage, phase, p);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
+    wait_for_previous();  // its run time is not counted against the limits below
     uint32_t stage = 0, phase = 0;
     for (uint32_t kb = kb0; kb < kb1; ++kb) {
       if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, kDevTimeoutMma, p.wait_cycles)) {

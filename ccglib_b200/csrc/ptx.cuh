@@ -108,7 +108,7 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
 
 // Wait until the kernels this launch depends on have finished and their writes are visible.  With
 // programmatic stream serialisation a CTA may be set up before that; nothing it does ahead of this may
-// touch global memory.
+// touch global memory (the status word included, so no bounded wait for data stands ahead of it).
 __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

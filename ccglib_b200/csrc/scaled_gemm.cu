@@ -616,6 +616,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_consta
       // Two warps take the blocks in turn, each its own accumulator buffer.  Issuing blocks while the tensor
       // core's short queue is full, so one warp alone leaves the tensor core idle while it waits for the
       // barriers of the next block (350 clocks of 1900); the other has done that when its turn comes.
+      wait_for_previous();  // its run time is not counted against the limits below
       const uint32_t acc = warp - 1;
       const uint64_t blocks = walk.blocks(p);
       uint32_t stage = acc, phase = 0, turn = 0;
