@@ -40,6 +40,12 @@ template <typename T> __host__ __device__ constexpr T ceil_div(T a, T b) { retur
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Two arrays share bytes.
+inline bool overlap(const void *p, size_t p_bytes, const void *q, size_t q_bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + q_bytes && b < a + p_bytes;
+}
+
 // Number of SMs of the current device (cached per device ordinal).
 int sm_count();
 

@@ -1498,6 +1498,15 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
     set_last_error("orthogonalize_run: input and output must be aligned to their elements");
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
+  // One launch takes the matrices of a batch in any order, each from its input to its output: only the same
+  // array in the same layout may be both.
+  const size_t values = d.batch * 2 * d.m * d.n;
+  const bool same = d_in == d_out && d.type_in == d.type_out && d.input_complex_axis == CCGLIB_B200_PLANAR;
+  if (!same && overlap(d_in, values * in_bytes, d_out, values * 2)) {
+    set_last_error("orthogonalize_run: input and output overlap (in place needs a planar input of the output's "
+                   "type, and the same address)");
+    return CCGLIB_B200_INVALID_ARGUMENT;
+  }
   int device = -1;
   CCGLIB_CUDA_TRY(cudaGetDevice(&device));
   if (device != plan->device) {

@@ -256,7 +256,8 @@ CCGLIB_B200_API int ccglib_b200_scaled_gemm_plan_tile(const ccglib_b200_scaled_g
  * planar [batch][2][M][N], float16 or bfloat16: an operand of the GEMM or input of the quantiser.
  * Norms are float64, sums float32; between the products X, S and P are float16 (rms error of the
  * result 1 to 2.5e-3 after 5 to 8 steps).  Results do not depend on timing.  In place (d_out ==
- * d_in) is allowed where input and output have the same type and the input is planar.
+ * d_in) is allowed where input and output have the same type and the input is planar; any other
+ * overlap of the two arrays is refused.
  * No counterpart in the reference.
  */
 typedef struct ccglib_b200_orthogonalize_desc {
