@@ -522,7 +522,6 @@ extern "C" int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *desc, c
     set_last_error("quantize_run: input and output must be 16-byte aligned, scales 4-byte aligned");
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
-  if (sm_count() <= 0) return CCGLIB_B200_CUDA_ERROR;
   QuantizeParams p{};
   p.in = d_in;
   p.out = static_cast<uint8_t *>(d_out);
@@ -534,6 +533,16 @@ extern "C" int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *desc, c
   p.blocks_k = ceil_div<size_t>(d.k, kBlockK);
   p.blocks_rows = ceil_div<size_t>(d.rows, d.block_rows);
   p.im_sign = d.conjugate ? -1.0f : 1.0f;
+  // blocks are read and written in any order
+  const size_t in_bytes = d.batch * 2 * d.rows * d.k * (d.type_in == CCGLIB_B200_FLOAT32 ? 4 : 2);
+  const size_t out_bytes = d.batch * 2 * d.rows * p.pitch;
+  const size_t scale_bytes = d.batch * p.blocks_k * p.blocks_rows * sizeof(float);
+  if (overlap(d_in, in_bytes, d_out, out_bytes) || overlap(d_in, in_bytes, d_scale, scale_bytes) ||
+      overlap(d_out, out_bytes, d_scale, scale_bytes)) {
+    set_last_error("quantize_run: input, output and scales must not overlap");
+    return CCGLIB_B200_INVALID_ARGUMENT;
+  }
+  if (sm_count() <= 0) return CCGLIB_B200_CUDA_ERROR;
   const bool il = d.input_complex_axis == CCGLIB_B200_INTERLEAVED;
   const bool e5m2 = d.type_out == CCGLIB_B200_FLOAT8E5M2;
   const bool col = d.input_mem_order == CCGLIB_B200_COL_MAJOR;

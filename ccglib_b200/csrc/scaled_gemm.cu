@@ -1080,6 +1080,16 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
     set_last_error("scaled_gemm_run: scales and C must be aligned to their elements");
     return CCGLIB_B200_INVALID_ARGUMENT;
   }
+  const size_t pitch = ceil_div<size_t>(d.k, 16) * 16;
+  const size_t c_bytes = d.batch * 2 * d.m * d.n * plan->out_bytes;
+  const size_t scale_bytes = d.batch * plan->k_blocks * sizeof(float);
+  if (overlap(d_c, c_bytes, d_a, d.batch * 2 * d.m * pitch) ||
+      overlap(d_c, c_bytes, d_b, d.batch * 2 * d.n * pitch) ||
+      overlap(d_c, c_bytes, d_a_scale, scale_bytes * ceil_div(d.m, d.a_block_rows)) ||
+      overlap(d_c, c_bytes, d_b_scale, scale_bytes * ceil_div(d.n, d.b_block_rows))) {
+    set_last_error("scaled_gemm_run: C overlaps an operand");
+    return CCGLIB_B200_INVALID_ARGUMENT;
+  }
   int device = -1;
   CCGLIB_CUDA_TRY(cudaGetDevice(&device));
   if (device != plan->device) {
@@ -1138,7 +1148,6 @@ extern "C" int ccglib_b200_scaled_gemm_run(ccglib_b200_scaled_gemm_plan *plan, c
                       (d.type_b == CCGLIB_B200_FLOAT8E5M2 ? 16.0 : 9.0);
   p.lift_limit = static_cast<uint32_t>(127 + static_cast<int>(std::floor((63.0 - most) / 2))) << 23;
 
-  const size_t pitch = ceil_div<size_t>(d.k, 16) * 16;
   CUtensorMap tm_a, tm_b, tm_c;
   int rc = make_map(&tm_a, plan->swapped ? d_b : d_a, d.k, plan->rows, 2 * d.batch, pitch,
                     pitch * plan->rows, 128, kBlockM, 2);

@@ -169,7 +169,7 @@ CCGLIB_B200_API int ccglib_b200_pack_run(size_t n, int direction, int input_comp
  *   amax = max(|re|, |im|) over its finite entries,  scale = max(amax / FMAX, 2^-126),
  *   q = x * (FMAX / amax), or x * 2^126 where scale is 2^-126, rounded to nearest even,
  * in float32; FMAX = 448 (e4m3) or 57344 (e5m2).  NaN stays NaN; an infinity becomes an infinity in e5m2 and NaN in e4m3.
- * Asynchronous on `stream`, one launch, no scratch.
+ * Asynchronous on `stream`, one launch, no scratch.  Input, output and scales must not overlap.
  *
  * The products of a backward pass of C = A x B^T are products of the same kind, over operands quantised
  * along their other axis: dA = dC x conj(B) contracts over n (rows = K of the col-major, conjugated B),
@@ -199,8 +199,9 @@ CCGLIB_B200_API int ccglib_b200_quantize_run(const ccglib_b200_quantize_desc *de
  * [batch][ceil(K / 128)][ceil(rows / block_rows)]: what ccglib_b200_quantize_run writes; for K a
  * multiple of 16 the planes are plain dense arrays.  A and B may have different fp8 types.
  * C in any of the four layouts of the GEMM above, float32, float16 or bfloat16; sums are float32 and
- * rounded once.  With beta = 0 C is not read.  Results do not depend on timing: the same call gives
- * the same bits.  No counterpart in the reference, whose fp8 GEMM takes unscaled values.
+ * rounded once.  With beta = 0 C is not read.  C must not overlap an operand or its scales.  Results
+ * do not depend on timing: the same call gives the same bits.  No counterpart in the reference, whose
+ * fp8 GEMM takes unscaled values.
  */
 typedef struct ccglib_b200_scaled_gemm_desc {
   size_t batch;
