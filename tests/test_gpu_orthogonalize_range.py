@@ -1,0 +1,62 @@
+"""Orthogonalisation of large wide matrices and of matrices with weak directions, against the iteration in
+64 bits with the bound of test_gpu_orthogonalize.py."""
+import numpy as np
+import pytest
+
+import block_util as bu
+from ccglib_b200 import capi
+from test_gpu_orthogonalize import CONVERGENT, QUINTIC, _check, _complex, _fro, _input, _iterate, _run
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = capi.FLOAT16, capi.BFLOAT16, capi.FLOAT32
+
+
+@pytest.mark.parametrize("m, n", [(600, 4000), (520, 1111), (1024, 1500), (4000, 600), (1111, 520)])
+@pytest.mark.parametrize("type_in, type_out, coefficients, steps", [(F32, F16, QUINTIC, 3), (BF16, BF16, CONVERGENT, 2)])
+def test_large(m, n, type_in, type_out, coefficients, steps):
+    """Wide ones contract over K-contiguous rows in S and read X with N as the other axis in the update."""
+    rng = np.random.default_rng(61)
+    x = _input(rng, 1, m, n, type_in)
+    plan = capi.OrthogonalizePlan(1, m, n, type_in, type_out, steps, coefficients)
+    _check(x, _run(plan, x, type_in, type_out, capi.PLANAR), steps, coefficients, type_out)
+
+
+def _with_singular_values(rng, m, n, s):
+    import torch
+
+    def basis(rows):
+        q, _ = np.linalg.qr(rng.standard_normal((rows, len(s))) + 1j * rng.standard_normal((rows, len(s))))
+        return q
+
+    x = (basis(m) * s) @ basis(n).conj().T
+    return torch.from_numpy(np.stack((x.real, x.imag))[None]).float()
+
+
+@pytest.mark.parametrize("steps, coefficients", [(5, QUINTIC), (8, QUINTIC), (8, CONVERGENT)])
+@pytest.mark.parametrize("m, n", [(24, 60), (60, 24), (130, 300), (300, 130)])
+def test_weak_directions(m, n, steps, coefficients):
+    """Singular values over five decades: within the bound, which grows with what the steps make of the
+    float16 roundings of X, and not worse than those roundings in directions that are strong enough."""
+    rng = np.random.default_rng(62)
+    r = min(m, n)
+    x = _with_singular_values(rng, m, n, np.geomspace(1, 1e-5, r))
+    plan = capi.OrthogonalizePlan(1, m, n, F32, F16, steps, coefficients)
+    got = _run(plan, x, F32, F16, capi.PLANAR)
+    xi, gi = _complex(x)[0], _complex(got)[0]
+    if m > n:
+        xi, gi = xi.T, gi.T
+    want, bound, _ = _iterate(xi, steps, coefficients)
+    assert _fro(gi - want) <= bound + 2.0 ** -11 * _fro(want) + 2.0 ** -24 * np.sqrt(want.size)
+
+
+@pytest.mark.parametrize("m, n", [(24, 60), (130, 300)])
+def test_rank_deficient(m, n):
+    """Directions that are not there stay out: rank 5, the rest rounding noise below float16's of X."""
+    rng = np.random.default_rng(63)
+    s = np.array([1, 0.8, 0.5, 0.3, 0.2])
+    x = _with_singular_values(rng, m, n, s)
+    plan = capi.OrthogonalizePlan(1, m, n, F32, F16, 4, CONVERGENT)
+    got = _complex(_run(plan, x, F32, F16, capi.PLANAR))[0]
+    want, bound, _ = _iterate(_complex(x)[0], 4, CONVERGENT)
+    assert _fro(got - want) <= bound + 2.0 ** -11 * _fro(want) + 2.0 ** -24 * np.sqrt(want.size)
