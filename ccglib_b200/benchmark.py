@@ -293,11 +293,8 @@ def bench_scaled_gemm(args) -> None:
     first = True
     for _ in range(args.nr_benchmarks):
         for M, N, K in zip(_sizes(args.m), _sizes(args.n), _sizes(args.k)):
-            pitch, kb = capi.operand_pitch(K), _ceil(K, 128)
-            a, b = (torch.full((args.b * 2 * rows * pitch,), 0x3C, dtype=torch.uint8, device="cuda")
-                    for rows in (M, N))
-            sa = torch.ones(args.b * kb * _ceil(M, args.a_block_rows), device="cuda")
-            sb = torch.ones(args.b * kb * _ceil(N, args.b_block_rows), device="cuda")
+            (a, sa), (b, sb) = (_quantised_noise(args.b, rows, K, code, block, stream) for rows, code, block in
+                                ((M, ta, args.a_block_rows), (N, tb, args.b_block_rows)))
             c = torch.empty(args.b * 2 * M * N * BITS[tout] // 8, dtype=torch.uint8, device="cuda")
             plan = capi.ScaledGemmPlan(args.b, M, N, K, ta, tb, tout, args.a_block_rows,
                                        args.b_block_rows)
@@ -307,7 +304,21 @@ def bench_scaled_gemm(args) -> None:
             first = False
             _report(args, (M, N, K), ms, 8e-9 * args.b * M * N * K / ms, "TOps/s",
                     watts)
-            del plan, a, b, c
+            del plan, a, b, sa, sb, c
+
+
+def _quantised_noise(batch, rows, k, code, block_rows, stream):
+    """Normally distributed samples as the quantiser leaves them (constant bytes would switch fewer
+    transistors, and large products run at what the power limit allows)."""
+    import torch
+
+    noise = torch.randn(batch * 2 * rows * k, dtype=torch.float16, device="cuda")
+    out = torch.empty(batch * 2 * rows * capi.operand_pitch(k), dtype=torch.uint8, device="cuda")
+    scale = torch.empty(batch * _ceil(k, 128) * _ceil(rows, block_rows), device="cuda")
+    capi.quantize(batch, rows, k, capi.FLOAT16, code, noise.data_ptr(), out.data_ptr(), scale.data_ptr(),
+                  stream, block_rows=block_rows)
+    torch.cuda.synchronize()  # the noise is released here
+    return out, scale
 
 
 def bench_orthogonalize(args) -> None:
