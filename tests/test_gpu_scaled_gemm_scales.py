@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 E4M3, E5M2, F32 = capi.FLOAT8E4M3, capi.FLOAT8E5M2, capi.FLOAT32
 K = 256  # two blocks: two roundings of at most 2^-150 each where the sums are subnormal
-# tiles of 64 columns, of 64 and of 16 columns with B or A as the row side, of 128 columns
+# tiles of 64 columns, of 64 and of 16 columns with B or A as the row side (128 columns: at the end)
 SHAPES = [(130, 140), (40, 200), (200, 40), (9, 150), (150, 9), (200, 260)]
 FORMS = [(1, 1), (1, 128), (128, 1), (128, 128)]
 
@@ -156,3 +156,25 @@ def test_silent_and_faint_rows_of_the_quantiser():
     sa, sb = (t.cpu() for t in s)
     assert (sa == 2.0 ** -126).any() and (sa > 2.0 ** -126).any()
     _compare(m, n, a, sa, 1, b, sb, 1, E4M3)
+
+
+@pytest.mark.parametrize("runs", ["0", "1"])
+def test_wide_tiles(runs, monkeypatch):
+    """All of the above on tiles of 128 columns."""
+    monkeypatch.setenv("CCGLIB_B200_SCALED_BN", "128")
+    monkeypatch.setenv("CCGLIB_B200_SCALED_RUNS", runs)
+    m, n = 200, 260
+    assert capi.ScaledGemmPlan(1, m, n, K, E4M3, E4M3, F32, 1, 1).tile["bn"] == 128
+    for test, names in ((test_range_of_scales, "code, top, ea, eb"), (test_infinite_sums_stay_infinite, "ea, eb"),
+                        (test_scales_that_change_along_k, "code"), (test_scales_that_change_along_k, "ea, eb")):
+        for mark in test.pytestmark:
+            if mark.args[0] != names:
+                continue
+            for values in mark.args[1]:
+                values = values if isinstance(values, tuple) else (values,)
+                kw = dict(zip(names.split(", "), values))
+                if test is test_scales_that_change_along_k:
+                    kw = {"code": E4M3, "ea": (-126, -3, -126, 40, -126), "eb": (-3, 12, -126, -20, -3), **kw}
+                test(m, n, **kw)
+    test_zero_sums_stay_zero(m, n)
+    test_silent_and_faint_rows_of_the_quantiser()
