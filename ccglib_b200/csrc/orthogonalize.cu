@@ -1,28 +1,29 @@
 // Orthogonalisation of complex matrices by Newton-Schulz products.
 //
-//   X <- X / ||X||_F;   `steps` times:  S = X X^H,  P = b S + c S S,  X <- a X + P X
+//   X <- X / ||X||_F;   `steps` times:  S = X X^H,  P = a I + b S + c S S,  X <- P X
 //
-// (M <= N; for M > N the same on X^T, i.e. S = X^T conj(X) and X <- a X + X P^T).  Every step keeps the
+// (M <= N; for M > N the same on X^T, i.e. S = X^T conj(X) and X <- X P^T).  Every step keeps the
 // singular vectors and maps each singular value s to s (a + b s^2 + c s^4).
 //
 // Three launches per step and nothing else, float32 sums on the tensor cores (kind::f16).  S and P are
 // Hermitian: only tiles on and above the diagonal are computed, each stored a second time as its
 // mirror image.  X is never transposed: where a product contracts over rows, its operand is read with
-// the rows as K (the MN-major form of the shared-memory descriptor).  b S and a X are added in the
-// epilogue; the last update writes the caller's type and layout.
-// The launches are programmatic: a product's CTAs set up while the one before it drains.
+// the rows as K (the MN-major form of the shared-memory descriptor).  The Gram product stores S + b/2c I,
+// whose square is P but for a factor and a multiple of I; the last update writes the caller's type and
+// layout.  The launches are programmatic: a product's CTAs set up while the one before it drains.
 //
-// Measured: 8 x 4096 x 1024, eight steps, 3.50 to 3.68 ms (0.97 to 1.02 PFLOP/s of the operations that the
-// Hermitian halves need, 1.3 PFLOP/s in the large products, power-capped); 1024 x 1024, five steps, 182 us
-// (a product of 1024^3 takes about 11 us: its operands' way from L2 into 144 SMs and two latencies).
+// X, S and P are states of the iteration and are kept as pairs of float16, the rounded value and what the
+// rounding leaves (X times a power of two near sqrt(long side), S and P times powers of two that keep them
+// inside float16): about 20 bits.  A product takes its K three times, low x high, high x low and high x
+// high, into the same float32 sums.  What is lost in the end is the rounding of the output (relative
+// error 2.1e-4 float16, 1.7e-3 bfloat16).  Single float16 iterates take a third of the multiplications, but
+// a step's roundings do not decay, those that turn the singular vectors least of all: they ended at 7e-4
+// after eight steps that converge and at 1.4 to 3.8e-3 after 5 to 8 of the steep quintic.  Leaving out one
+// of the low halves (of X in S, of S, of P) still ends at 5e-4 to 3e-3.
 //
-// Between products X, S and P are float16.  All three are bounded (singular values stay near or below
-// one), X is kept times a power of two near sqrt(long side) so that its entries are near one, and float16
-// keeps eleven bits where bfloat16, the usual 16-bit choice, keeps eight.  A step is computed from the
-// rounded X throughout, a X included: an error of X then goes through the map like X itself, which
-// contracts it.  (A float32 copy of X for the a X term alone adds a times the rounding of X instead; it
-// took the error of eight steps of the steep quintic from 2.1e-3 to 3.7e-3.)  Error of the result, rms:
-// 0.7e-3 after eight steps that converge, 1.2 to 2.5e-3 after 5 to 8 of the quintic.
+// Measured: 8 x 4096 x 1024, eight steps, 9.8 ms (1.09 PFLOP/s in the three passes over K, power-capped);
+// 1024 x 1024, five steps, 344 us (23 us a product of 1024^3 in three passes: operands on their way from L2
+// into 144 SMs, and two latencies).  Single float16: 3.5 ms and 182 us.
 #include <cmath>
 #include <cstdlib>
 #include <new>
@@ -36,17 +37,20 @@ constexpr int kOrthK = 64;          // float16 values of K per stage: one 128-by
 constexpr int kOrthBox = 32 * 64;   // staging box: 32 rows x 32 float16
 constexpr int kOrthStaging = 4 * 4 * kOrthBox;  // per epilogue warp: Re, Im and their mirror images
 
+// The products are taken over K three times: low halves of A by high halves of B, high by low, high by high.
+// (low by low is below the last bit of either.)
+constexpr uint32_t kPasses = 3;
+
 struct OrthParams {
   uint32_t m, n;        // result: m x n per batch item
-  uint32_t k_blocks;
+  uint32_t k_blocks;    // of one pass
   uint32_t tiles_m, tiles_n, group_n;
   uint32_t per_batch, num_tiles;
   uint32_t hermitian;   // compute tiles that touch or lie above the diagonal, store their mirror image
   uint32_t conj_b;      // A x B^H instead of A x B^T
-  float alpha, beta, gain;  // result = gain * (alpha * sum + beta * c0)
-  const __half *c0;     // [batch][2][m][c0_pitch] (null: none)
-  uint32_t c0_pitch;
-  uint32_t bf16;        // the result is bfloat16
+  float alpha, diag;    // result = alpha * sum + diag * I
+  uint32_t pair;        // the result is a pair of float16; else float16 or bfloat16
+  uint32_t bf16;
   uint32_t boxes;       // the result leaves by TMA; else value by value to `out` [batch][2][m][n_out]
   uint16_t *out;
   uint32_t n_out;
@@ -116,52 +120,17 @@ __device__ __forceinline__ void st_shared_u16(uint32_t addr, uint16_t v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
 }
 
-// c0 of this lane's row m, 32 columns from n0: Re in c[0..3], Im in c[4..7].  Loaded well before it is used.
-__device__ __forceinline__ void load_c0(const OrthParams &p, uint32_t b, uint32_t m, uint32_t n0,
-                                        uint4 (&c)[8]) {
-  if (p.c0 == nullptr) return;
-  const size_t plane = static_cast<size_t>(p.m) * p.c0_pitch;
-  const __half *src = p.c0 + static_cast<size_t>(b) * 2 * plane + static_cast<size_t>(m) * p.c0_pitch + n0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool inside = m < p.m && n0 + 8 * j < p.c0_pitch;  // the pitch is a multiple of eight
-    c[j] = inside ? *reinterpret_cast<const uint4 *>(src + 8 * j) : make_uint4(0, 0, 0, 0);
-    c[4 + j] = inside ? *reinterpret_cast<const uint4 *>(src + plane + 8 * j) : make_uint4(0, 0, 0, 0);
-  }
-}
-
-// 32 rows x 32 columns (one row per lane, from m0; columns from n0) of one batch item; c as load_c0 left it.
+// 32 rows x 32 columns (one row per lane, from m0; columns from n0) of one batch item: the sums -> the result.
 __device__ __forceinline__ void orth_store(const OrthParams &p, const CUtensorMap *tm_c,
                                            uint32_t staging, uint32_t lane, uint32_t b, uint32_t m0,
-                                           uint32_t n0, const uint4 (&c)[8], float (&re)[32],
-                                           float (&im)[32]) {
+                                           uint32_t n0, float (&re)[32], float (&im)[32]) {
   const uint32_t m = m0 + lane;
+  const bool diagonal = p.hermitian && n0 == m0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
     re[j] *= p.alpha;
     im[j] *= p.alpha;
-  }
-  if (p.c0 != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t rw[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
-      const uint32_t iw[4] = {c[4 + j].x, c[4 + j].y, c[4 + j].z, c[4 + j].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 rv = __half22float2(*reinterpret_cast<const __half2 *>(&rw[e]));
-        const float2 iv = __half22float2(*reinterpret_cast<const __half2 *>(&iw[e]));
-        const int at = 8 * j + 2 * e;
-        re[at] = fmaf(p.beta, rv.x, re[at]);
-        re[at + 1] = fmaf(p.beta, rv.y, re[at + 1]);
-        im[at] = fmaf(p.beta, iv.x, im[at]);
-        im[at + 1] = fmaf(p.beta, iv.y, im[at + 1]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    re[j] *= p.gain;
-    im[j] *= p.gain;
+    if (diagonal && j == static_cast<int>(lane)) re[j] += p.diag;
   }
   if (!p.boxes) {
     if (m < p.m) {
@@ -177,80 +146,102 @@ __device__ __forceinline__ void orth_store(const OrthParams &p, const CUtensorMa
     }
     return;
   }
-  const bool diagonal = p.hermitian && n0 == m0;
-  // 16-byte piece j of row r of a box stands at j ^ ((r >> 1) & 3): the 64-byte swizzle
-  if (lane == 0) bulk_wait_group_read<0>();
-  __syncwarp();
+  const uint32_t halves = p.pair ? 2 : 1;
   const uint32_t row = staging + lane * 64;
+#pragma unroll 1
+  for (uint32_t half = 0; half < halves; ++half) {
+    // 16-byte piece j of row r of a box stands at j ^ ((r >> 1) & 3): the 64-byte swizzle
+    if (lane == 0) bulk_wait_group_read<0>();
+    __syncwarp();
+    uint32_t r[16], i[16];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t at = row + ((j ^ ((lane >> 1) & 3)) << 4);
-    const int e = 8 * j;
-    st_shared_v4(at, pack_half(re[e], re[e + 1], p.bf16), pack_half(re[e + 2], re[e + 3], p.bf16),
-                 pack_half(re[e + 4], re[e + 5], p.bf16), pack_half(re[e + 6], re[e + 7], p.bf16));
-    st_shared_v4(at + kOrthBox, pack_half(im[e], im[e + 1], p.bf16),
-                 pack_half(im[e + 2], im[e + 3], p.bf16), pack_half(im[e + 4], im[e + 5], p.bf16),
-                 pack_half(im[e + 6], im[e + 7], p.bf16));
-  }
-  if (p.hermitian) {
-    // the mirror image: row n0 + j, this lane's column.  On the diagonal block it goes over the
-    // rows just written: below the diagonal, and zero imaginary parts on it.
-    const uint32_t mirror = diagonal ? staging : staging + 2 * kOrthBox;
-    if (diagonal) __syncwarp();
+    for (int j = 0; j < 16; ++j) {
+      r[j] = pack_half(re[2 * j], re[2 * j + 1], p.bf16);
+      i[j] = pack_half(im[2 * j], im[2 * j + 1], p.bf16);
+    }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (!diagonal || j > static_cast<int>(lane)) {
-        const uint32_t at = mirror + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
-        st_shared_u16(at, __half_as_ushort(__float2half_rn(re[j])));
-        st_shared_u16(at + kOrthBox, __half_as_ushort(__float2half_rn(-im[j])));
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = row + ((j ^ ((lane >> 1) & 3)) << 4);
+      st_shared_v4(at, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+      st_shared_v4(at + kOrthBox, i[4 * j], i[4 * j + 1], i[4 * j + 2], i[4 * j + 3]);
+    }
+    if (p.hermitian) {
+      // the mirror image: row n0 + j, this lane's column.  On the diagonal block it goes over the
+      // rows just written: below the diagonal, and zero imaginary parts on it.
+      const uint32_t mirror = diagonal ? staging : staging + 2 * kOrthBox;
+      if (diagonal) __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        if (!diagonal || j > static_cast<int>(lane)) {
+          const uint32_t at = mirror + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2;
+          const int shift = 16 * (j & 1);
+          st_shared_u16(at, static_cast<uint16_t>(r[j / 2] >> shift));
+          st_shared_u16(at + kOrthBox, static_cast<uint16_t>((i[j / 2] >> shift) ^ 0x8000u));
+        }
+      }
+      if (diagonal) {
+        st_shared_u16(staging + kOrthBox + lane * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4) +
+                          (lane & 7) * 2, 0);
       }
     }
-    if (diagonal) {
-      st_shared_u16(staging + kOrthBox + lane * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4) +
-                        (lane & 7) * 2, 0);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      const int32_t z = static_cast<int32_t>(2 * (halves * b + half));
+      const int32_t x = static_cast<int32_t>(n0 * 2), y = static_cast<int32_t>(m0);
+      if (m0 < p.m) {
+        tma_store_3d(tm_c, staging, x, y, z);
+        tma_store_3d(tm_c, staging + kOrthBox, x, y, z + 1);
+        if (p.hermitian && !diagonal && n0 < p.m) {
+          const int32_t tx = static_cast<int32_t>(m0 * 2), ty = static_cast<int32_t>(n0);
+          tma_store_3d(tm_c, staging + 2 * kOrthBox, tx, ty, z);
+          tma_store_3d(tm_c, staging + 3 * kOrthBox, tx, ty, z + 1);
+        }
+      }
+      bulk_commit_group();
     }
-  }
-  fence_proxy_async_smem();
-  __syncwarp();
-  if (lane == 0) {
-    const int32_t z = static_cast<int32_t>(2 * b);
-    const int32_t x = static_cast<int32_t>(n0 * 2), y = static_cast<int32_t>(m0);
-    if (m0 < p.m) {
-      tma_store_3d(tm_c, staging, x, y, z);
-      tma_store_3d(tm_c, staging + kOrthBox, x, y, z + 1);
-      if (p.hermitian && !diagonal && n0 < p.m) {
-        const int32_t tx = static_cast<int32_t>(m0 * 2), ty = static_cast<int32_t>(n0);
-        tma_store_3d(tm_c, staging + 2 * kOrthBox, tx, ty, z);
-        tma_store_3d(tm_c, staging + 3 * kOrthBox, tx, ty, z + 1);
+    if (half + 1 < halves) {  // what the rounding leaves (pairs are float16)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 hr = __half22float2(*reinterpret_cast<const __half2 *>(&r[j]));
+        const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&i[j]));
+        re[2 * j] -= hr.x;
+        re[2 * j + 1] -= hr.y;
+        im[2 * j] -= hi.x;
+        im[2 * j + 1] -= hi.y;
       }
     }
-    bulk_commit_group();
   }
 }
 
 constexpr uint32_t kAtom = 2 * kOrthK * 128;  // 64 values along M or N of both planes, MN-major
 
-// Loads of one stage: block kb of K of tile t.
+// Loads of one stage: block kb (of all passes) of tile t.
 template <int BN, bool A_MN, bool B_MN>
-__device__ __forceinline__ void load_stage(const CUtensorMap *tm_a, const CUtensorMap *tm_b,
-                                           const TileCoord &t, uint32_t kb, uint32_t dst, uint32_t full) {
+__device__ __forceinline__ void load_stage(const OrthParams &p, const CUtensorMap *tm_a,
+                                           const CUtensorMap *tm_b, const TileCoord &t, uint32_t kb,
+                                           uint32_t dst, uint32_t full) {
   using C = OrthCfg<BN>;
-  const int32_t k = static_cast<int32_t>(kb * kOrthK), z = static_cast<int32_t>(2 * t.b);
+  const uint32_t pass = kb / p.k_blocks;
+  const int32_t k = static_cast<int32_t>((kb - pass * p.k_blocks) * kOrthK);
+  // the planes of a batch item: high Re, Im, low Re, Im
+  const int32_t z_a = static_cast<int32_t>(4 * t.b + (pass == 0 ? 2 : 0));
+  const int32_t z_b = static_cast<int32_t>(4 * t.b + (pass == 1 ? 2 : 0));
   const int32_t m0 = static_cast<int32_t>(t.mt * kBlockM), n0 = static_cast<int32_t>(t.nt * BN);
   mbar_arrive_expect_tx(full, C::kStageBytes);
   if constexpr (A_MN) {
 #pragma unroll
-    for (int i = 0; i < kBlockM / 64; ++i) tma_load_3d(dst + i * kAtom, tm_a, (m0 + 64 * i) * 2, k, z, full);
+    for (int i = 0; i < kBlockM / 64; ++i) tma_load_3d(dst + i * kAtom, tm_a, (m0 + 64 * i) * 2, k, z_a, full);
   } else {
-    tma_load_3d(dst, tm_a, k * 2, m0, z, full);
+    tma_load_3d(dst, tm_a, k * 2, m0, z_a, full);
   }
   if constexpr (B_MN) {
 #pragma unroll
     for (int i = 0; i < BN / 64; ++i) {
-      tma_load_3d(dst + C::kABytes + i * kAtom, tm_b, (n0 + 64 * i) * 2, k, z, full);
+      tma_load_3d(dst + C::kABytes + i * kAtom, tm_b, (n0 + 64 * i) * 2, k, z_b, full);
     }
   } else {
-    tma_load_3d(dst + C::kABytes, tm_b, k * 2, n0, z, full);
+    tma_load_3d(dst + C::kABytes, tm_b, k * 2, n0, z_b, full);
   }
 }
 
@@ -333,8 +324,9 @@ __device__ __forceinline__ void drain_loads(uint32_t bar_full, uint32_t issued, 
   }
 }
 
-// result = gain * (alpha * A x op(B)^T + beta * c0), tiles of 128 x BN.  An operand that is MN-major is
-// stored [K][M or N]; the others are stored [M or N][K].  Roles as in cgemm_tcgen05_kernel.
+// result = alpha * A x op(B)^T + diag * I, tiles of 128 x BN, of operands that are pairs of float16.  An
+// operand that is MN-major is stored [K][M or N]; the others are stored [M or N][K].  Roles as in
+// cgemm_tcgen05_kernel.
 template <int BN, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kThreads, 1)
 orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
@@ -388,14 +380,14 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
     bool ok = true;
     for (uint32_t tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
       const TileCoord t = orth_tile<BN>(p, tile);
-      for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
+      for (uint32_t kb = 0; kb < kPasses * p.k_blocks; ++kb) {
         if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, kDevTimeoutProducer,
                        p.wait_cycles)) {
           ok = false;
           break;
         }
         if (lane == 0) {
-          load_stage<BN, A_MN, B_MN>(&tm_a, &tm_b, t, kb, smem_base + stage * C::kStageBytes,
+          load_stage<BN, A_MN, B_MN>(p, &tm_a, &tm_b, t, kb, smem_base + stage * C::kStageBytes,
                                      bar_full + 8 * stage);
         }
         __syncwarp();
@@ -419,7 +411,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
       }
       tc_fence_after();
       const uint32_t d = tmem_base + acc * C::kAccCols;
-      for (uint32_t kb = 0; kb < p.k_blocks; ++kb) {
+      for (uint32_t kb = 0; kb < kPasses * p.k_blocks; ++kb) {
         if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, kDevTimeoutMma,
                        p.wait_cycles)) {
           ok = false;
@@ -429,7 +421,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
         if (lane == 0) {
           issue_stage<BN, A_MN, B_MN>(smem_base + stage * C::kStageBytes, d, p.conj_b != 0, kb != 0);
           tc_commit(bar_empty + 8 * stage);
-          if (kb + 1 == p.k_blocks) tc_commit(bar_acc_full + 8 * acc);
+          if (kb + 1 == kPasses * p.k_blocks) tc_commit(bar_acc_full + 8 * acc);
         }
         __syncwarp();
         if (++stage == kStages) {
@@ -451,8 +443,6 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
     for (uint32_t tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x) {
       const TileCoord t = orth_tile<BN>(p, tile);
       const uint32_t m0 = t.mt * kBlockM + quad * 32;
-      uint4 c_next[8];  // while the tile is multiplied
-      load_c0(p, t.b, m0 + lane, t.nt * BN, c_next);
       bool ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.status,
                           kDevTimeoutEpilogue, p.wait_cycles);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
@@ -462,14 +452,10 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
       for (uint32_t c0 = 0; c0 < BN; c0 += 32) {
         const uint32_t n0 = t.nt * BN + c0;
         if (n0 >= p.n) break;
-        uint4 c_now[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c_now[j] = c_next[j];
-        if (c0 + 32 < BN) load_c0(p, t.b, m0 + lane, n0 + 32, c_next);
         if (m0 >= p.m || (p.hermitian && n0 < m0)) continue;  // comes from the mirror image
         float re[32], im[32];
         read_chunk<BN>(taddr + c0, p.conj_b != 0, re, im);
-        orth_store(p, &tm_c, staging, lane, t.b, m0, n0, c_now, re, im);
+        orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
       }
       tc_fence_before();
       __syncwarp();
@@ -544,9 +530,8 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   let_next_start();
 
   const TileCoord t = orth_tile<BN>(p, cluster_id_x());
-  const uint32_t kb0 = p.k_blocks * rank / SPLIT, kb1 = p.k_blocks * (rank + 1) / SPLIT;
+  const uint32_t kb0 = kPasses * p.k_blocks * rank / SPLIT, kb1 = kPasses * p.k_blocks * (rank + 1) / SPLIT;
   bool done = false;  // epilogue warps: this CTA's sums are complete
-  uint4 c_next[8];
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     wait_for_previous();
@@ -557,7 +542,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         break;
       }
       if (lane == 0) {
-        load_stage<BN, A_MN, B_MN>(&tm_a, &tm_b, t, kb, smem_base + stage * C::kStageBytes,
+        load_stage<BN, A_MN, B_MN>(p, &tm_a, &tm_b, t, kb, smem_base + stage * C::kStageBytes,
                                    bar_full + 8 * stage);
       }
       __syncwarp();
@@ -590,7 +575,6 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     }
   } else {
     wait_for_previous();
-    load_c0(p, t.b, t.mt * kBlockM + (warp & 3) * 32 + lane, t.nt * BN + rank * kChunks * 32, c_next);
     done = mbar_wait(bar_acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue, p.wait_cycles);
     done = __all_sync(0xFFFFFFFFu, done);
   }
@@ -635,10 +619,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll 1
     for (uint32_t c = 0; c < kChunks; ++c) {
       const uint32_t col = (rank * kChunks + c) * 32, n0 = t.nt * BN + col;
-      if (n0 >= p.n || m0 >= p.m || (p.hermitian && n0 < m0)) {
-        if (c + 1 < kChunks) load_c0(p, t.b, m0 + lane, n0 + 32, c_next);
-        continue;
-      }
+      if (n0 >= p.n || m0 >= p.m || (p.hermitian && n0 < m0)) continue;
       float re[32], im[32];
       read_chunk<BN>(taddr + col, p.conj_b != 0, re, im);
 #pragma unroll 1
@@ -657,8 +638,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           }
         }
       }
-      orth_store(p, &tm_c, staging, lane, t.b, m0, n0, c_next, re, im);
-      if (c + 1 < kChunks) load_c0(p, t.b, m0 + lane, n0 + 32, c_next);
+      orth_store(p, &tm_c, staging, lane, t.b, m0, n0, re, im);
     }
     if (lane == 0) bulk_wait_group<0>();
   }
@@ -695,14 +675,16 @@ int orth_smem(int bn) { return bn == 128 ? OrthCfg<128>::kSmemBytes : OrthCfg<64
 struct ProductShape {
   int bn, split;
   size_t per_batch;
+  double clocks;  // estimated
 };
 
-// Estimated clocks: a block of K costs what its bytes take through the SM's port to L2 (64 KiB resp. 48 KiB,
-// 128 resp. 64 columns), a tile its epilogue, an exchange of partial sums 60 per column.
+// Estimated clocks: a block of K (of three passes) costs what its bytes take through the SM's port to L2 (64 KiB resp. 48 KiB,
+// 128 resp. 64 columns), a tile its epilogue (of mostly Hermitian blocks 100 per column, else 60), an
+// exchange of partial sums 60 per column.
 ProductShape pick_shape(size_t batch, size_t m, size_t n, size_t k, bool hermitian, size_t sms) {
-  ProductShape best{0, 1, 0};
+  ProductShape best{0, 1, 0, 0.0};
   double least = 0.0;
-  const size_t k_blocks = ceil_div<size_t>(k, kOrthK);
+  const size_t k_blocks = kPasses * ceil_div<size_t>(k, kOrthK);
   const char *env = std::getenv("CCGLIB_B200_ORTH_SPLIT");  // 1, 2 or 4: by hand, where it fits
   const int forced = env != nullptr ? std::atoi(env) : 0;
   for (int bn : {128, 64}) {
@@ -715,11 +697,12 @@ ProductShape pick_shape(size_t batch, size_t m, size_t n, size_t k, bool hermiti
       if (split > 1 && (ctas > (split == 4 ? sms * 86 / 100 : sms) || k_blocks < static_cast<size_t>(split) || bn < 32 * split)) continue;
       const double blocks = static_cast<double>(ceil_div<size_t>(k_blocks, split));
       double cost = static_cast<double>(ceil_div(ctas, sms)) *
-                        (blocks * (bn == 128 ? 1250.0 : 950.0) + 25.0 * bn / split) +
+                        (blocks * (bn == 128 ? 1250.0 : 950.0) + (hermitian ? 100.0 : 60.0) * bn / split) +
                     (split > 1 ? 60.0 * bn : 0.0);
+      const double clocks = cost;
       if (forced != 0 && split == forced) cost *= 1e-3;
       if (best.bn == 0 || cost < least) {
-        best = {bn, split, tiles};
+        best = {bn, split, tiles, clocks};
         least = cost;
       }
     }
@@ -802,12 +785,19 @@ struct FirstParams {
   const void *in;      // the caller's matrices, rows x cols
   const double *sums;  // [batch][chunks]
   size_t chunks, batch, rows, cols;
-  __half *x;           // [batch][2][rows][pitch], zeros behind cols
+  __half *x;           // [batch][high Re, Im, low Re, Im][rows][pitch], zeros behind cols
   size_t pitch;
   float scale;
 };
 
 constexpr size_t kFirstChunk = 8192;  // complex values (padded rows) one CTA converts
+
+// x -> its float16 and what the rounding leaves.
+__device__ __forceinline__ void split_pair(float v0, float v1, __half2 &high, __half2 &low) {
+  high = __floats2half2_rn(v0, v1);
+  const float2 h = __half22float2(high);
+  low = __floats2half2_rn(v0 - h.x, v1 - h.y);
+}
 
 // X0 = scale * input / norm.  VEC: rows need no padding, the planes are converted as they lie.
 template <typename T, bool IL, bool VEC>
@@ -830,7 +820,7 @@ __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
     const double half = factor < 1e-30 ? 1e-25 : factor > 1e30 ? 1e25 : 1.0;
     const float f0 = static_cast<float>(half), f1 = static_cast<float>(factor / half);
     const T *in = static_cast<const T *>(p.in) + b * 2 * p.rows * p.cols;
-    __half *x = p.x + b * 2 * plane;
+    __half *x = p.x + b * 4 * plane;
     const size_t first = (item - b * per_batch) * kFirstChunk;
     const size_t end = min(plane, first + kFirstChunk);
     if constexpr (VEC) {
@@ -839,7 +829,7 @@ __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
         float v[2][8];
         load8(IL ? in + 2 * i : in + i, v[0]);
         load8(IL ? in + 2 * i + 8 : in + i + plane, v[1]);
-        __half2 re[4], im[4];
+        __half2 re[4], im[4], re_low[4], im_low[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           // interleaved: pairs 2j, 2j + 1 of the 16 values
@@ -847,11 +837,13 @@ __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
           const float i0 = IL ? v[j / 2][(4 * j + 1) & 7] : v[1][2 * j];
           const float r1 = IL ? v[j / 2][(4 * j + 2) & 7] : v[0][2 * j + 1];
           const float i1 = IL ? v[j / 2][(4 * j + 3) & 7] : v[1][2 * j + 1];
-          re[j] = __floats2half2_rn(r0 * f0 * f1, r1 * f0 * f1);
-          im[j] = __floats2half2_rn(i0 * f0 * f1, i1 * f0 * f1);
+          split_pair(r0 * f0 * f1, r1 * f0 * f1, re[j], re_low[j]);
+          split_pair(i0 * f0 * f1, i1 * f0 * f1, im[j], im_low[j]);
         }
         *reinterpret_cast<uint4 *>(x + i) = *reinterpret_cast<const uint4 *>(re);
         *reinterpret_cast<uint4 *>(x + i + plane) = *reinterpret_cast<const uint4 *>(im);
+        *reinterpret_cast<uint4 *>(x + i + 2 * plane) = *reinterpret_cast<const uint4 *>(re_low);
+        *reinterpret_cast<uint4 *>(x + i + 3 * plane) = *reinterpret_cast<const uint4 *>(im_low);
       }
     } else {
 #pragma unroll 4
@@ -863,8 +855,12 @@ __global__ void __launch_bounds__(256) first_kernel(const FirstParams p) {
           re = as_float(IL ? in[2 * s] : in[s]);
           im = as_float(IL ? in[2 * s + 1] : in[s + p.rows * p.cols]);
         }
-        x[i] = __float2half_rn(re * f0 * f1);
-        x[i + plane] = __float2half_rn(im * f0 * f1);
+        __half2 high, low;
+        split_pair(re * f0 * f1, im * f0 * f1, high, low);
+        x[i] = __low2half(high);
+        x[i + plane] = __high2half(high);
+        x[i + 2 * plane] = __low2half(low);
+        x[i + 3 * plane] = __high2half(low);
       }
     }
     __syncthreads();
@@ -1189,12 +1185,23 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const SmallParams 
 
 using namespace ccglib_b200;
 
+// How P = a I + b S + c S^2 is computed:
+//   kSquare   c (S + h I)^2 + (a - c h^2) I with h = b / 2c, one Hermitian square of what the Gram product
+//             stores (h on its diagonal);
+//   kLinear   c = 0: the Gram product stores it;
+//   kProduct  (c S + b I) S + a I, the Gram product computed twice, for b so much larger than c that the
+//             square would cancel: c h^2 more than eight times the largest coefficient.
+enum PolyForm { kSquare, kLinear, kProduct };
+
 struct ccglib_b200_orthogonalize_plan {
   ccglib_b200_orthogonalize_desc desc;
   size_t n, l;          // short and long side
   size_t n_p, cols_p;   // row pitches of S and P, and of X: multiples of eight
   bool tall;            // m > n
-  float scale;          // power of two near sqrt(long side)
+  float scale;          // power of two near sqrt(long side): X is kept times this
+  PolyForm form;
+  float shift;          // kSquare: b / 2c
+  float s_scale, t_scale, p_scale;  // powers of two that S (+ shift I), T and P are kept times
   ProductShape gram, poly, update;
   uint32_t small;       // > 0: the whole iteration in one launch, so many CTAs per matrix
   size_t chunks;
@@ -1203,11 +1210,11 @@ struct ccglib_b200_orthogonalize_plan {
   unsigned *status;
   void *scratch;
   size_t scratch_bytes;
-  __half *x[2], *s, *p;  // [batch][2][m][cols_p], [batch][2][n][n_p]
+  __half *x[2], *s, *t, *p;  // [batch][4][m][cols_p], [batch][4][n][n_p]: high Re, Im, low Re, Im
   double *sums;
   // tensor maps of the workspace: X as either operand of the Gram product and as the operand of the
-  // update, S as either operand, P as the operand of the update, and all three as results
-  CUtensorMap gram_a[2], gram_b[2], update_x[2], x_out[2], s_a, s_b, update_p, s_out, p_out;
+  // update, T (or S) and S as the operands of their product, P as the operand of the update, and all as results
+  CUtensorMap gram_a[2], gram_b[2], update_x[2], x_out[2], poly_a, poly_b, update_p, s_out, t_out, p_out;
 };
 
 namespace {
@@ -1226,23 +1233,23 @@ struct Product {
   size_t m, n;  // n: columns written
   ProductShape shape;
   bool hermitian, conj;
-  float alpha, beta, gain;
-  const __half *c0;
-  size_t c0_pitch;
-  void *out;
-  size_t out_pitch;
-  bool boxes, bf16;
+  float alpha, diag;
+  bool pair;
+  // what the last product has of its own
+  void *out = nullptr;
+  size_t out_pitch = 0;
+  bool boxes = true, bf16 = false;
 };
 
 // Map of an operand whose tile has `tile` rows of the result's.
 int operand_map(CUtensorMap *tm, const Operand &o, size_t batch, int tile) {
   const uint32_t box = o.by_rows ? kOrthK : static_cast<uint32_t>(tile);
-  return make_map(tm, o.data, o.cols * 2, o.rows, 2 * batch, o.pitch * 2, o.rows * o.pitch * 2, 128, box, 2);
+  return make_map(tm, o.data, o.cols * 2, o.rows, 4 * batch, o.pitch * 2, o.rows * o.pitch * 2, 128, box, 2);
 }
 
 // Map of a result: planes of rows x cols 16-bit values.
-int result_map(CUtensorMap *tm, const void *out, size_t batch, size_t rows, size_t cols) {
-  return make_map(tm, out, cols * 2, rows, 2 * batch, cols * 2, rows * cols * 2, 64, 32, 1);
+int result_map(CUtensorMap *tm, const void *out, size_t planes, size_t rows, size_t cols) {
+  return make_map(tm, out, cols * 2, rows, planes, cols * 2, rows * cols * 2, 64, 32, 1);
 }
 
 // X as an operand: contracted over the long side in S, over the short side in the update.
@@ -1254,13 +1261,15 @@ Operand square_operand(const ccglib_b200_orthogonalize_plan &plan, const __half 
 }
 
 int make_maps(ccglib_b200_orthogonalize_plan &plan) {
-  const size_t batch = plan.desc.batch;
-  const Operand s = square_operand(plan, plan.s), p = square_operand(plan, plan.p);
-  int rc = operand_map(&plan.s_a, s, batch, kBlockM);
-  if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.s_b, s, batch, plan.poly.bn);
+  const size_t batch = plan.desc.batch, planes = 4 * batch;
+  const Operand s = square_operand(plan, plan.s), t = square_operand(plan, plan.t),
+                p = square_operand(plan, plan.p);
+  int rc = operand_map(&plan.poly_a, t, batch, kBlockM);
+  if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.poly_b, s, batch, plan.poly.bn);
   if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.update_p, p, batch, plan.tall ? plan.update.bn : kBlockM);
-  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.s_out, plan.s, batch, plan.n, plan.n_p);
-  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.p_out, plan.p, batch, plan.n, plan.n_p);
+  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.s_out, plan.s, planes, plan.n, plan.n_p);
+  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.t_out, plan.t, planes, plan.n, plan.n_p);
+  if (rc == CCGLIB_B200_OK) rc = result_map(&plan.p_out, plan.p, planes, plan.n, plan.n_p);
   for (int i = 0; i < 2; ++i) {
     const Operand x_long = x_operand(plan, i, true), x_short = x_operand(plan, i, false);
     if (rc == CCGLIB_B200_OK) rc = operand_map(&plan.gram_a[i], x_long, batch, kBlockM);
@@ -1268,7 +1277,7 @@ int make_maps(ccglib_b200_orthogonalize_plan &plan) {
     if (rc == CCGLIB_B200_OK) {
       rc = operand_map(&plan.update_x[i], x_short, batch, plan.tall ? kBlockM : plan.update.bn);
     }
-    if (rc == CCGLIB_B200_OK) rc = result_map(&plan.x_out[i], plan.x[i], batch, plan.desc.m, plan.cols_p);
+    if (rc == CCGLIB_B200_OK) rc = result_map(&plan.x_out[i], plan.x[i], planes, plan.desc.m, plan.cols_p);
   }
   return rc;
 }
@@ -1287,10 +1296,8 @@ int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q,
   g.hermitian = q.hermitian ? 1u : 0u;
   g.conj_b = q.conj ? 1u : 0u;
   g.alpha = q.alpha;
-  g.beta = q.beta;
-  g.gain = q.gain;
-  g.c0 = q.c0;
-  g.c0_pitch = static_cast<uint32_t>(q.c0_pitch);
+  g.diag = q.diag;
+  g.pair = q.pair ? 1u : 0u;
   g.bf16 = q.bf16 ? 1u : 0u;
   g.boxes = q.boxes ? 1u : 0u;
   g.out = static_cast<uint16_t *>(q.out);
@@ -1334,6 +1341,51 @@ int launch_first(const ccglib_b200_orthogonalize_plan &plan, const void *d_in, c
                        d.n % 8 == 0 && aligned16(d_in), grid, stream);
   CCGLIB_CUDA_TRY(cudaGetLastError());
   return CCGLIB_B200_OK;
+}
+
+// 2^e, |e| at most 14, that takes `bound` to 2^13 .. 2^14 (to 2^14 at most where it is large).
+float scale_for(double bound) {
+  if (!(bound > 0.0)) return 1.0f;
+  const double e = std::floor(14.0 - std::log2(bound));
+  return static_cast<float>(std::exp2(e > 14.0 ? 14.0 : e < -14.0 ? -14.0 : e));
+}
+
+// Powers of two that keep the iterates inside float16: the entries of a Hermitian matrix are bounded by
+// its largest eigenvalue, and the largest singular value in any step follows from the map (1.0001 and 1.1:
+// what the points miss and rounding adds).
+void choose_scales(ccglib_b200_orthogonalize_plan &plan) {
+  const double a = plan.desc.a, b = plan.desc.b, c = plan.desc.c;
+  constexpr int kPoints = 512;
+  double top = 1.0, most = 1.0;
+  for (int step = 0; step < plan.desc.steps && most < 1e6; ++step) {
+    double next = 0.0;
+    for (int i = 1; i <= kPoints; ++i) {
+      const double v = top * i / kPoints, q = v * v;
+      next = std::fmax(next, std::fabs(v * (a + b * q + c * q * q)));
+    }
+    top = 1.0001 * next;
+    most = std::fmax(most, top);
+  }
+  plan.form = c == 0.0 ? kLinear : kSquare;
+  if (plan.form == kSquare) {
+    plan.shift = static_cast<float>(b / (2.0 * c));
+    const double largest = std::fmax(std::fabs(a), std::fmax(std::fabs(b), std::fabs(c)));
+    // (the negation catches an infinite quotient too)
+    if (!(std::fabs(c) * plan.shift * plan.shift <= 8.0 * largest)) plan.form = kProduct;
+  }
+  if (plan.form != kSquare) plan.shift = 0.0f;
+  double s = 0.0, t = 0.0, p = 0.0;
+  for (int i = 0; i <= kPoints; ++i) {
+    const double q = most * most * i / kPoints;
+    s = std::fmax(s, std::fabs(q + plan.shift));
+    t = std::fmax(t, std::fabs(b + c * q));
+    p = std::fmax(p, std::fabs(a + b * q + c * q * q));
+  }
+  plan.s_scale = scale_for(1.1 * s);
+  plan.t_scale = scale_for(1.1 * t);
+  plan.p_scale = scale_for(1.1 * p);
+  // entries near one where the rows (columns) are orthonormal
+  plan.scale = std::exp2(std::rint(0.5f * std::log2(static_cast<float>(plan.l))));
 }
 
 } // namespace
@@ -1385,7 +1437,7 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.l = plan.tall ? d.m : d.n;
   plan.n_p = ceil_div<size_t>(plan.n, 8) * 8;
   plan.cols_p = ceil_div<size_t>(d.n, 8) * 8;
-  plan.scale = std::exp2(std::rint(0.5f * std::log2(static_cast<float>(plan.l))));
+  choose_scales(plan);
   CCGLIB_CUDA_TRY(cudaGetDevice(&plan.device));
   plan.sms = sm_count();
   if (plan.sms <= 0) return CCGLIB_B200_CUDA_ERROR;
@@ -1402,13 +1454,11 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   plan.poly = pick_shape(d.batch, plan.n, plan.n_p, plan.n, true, plan.sms);
   plan.update = pick_shape(d.batch, d.m, plan.cols_p, plan.n, false, plan.sms);
   // One launch (with how many CTAs per matrix), or three launches per step?  Estimates in microseconds
-  // per step, within 40 % of what the forms take on short sides 1 .. 64, long sides to 1600, batches to
-  // 1024: 64 x 64 x 64 150 us in one launch against 95 for five steps, 16 x 32 x 1024 92 against 211.
+  // per step.  On short sides 1 .. 64, long sides 1 .. 4000 and batches 1, 64 and 1024 the choice is within
+  // 26 % of the best form, in nine of ten cases within 6 % (33 x 400 x 64, five steps: 128 us in one launch,
+  // 188 in three; 64 x 64: 155 and 136).
   const size_t sms = static_cast<size_t>(plan.sms);
-  const double waves = static_cast<double>(ceil_div(d.batch * plan.gram.per_batch, sms)) +
-                       static_cast<double>(ceil_div(d.batch * plan.poly.per_batch, sms)) +
-                       static_cast<double>(ceil_div(d.batch * plan.update.per_batch, sms));
-  double least = 3 * 4.8 + 2.5 * (waves - 3.0);
+  double least = 3 * 1.5 + (plan.gram.clocks + plan.poly.clocks + plan.update.clocks) / 1900.0;
   // CCGLIB_B200_ORTH_SMALL: 0 for three launches, 1, 2, 4 or 8 for one with so many CTAs (where it fits)
   const char *env = std::getenv("CCGLIB_B200_ORTH_SMALL");
   const int forced = env != nullptr && *env != '\0' ? std::atoi(env) : -1;
@@ -1438,6 +1488,10 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     }
     return CCGLIB_B200_OK;
   }
+  if (d.batch > 0x1FFFFFFFull) {  // 32-bit signed plane coordinates in the TMA unit
+    set_last_error("orthogonalize_plan_create: dimension too large");
+    return CCGLIB_B200_INVALID_ARGUMENT;
+  }
   if (d.batch * plan.gram.per_batch > 0x7FFFFFFFull ||
       d.batch * plan.poly.per_batch > 0x7FFFFFFFull ||
       d.batch * plan.update.per_batch > 0x7FFFFFFFull) {
@@ -1452,9 +1506,10 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
     }
   }
   plan.chunks = ceil_div<size_t>(2 * d.m * d.n, kNormChunk);
-  const size_t x_bytes = ceil_div<size_t>(d.batch * 2 * d.m * plan.cols_p * 2, 256) * 256;
-  const size_t s_bytes = ceil_div<size_t>(d.batch * 2 * plan.n * plan.n_p * 2, 256) * 256;
-  plan.scratch_bytes = 2 * x_bytes + 2 * s_bytes + d.batch * plan.chunks * sizeof(double);
+  const size_t x_bytes = ceil_div<size_t>(d.batch * 4 * d.m * plan.cols_p * 2, 256) * 256;
+  const size_t s_bytes = ceil_div<size_t>(d.batch * 4 * plan.n * plan.n_p * 2, 256) * 256;
+  const size_t squares = plan.form == kSquare ? 2 : plan.form == kLinear ? 1 : 3;
+  plan.scratch_bytes = 2 * x_bytes + squares * s_bytes + d.batch * plan.chunks * sizeof(double);
   if (cudaMalloc(&plan.scratch, plan.scratch_bytes) != cudaSuccess) {
     cudaGetLastError();
     set_last_error("orthogonalize_plan_create: could not allocate %zu bytes of workspace",
@@ -1469,8 +1524,10 @@ extern "C" int ccglib_b200_orthogonalize_plan_create(const ccglib_b200_orthogona
   };
   plan.x[0] = reinterpret_cast<__half *>(take(x_bytes));
   plan.x[1] = reinterpret_cast<__half *>(take(x_bytes));
-  plan.s = reinterpret_cast<__half *>(take(s_bytes));
+  // (what a form has no use for stands for the array that it is not)
   plan.p = reinterpret_cast<__half *>(take(s_bytes));
+  plan.s = plan.form == kLinear ? plan.p : reinterpret_cast<__half *>(take(s_bytes));
+  plan.t = plan.form == kProduct ? reinterpret_cast<__half *>(take(s_bytes)) : plan.s;
   plan.sums = reinterpret_cast<double *>(at);
   rc = make_maps(plan);
   if (rc != CCGLIB_B200_OK) {
@@ -1555,32 +1612,48 @@ extern "C" int ccglib_b200_orthogonalize_run(ccglib_b200_orthogonalize_plan *pla
                                               : launch_first<__nv_bfloat16>(*plan, d_in, stream);
   const size_t n = plan->n, n_p = plan->n_p, cols_p = plan->cols_p;
   const bool tall = plan->tall;
-  const float unscale = 1.0f / (plan->scale * plan->scale);
+  const float s_scale = plan->s_scale, t_scale = plan->t_scale, p_scale = plan->p_scale;
   for (int step = 0; rc == CCGLIB_B200_OK && step < d.steps; ++step) {
     const bool last = step + 1 == d.steps;
     const int now = step & 1;
     const Operand x_long = x_operand(*plan, now, true), x_short = x_operand(*plan, now, false);
-    const Operand s = square_operand(*plan, plan->s), p = square_operand(*plan, plan->p);
-    rc = launch_product(*plan, {x_long, x_long, &plan->gram_a[now], &plan->gram_b[now], &plan->s_out, n, n_p,
-                                plan->gram, true, true, unscale, 0.0f, 1.0f, nullptr, 0, plan->s, n_p,
-                                true, false}, stream);
+    const Operand s = square_operand(*plan, plan->s), t = square_operand(*plan, plan->t),
+                  p = square_operand(*plan, plan->p);
+    // the Gram product X X^H as alpha S + diag I
+    const auto gram = [&](const CUtensorMap *out, float alpha, float diag) {
+      return launch_product(*plan, {x_long, x_long, &plan->gram_a[now], &plan->gram_b[now], out, n, n_p, plan->gram,
+                                    true, true, alpha / (plan->scale * plan->scale), diag, true}, stream);
+    };
+    if (plan->form == kLinear) {
+      rc = gram(&plan->p_out, p_scale * d.b, p_scale * d.a);
+    } else {
+      rc = gram(&plan->s_out, s_scale, s_scale * plan->shift);
+      float alpha = p_scale / (s_scale * s_scale) * d.c;
+      double diag = d.a - static_cast<double>(d.c) * plan->shift * plan->shift;
+      if (rc == CCGLIB_B200_OK && plan->form == kProduct) {
+        rc = gram(&plan->t_out, t_scale * d.c, t_scale * d.b);
+        alpha = p_scale / (s_scale * t_scale);
+        diag = d.a;
+      }
+      if (rc != CCGLIB_B200_OK) break;
+      rc = launch_product(*plan, {t, s, &plan->poly_a, &plan->poly_b, &plan->p_out, n, n_p, plan->poly, true, true,
+                                  alpha, static_cast<float>(p_scale * diag), true}, stream);
+    }
     if (rc != CCGLIB_B200_OK) break;
-    rc = launch_product(*plan, {s, s, &plan->s_a, &plan->s_b, &plan->p_out, n, n_p, plan->poly, true, true,
-                                d.c, d.b, 1.0f, plan->s, n_p, plan->p, n_p, true, false}, stream);
-    if (rc != CCGLIB_B200_OK) break;
+    // X = P X
     const CUtensorMap *tm_x = &plan->update_x[now], *tm_p = &plan->update_p;
     Product update{tall ? x_short : p, tall ? p : x_short, tall ? tm_x : tm_p, tall ? tm_p : tm_x,
-                   &plan->x_out[now ^ 1], d.m, cols_p, plan->update, false, false, 1.0f, d.a, 1.0f,
-                   plan->x[now], cols_p, plan->x[now ^ 1], cols_p, true, false};
+                   &plan->x_out[now ^ 1], d.m, cols_p, plan->update, false, false, 1.0f / p_scale, 0.0f, true};
     CUtensorMap tm_out;
     if (last) {
-      update.gain = 1.0f / plan->scale;
+      update.alpha = 1.0f / (p_scale * plan->scale);
+      update.pair = false;
       update.out = d_out;
       update.out_pitch = d.n;
       update.boxes = d.n % 8 == 0 && aligned16(d_out);
       update.bf16 = d.type_out == CCGLIB_B200_BFLOAT16;
       if (update.boxes) {
-        rc = result_map(&tm_out, d_out, d.batch, d.m, d.n);
+        rc = result_map(&tm_out, d_out, 2 * d.batch, d.m, d.n);
         if (rc != CCGLIB_B200_OK) break;
         update.tm_c = &tm_out;
       }

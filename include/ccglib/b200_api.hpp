@@ -365,7 +365,7 @@ namespace orthogonalize {
 struct Coefficients {
   float a, b, c;
 };
-// Steep at zero; five steps bring the singular values of any full-rank matrix to about 0.7 .. 1.2.
+// Steep at zero; five steps bring singular values of 1.5e-3 of the Frobenius norm and more to 0.65 .. 1.21.
 constexpr Coefficients quintic{3.4445f, -4.7750f, 2.0315f};
 // Newton-Schulz of fifth order: converges to orthonormal rows (columns).
 constexpr Coefficients convergent{1.875f, -1.25f, 0.375f};

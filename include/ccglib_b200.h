@@ -248,17 +248,19 @@ CCGLIB_B200_API int ccglib_b200_scaled_gemm_plan_tile(const ccglib_b200_scaled_g
  *   X <- X / ||X||_F,  then `steps` times on the shorter side (M <= N: S = X X^H, else S = X^H X)
  *   X <- a X + (b S + c S^2) X     (M > N: X <- a X + X (b S + c S^2)),
  * which keeps the singular vectors and maps every singular value s to s (a + b s^2 + c s^4).  The
- * coefficients (3.4445, -4.7750, 2.0315) take any full-rank matrix to singular values of about
- * 0.7 .. 1.2 in five steps; (15/8, -5/4, 3/8) converge to 1: orthonormal rows (columns), e.g. a
- * set of beam weights or the basis of a subspace iteration.  A zero matrix stays zero; a NaN or an
- * infinity makes its own matrix NaN.
+ * coefficients (3.4445, -4.7750, 2.0315) take singular values of at least 1.5e-3 of the Frobenius norm to
+ * 0.65 .. 1.21 in five steps (4.2e-4 in six, 1.3e-4 in seven); smaller ones grow by up to 3.4445 per
+ * step (1e-4 ends at 0.05 after five).  (15/8, -5/4, 3/8) converge to 1, growing small ones by 15/8 per
+ * step: orthonormal rows (columns), e.g. a set of beam weights or the basis of a subspace iteration.  A
+ * zero matrix stays zero; a NaN or an infinity makes its own matrix NaN.
  *
  * Input planar [batch][2][M][N] or interleaved [batch][M][N][2], float16, bfloat16 or float32; output
  * planar [batch][2][M][N], float16 or bfloat16: an operand of the GEMM or input of the quantiser.
- * Norms are float64, sums float32; between the products X, S and P are float16 (rms error of the
- * result 1 to 2.5e-3 after 5 to 8 steps).  Results do not depend on timing.  In place (d_out ==
- * d_in) is allowed where input and output have the same type and the input is planar; any other
- * overlap of the two arrays is refused.
+ * Norms are float64, sums float32; between the products X, S and P are float32 (short sides up to 64,
+ * where that is faster) or pairs of float16 of about 20 bits: the error of the result is that of its
+ * rounding to the output type (2.1e-4 float16, 1.7e-3 bfloat16, relative).  Results do not depend on
+ * timing.  In place (d_out == d_in) is allowed where input and output have the same type and the input is
+ * planar; any other overlap of the two arrays is refused.
  * No counterpart in the reference.
  */
 typedef struct ccglib_b200_orthogonalize_desc {

@@ -60,3 +60,45 @@ def test_rank_deficient(m, n):
     got = _complex(_run(plan, x, F32, F16, capi.PLANAR))[0]
     want, bound, _ = _iterate(_complex(x)[0], 4, CONVERGENT)
     assert _fro(got - want) <= bound + 2.0 ** -11 * _fro(want) + 2.0 ** -24 * np.sqrt(want.size)
+
+
+@pytest.mark.parametrize("coefficients", [
+    (1.5, -0.5, 0.0),       # third order: no square
+    (1.5, -0.5, 0.001),     # its square would cancel
+    (1.0, 0.0, 0.0),        # the matrix over its norm
+    (2.0, -1.5, 0.5), (3.0, -3.2, 1.2), (0.5, 0.25, -0.125), (0.0, 0.0, 1.0),
+    (20.0, -160.0, 300.0),  # entries of P far above one
+])
+@pytest.mark.parametrize("m, n", [(24, 60), (130, 300), (300, 130), (200, 200)])
+def test_coefficients(m, n, coefficients):
+    """Every way in which a I + b S + c S^2 is computed."""
+    rng = np.random.default_rng(64)
+    # (the last map would take three steps past float32: its results are no float16 either way)
+    for steps in (1, 3) if coefficients[0] < 20 else (1,):
+        x = _input(rng, 2, m, n, F32)
+        plan = capi.OrthogonalizePlan(2, m, n, F32, F16, steps, coefficients)
+        _check(x, _run(plan, x, F32, F16, capi.PLANAR), steps, coefficients, F16)
+
+
+# A rounding is off by at most half a step, 2^-11 (float16) or 2^-8 (bfloat16) of the value, and evenly
+# distributed up to that: rms at most 1 / sqrt(3) of it, relative to the Frobenius norm.  10 % on top are for the
+# iteration, whose iterates have about 20 bits: roundings of 2^-21 in X, S and P, which eight steps
+# multiply by less than 20 (single float16 iterates, 2^-12, end at 3.8e-3 at most), are 1e-5, and add to the
+# output's as squares.
+@pytest.mark.parametrize("type_in, type_out, half_step", [(F32, F16, 2.0 ** -11), (F16, F16, 2.0 ** -11),
+                                                          (F32, BF16, 2.0 ** -8)])
+@pytest.mark.parametrize("batch, m, n, steps, coefficients", [
+    (1, 256, 1024, 8, CONVERGENT), (2, 1024, 256, 8, CONVERGENT), (1, 256, 256, 5, QUINTIC),
+    (1, 400, 420, 8, QUINTIC), (1, 200, 2000, 8, QUINTIC), (3, 40, 72, 8, QUINTIC)])
+def test_the_output_rounding_is_what_is_lost(batch, m, n, steps, coefficients, type_in, type_out, half_step):
+    """The result is as near as its type allows, in every form, whatever the input's type."""
+    rng = np.random.default_rng(65)
+    x = _input(rng, batch, m, n, type_in)
+    plan = capi.OrthogonalizePlan(batch, m, n, type_in, type_out, steps, coefficients)
+    for xi, gi in zip(_complex(x), _complex(_run(plan, x, type_in, type_out, capi.PLANAR))):
+        u, s, v = np.linalg.svd(xi, full_matrices=False)
+        s /= _fro(xi)
+        for _ in range(steps):
+            s = s * (coefficients[0] + coefficients[1] * s ** 2 + coefficients[2] * s ** 4)
+        want = (u * s) @ v
+        assert _fro(gi - want) <= 1.1 * half_step / np.sqrt(3) * _fro(want)
