@@ -56,6 +56,7 @@ struct OrthParams {
   uint32_t n_out;
   unsigned int *status;
   long long wait_cycles;
+  long long tile_cycles;  // limit of the wait for a tile's sums, all of K
 };
 
 template <int BN> struct OrthCfg {
@@ -444,7 +445,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap tm_a,
       const TileCoord t = orth_tile<BN>(p, tile);
       const uint32_t m0 = t.mt * kBlockM + quad * 32;
       bool ok = mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.status,
-                          kDevTimeoutEpilogue, p.wait_cycles);
+                          kDevTimeoutEpilogue, p.tile_cycles);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((quad * 32) << 16) + acc * C::kAccCols;
@@ -575,7 +576,7 @@ orth_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     }
   } else {
     wait_for_previous();
-    done = mbar_wait(bar_acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue, p.wait_cycles);
+    done = mbar_wait(bar_acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue, p.tile_cycles);
     done = __all_sync(0xFFFFFFFFu, done);
   }
   __syncwarp();
@@ -1304,6 +1305,8 @@ int launch_product(const ccglib_b200_orthogonalize_plan &plan, const Product &q,
   g.n_out = static_cast<uint32_t>(q.out_pitch);
   g.status = plan.status;
   g.wait_cycles = plan.wait_cycles;
+  // a block takes about a thousand clocks: K of 1e8 values would come near the default limit by itself
+  g.tile_cycles = plan.wait_cycles + 8192ll * kPasses * g.k_blocks;
   unsigned grid = g.num_tiles < static_cast<uint32_t>(plan.sms) ? g.num_tiles : plan.sms;
   if (q.shape.split > 1) grid = g.num_tiles * q.shape.split;  // one cluster per tile
   CCGLIB_CUDA_TRY(launch_programmatic(

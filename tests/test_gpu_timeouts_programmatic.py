@@ -48,3 +48,20 @@ def test_limit_shorter_than_the_kernel_before(m, n, monkeypatch):
     assert torch.equal(c, want)
     # 1.0 x 1.0 summed: Re = k - k, Im = 2 k, exact in float32
     assert not long_c[:, 0].any() and (long_c[:, 1] == 2 * k_long).all()
+
+
+def test_limit_shorter_than_a_long_tile(monkeypatch):
+    """The sums of a tile take as long as its K: that is not a wait that has gone wrong."""
+    import torch
+
+    monkeypatch.setenv("CCGLIB_B200_ORTH_SMALL", "0")
+    rng = np.random.default_rng(42)
+    x = torch.from_numpy(rng.standard_normal((1, 2, 300_000, 48))).float().cuda()
+    out = [torch.empty((1, 2, 300_000, 48), dtype=torch.float16, device="cuda") for _ in range(2)]
+    for i, limit in enumerate(("", "400000")):
+        monkeypatch.setenv("CCGLIB_B200_WAIT_CYCLES", limit)
+        plan = capi.OrthogonalizePlan(1, 300_000, 48, F32, capi.FLOAT16, 2)
+        plan.run(x.data_ptr(), out[i].data_ptr(), gu.stream_handle())
+        torch.cuda.synchronize()
+        gu.check_device_status()
+    assert torch.equal(*out) and out[0].any()
