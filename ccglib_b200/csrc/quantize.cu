@@ -16,8 +16,9 @@
 //
 // Memory-bound: every input byte is read once, every output byte written once, the block lives in
 // registers between its maximum and its rounding.  K contiguous, float32 interleaved 4 x 4096 x 16384:
-// 445 to 465 us for 2.69 GB, 5.8 to 6.0 TB/s.  Rows contiguous, bfloat16 3 x 5003 x 4001 (odd: two-byte
-// loads): 111 us for 0.36 GB, 3.2 TB/s, bound by issuing and waiting for those loads.
+// 445 to 467 us for 2.69 GB, 5.8 to 6.0 TB/s.  Rows contiguous, bfloat16 3 x 5003 x 4001: 111 us for
+// 0.36 GB, 3.2 TB/s, bound by issuing and waiting for its loads, which are two bytes wide for planar 16-bit
+// input of any size and alignment (a lane reads one row of one k).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

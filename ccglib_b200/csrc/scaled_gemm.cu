@@ -15,12 +15,12 @@
 // 1570 (a 128-column MMA reads 8 KiB of operands from shared memory beside the 64 KiB that TMA brings in
 // per block; their arithmetic alone is 1024), adding a block to the sums takes 600 of an epilogue
 // warp's time and hides behind them.  With normally distributed operands the 1 kW power cap takes the
-// clock to 1.25 .. 1.45 GHz: 1.95 to 2.06 PFLOP/s, against 2.31 of the unscaled kernel with the same
+// clock to 1.25 .. 1.45 GHz: 1.95 to 2.02 PFLOP/s, against 2.31 of the unscaled kernel with the same
 // tile and 2.69 with 256 columns.  Tried and dropped: sixteen epilogue warps (2640 clocks), packed
 // two-value arithmetic (more register moves than it saves), Re and Im handed over apart (2500).
 //
-// Either operand may be the 128-row side of the tile (the product is symmetric in A and B); the
-// plan takes the one that wastes fewer rows, so one row of A against many rows of B is a
+// Either operand may be the 128-row side of the tile (the product is symmetric in A and B): A, unless
+// it has at most 64 rows and fewer than B.  So one row of A against many rows of B is a
 // 128 x 16 tile that reads B once: memory-bound, 1 x 8192 x 8192 in 31 us (134 MB, 4.3 TB/s; a set-up of
 // 3 us and the last exchange of 2 us are in it).  Problems whose tiles do not fill the device evenly may
 // be cut into equal runs of 128-k blocks instead of whole tiles: a CTA that holds part of a tile's blocks
@@ -75,7 +75,8 @@ template <int BN> struct ScaledCfg {
   // Up to 64 columns one MMA multiplies an A plane by both B planes, which lie one behind the other in
   // the stage: columns [Ar.Br | Ar.Bi] and [Ai.Br | Ai.Bi], added up on the way out of tensor
   // memory.  An MMA of 128 rows costs the same for 64 columns as for 128, so this halves the tensor
-  // time of narrow tiles; at 128 columns there is no tensor memory for it.
+  // time of narrow tiles.  At 128 columns the four products of two buffers would be twice the tensor
+  // memory there is.
   static constexpr bool kStacked = BN <= 64;
   static constexpr int kAccCols = kStacked ? 4 * BN : 2 * BN;
   static_assert(kAccCols * kAccBuffers <= kTmemCols, "accumulators exceed tensor memory");
@@ -978,9 +979,9 @@ extern "C" int ccglib_b200_scaled_gemm_plan_create(const ccglib_b200_scaled_gemm
   env = std::getenv("CCGLIB_B200_SCALED_RUNS");
   const int forced_runs = env != nullptr && *env != '\0' ? std::atoi(env) : -1;
   // Whole tiles, or all blocks in equal runs?  And 128 or 64 columns where there is a choice?  Estimated
-  // in clocks; on 16 shapes from 256 x 256 x 256 to 4096 x 4096 x 4096 the choice is within 6 % of the
-  // best of the four forms (1024 x 1024 x 1024: 10.4 us, the others 13 to 18; 256 x 256 x 4096: 16.7,
-  // the others 23 to 32; 2048 x 2048 x 2048: 38, the others 49 to 53).
+  // in clocks; on 16 shapes from 256 x 256 x 256 to 4096 x 4096 x 4096 the choice is within 4 % of the
+  // best of the four forms (1024 x 1024 x 1024: 11.0 us, the others 13.6 to 18.8; 256 x 256 x 4096: 17.5,
+  // the others 24 to 32; 2048 x 2048 x 2048: 39, the others 52 to 59).
   const size_t col_block = plan.swapped ? d.a_block_rows : d.b_block_rows;
   double least = 0.0;
   for (int bn : {128, 64, 32, 16}) {
