@@ -13,16 +13,16 @@
 // layout.  The launches are programmatic: a product's CTAs set up while the one before it drains.
 //
 // X, S and P are states of the iteration and are kept as pairs of float16, the rounded value and what the
-// rounding leaves (X times a power of two near sqrt(long side), S and P times powers of two that keep them
-// inside float16): about 20 bits.  A product takes its K three times, low x high, high x low and high x
+// rounding leaves, times powers of two that put their largest possible entries near the top of float16
+// (choose_scales): about 20 bits, also in rows fainter than the others by several decades.  A product takes its K three times, low x high, high x low and high x
 // high, into the same float32 sums.  What is lost in the end is the rounding of the output (relative
 // error 2.1e-4 float16, 1.7e-3 bfloat16).  Single float16 iterates take a third of the multiplications, but
 // a step's roundings do not decay, those that turn the singular vectors least of all: they ended at 7e-4
 // after eight steps that converge and at 1.4 to 3.8e-3 after 5 to 8 of the steep quintic.  Leaving out one
 // of the low halves (of X in S, of S, of P) still ends at 5e-4 to 3e-3.
 //
-// Measured: 8 x 4096 x 1024, eight steps, 9.8 ms (1.09 PFLOP/s in the three passes over K, power-capped);
-// 1024 x 1024, five steps, 344 us (23 us a product of 1024^3 in three passes: operands on their way from L2
+// Measured: 8 x 4096 x 1024, eight steps, 9.8 to 10.1 ms (1.07 PFLOP/s in the three passes over K,
+// power-capped); 1024 x 1024, five steps, 344 to 353 us (23 us a product of 1024^3 in three passes: operands on their way from L2
 // into 144 SMs, and two latencies).  Single float16: 3.5 ms and 182 us.
 #include <cmath>
 #include <cstdlib>
@@ -1199,10 +1199,9 @@ struct ccglib_b200_orthogonalize_plan {
   size_t n, l;          // short and long side
   size_t n_p, cols_p;   // row pitches of S and P, and of X: multiples of eight
   bool tall;            // m > n
-  float scale;          // power of two near sqrt(long side): X is kept times this
   PolyForm form;
   float shift;          // kSquare: b / 2c
-  float s_scale, t_scale, p_scale;  // powers of two that S (+ shift I), T and P are kept times
+  float scale, s_scale, t_scale, p_scale;  // powers of two that X, S (+ shift I), T and P are kept times
   ProductShape gram, poly, update;
   uint32_t small;       // > 0: the whole iteration in one launch, so many CTAs per matrix
   size_t chunks;
@@ -1353,8 +1352,8 @@ float scale_for(double bound) {
   return static_cast<float>(std::exp2(e > 14.0 ? 14.0 : e < -14.0 ? -14.0 : e));
 }
 
-// Powers of two that keep the iterates inside float16: the entries of a Hermitian matrix are bounded by
-// its largest eigenvalue, and the largest singular value in any step follows from the map (1.0001 and 1.1:
+// Powers of two that keep the iterates inside float16 and as far from its smallest values as that allows: no
+// entry of a matrix exceeds its largest singular value, and the largest in any step follows from the map (1.0001 and 1.1:
 // what the points miss and rounding adds).
 void choose_scales(ccglib_b200_orthogonalize_plan &plan) {
   const double a = plan.desc.a, b = plan.desc.b, c = plan.desc.c;
@@ -1387,8 +1386,7 @@ void choose_scales(ccglib_b200_orthogonalize_plan &plan) {
   plan.s_scale = scale_for(1.1 * s);
   plan.t_scale = scale_for(1.1 * t);
   plan.p_scale = scale_for(1.1 * p);
-  // entries near one where the rows (columns) are orthonormal
-  plan.scale = std::exp2(std::rint(0.5f * std::log2(static_cast<float>(plan.l))));
+  plan.scale = scale_for(1.1 * most);
 }
 
 } // namespace

@@ -50,6 +50,32 @@ def test_weak_directions(m, n, steps, coefficients):
     assert _fro(gi - want) <= bound + 2.0 ** -11 * _fro(want) + 2.0 ** -24 * np.sqrt(want.size)
 
 
+@pytest.mark.parametrize("m, n", [(40, 300), (200, 1024), (1024, 200), (160, 160)])
+@pytest.mark.parametrize("decades", [3, 5])
+def test_rows_of_different_levels(m, n, decades):
+    """Antennas with gains over several decades: faint rows keep their bits beside strong ones (a row's
+    error is measured against that row)."""
+    import torch
+
+    rng = np.random.default_rng(66)
+    gain = 10.0 ** -np.linspace(0, decades, min(m, n))
+    gain = gain[:, None] if m <= n else gain[None, :]
+    x = torch.from_numpy(rng.standard_normal((1, 2, m, n)) * gain).float()
+    plan = capi.OrthogonalizePlan(1, m, n, F32, BF16, 3, CONVERGENT)  # (bfloat16: faint rows of the result too)
+    xi, gi = (_complex(v)[0] for v in (x, _run(plan, x, F32, BF16, capi.PLANAR)))
+    u, s, v = np.linalg.svd(xi, full_matrices=False)
+    s /= _fro(xi)
+    for _ in range(3):
+        s = s * (CONVERGENT[0] + CONVERGENT[1] * s ** 2 + CONVERGENT[2] * s ** 4)
+    want = (u * s) @ v
+    if m > n:
+        want, gi = want.T, gi.T
+    error = np.linalg.norm(gi - want, axis=1) / np.linalg.norm(want, axis=1)
+    # half a step of bfloat16 at most, rms 1 / sqrt(3) of that; entries of one row differ little, so a row of n
+    # has rms within 10 % of the expected one; the iteration may add a fifth of it
+    assert (error <= 1.1 * 1.02 * 2.0 ** -8 / np.sqrt(3)).all(), error.max()
+
+
 @pytest.mark.parametrize("m, n", [(24, 60), (130, 300)])
 def test_rank_deficient(m, n):
     """Directions that are not there stay out: rank 5, the rest rounding noise below float16's of X."""
