@@ -14,16 +14,17 @@
 //
 // X, S and P are states of the iteration and are kept as pairs of float16, the rounded value and what the
 // rounding leaves, times powers of two that put their largest possible entries near the top of float16
-// (choose_scales): about 20 bits, also in rows fainter than the others by several decades.  A product takes its K three times, low x high, high x low and high x
-// high, into the same float32 sums.  What is lost in the end is the rounding of the output (relative
-// error 2.1e-4 float16, 1.7e-3 bfloat16).  Single float16 iterates take a third of the multiplications, but
-// a step's roundings do not decay, those that turn the singular vectors least of all: they ended at 7e-4
-// after eight steps that converge and at 1.4 to 3.8e-3 after 5 to 8 of the steep quintic.  Leaving out one
-// of the low halves (of X in S, of S, of P) still ends at 5e-4 to 3e-3.
+// (choose_scales): about 20 bits, also in rows fainter than the others by several decades.  A product
+// takes its K three times, low x high, high x low and high x high, into the same float32 sums.  What is
+// lost in the end is the rounding of the output (relative error 2.1e-4 float16, 1.7e-3 bfloat16).  Single
+// float16 iterates take a third of the multiplications, but a step's roundings do not decay, those that
+// turn the singular vectors least of all: they ended at 7e-4 after eight steps that converge and at 1.4 to
+// 3.8e-3 after 5 to 8 of the steep quintic.  Leaving out one of the low halves (of X in S, of S, of P)
+// still ends at 5e-4 to 3e-3 in the steep map.
 //
 // Measured: 8 x 4096 x 1024, eight steps, 9.8 to 10.1 ms (1.07 PFLOP/s in the three passes over K,
-// power-capped); 1024 x 1024, five steps, 344 to 353 us (23 us a product of 1024^3 in three passes: operands on their way from L2
-// into 144 SMs, and two latencies).  Single float16: 3.5 ms and 182 us.
+// power-capped); 1024 x 1024, five steps, 344 to 353 us (23 us a product of 1024^3 in three passes: operands
+// on their way from L2 into 144 SMs, and two latencies).  Single float16: 3.5 ms and 182 us.
 #include <cmath>
 #include <cstdlib>
 #include <new>
@@ -679,9 +680,9 @@ struct ProductShape {
   double clocks;  // estimated
 };
 
-// Estimated clocks: a block of K (of three passes) costs what its bytes take through the SM's port to L2 (64 KiB resp. 48 KiB,
-// 128 resp. 64 columns), a tile its epilogue (of mostly Hermitian blocks 100 per column, else 60), an
-// exchange of partial sums 60 per column.
+// Estimated clocks: a block of K (of three passes) costs what its bytes take through the SM's port to L2
+// (64 KiB resp. 48 KiB, 128 resp. 64 columns), a tile its epilogue (of a Hermitian result 100 per column,
+// else 60), an exchange of partial sums 60 per column.
 ProductShape pick_shape(size_t batch, size_t m, size_t n, size_t k, bool hermitian, size_t sms) {
   ProductShape best{0, 1, 0, 0.0};
   double least = 0.0;
@@ -1353,8 +1354,8 @@ float scale_for(double bound) {
 }
 
 // Powers of two that keep the iterates inside float16 and as far from its smallest values as that allows: no
-// entry of a matrix exceeds its largest singular value, and the largest in any step follows from the map (1.0001 and 1.1:
-// what the points miss and rounding adds).
+// entry of a matrix exceeds its largest singular value, and the largest in any step follows from the map
+// (1.0001 and 1.1: what the points miss and rounding adds).
 void choose_scales(ccglib_b200_orthogonalize_plan &plan) {
   const double a = plan.desc.a, b = plan.desc.b, c = plan.desc.c;
   constexpr int kPoints = 512;
