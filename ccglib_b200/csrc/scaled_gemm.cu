@@ -203,8 +203,9 @@ __device__ __forceinline__ void tmem_st_8(uint32_t taddr, const uint32_t *r) {
 //   t from 2^-126 and s 2^p from 2^-9: s 2^p t, at least 2^-135, is below the normal range only where
 //   s t < 2^-190 and d s t vanishes, and is not zero, so that an infinite sum stays infinite.  s 2^p
 //   up to 2^(l + 64) and t up to 2^l keep the sum of all blocks below 2^127 (2^l is lift_limit).
-//   A block with any other scale: scale_block writes d s t over d first (1.3 to 1.5 times the time where
-//   every block needs it).
+//   A block with any other scale: scale_block writes d s t over d first.  Where every block needs it that
+//   takes 1.1 (one row) to 1.75 times the time, in float64 (a scale above 2^63 or subnormal) 1.4 to 4.2
+//   times: 4096 x 4096 x 16384 0.91, 1.59 and 3.87 ms.
 // A power of two taken out of d in add_block instead, one multiplication per value, took 3 to 12 % more time
 // where one row in 64 is silent; this takes 0 to 4 % more than d * (s t) alone, which was wrong there.
 __host__ __device__ constexpr uint32_t exponent_bits(int e) { return static_cast<uint32_t>(127 + e) << 23; }
